@@ -241,6 +241,154 @@ SUPRA_ATTN_API int supra_attn_enqueue_linear(supra_attn_ctx* ctx, const supra_at
 /* Validates a linear descriptor as supra_attn_enqueue_linear does (pure host function). */
 SUPRA_ATTN_API int supra_attn_check_linear_desc(const supra_attn_linear_desc* desc, char* msg, int32_t cap);
 
+/* ---- norm and rotation of query and key heads ----------------------------------------------- */
+/* Element types of the buffers of the calls below. Strides and offsets count elements of the type. */
+enum { SUPRA_ATTN_T_F32 = 0, SUPRA_ATTN_T_F16 = 1, SUPRA_ATTN_T_BF16 = 2 };
+
+/* One operand of a qk_norm call: H heads of D channels in each row, head h of row i at
+ * x[x_off + i*ldx + h*D + 0..D), written to y[y_off + i*ldy + h*D + 0..D). y may be x itself with
+ * the same offset and stride (in place); otherwise they may not overlap. */
+typedef struct supra_attn_qk_operand {
+  const void* x;
+  void* y;
+  const float* w; /* D channel weights shared by the heads, or NULL (ones) */
+  int64_t x_size, y_size, w_size;
+  int64_t ldx, ldy, x_off, y_off;
+  int32_t H;
+  int32_t reserved; /* 0 */
+} supra_attn_qk_operand;
+
+/* Flags of a qk_norm call. */
+#define SUPRA_ATTN_QK_NO_NORM 0x1u     /* rotate only: no RMS norm and no weights */
+#define SUPRA_ATTN_QK_INTERLEAVED 0x2u /* pairs (2i, 2i+1) instead of (i, i + rot/2) */
+
+/* RMS norm of every head of the queries and of the keys, with the position rotation in the same
+ * pass (not in the reference, whose DiT normalises whole rows and adds its positions):
+ *   n = x / sqrt(mean(x^2) + eps) * w                    over the D channels of one head
+ *   (y_a, y_b) = (n_a cos - n_b sin, n_b cos + n_a sin)  for the rot/2 channel pairs (a, b) of
+ *                                                        the first rot channels; the others stay n
+ * with cos = turns[position*rot + i], sin = turns[position*rot + rot/2 + i] for pair i: the caller
+ * lays the table out once for its positions (n_turns rows), which may stand for one axis or for
+ * a patch grid. position = positions[row], or the row index when positions is NULL. A position
+ * outside [0, n_turns) leaves its row unwritten and is reported at sync (SUPRA_ATTN_EDEVICE).
+ * Sums and products are held in 32 bits; the result is rounded once, to `type`.
+ * 1 <= D <= 256, even; 0 <= rot <= D, even (0: no rotation, turns and positions NULL). k.H = 0:
+ * no keys. Recorded like an attention problem (same queue and hazard tracking). */
+typedef struct supra_attn_qk_norm_desc {
+  supra_attn_qk_operand q, k;
+  const float* turns;
+  const int32_t* positions;
+  int64_t turns_size, positions_size;
+  int32_t M, D, rot, n_turns;
+  int32_t type;   /* SUPRA_ATTN_T_* of x and y */
+  uint32_t flags; /* SUPRA_ATTN_QK_* */
+  float eps;
+  int32_t reserved; /* 0 */
+} supra_attn_qk_norm_desc;
+SUPRA_ATTN_API int supra_attn_enqueue_qk_norm(supra_attn_ctx* ctx, const supra_attn_qk_norm_desc* desc);
+/* Validates as supra_attn_enqueue_qk_norm does (pure host function). */
+SUPRA_ATTN_API int supra_attn_check_qk_norm_desc(const supra_attn_qk_norm_desc* desc, char* msg, int32_t cap);
+
+/* ---- the paged 8-bit K/V cache ---------------------------------------------------------------- */
+/* Keys and values of many sequences (prompts) held in 8 bits, the reference's cached FP32 K/V
+ * (app/models/dit.js:137-144, app/pipeline.js:97-117) in a quarter of the bytes. The pool is split into blocks of block_tokens tokens, and each block has one scale per head, for K and
+ * for V: value = code * scale[block*H + head]. Codes of one block and head are contiguous:
+ *   codes[((block*H + head)*block_tokens + slot)*D + channel]
+ * SUPRA_ATTN_CACHE_INT8: signed bytes in [-127, 127]; SUPRA_ATTN_CACHE_E4M3: 8-bit floats with 4
+ * exponent and 3 mantissa bits. D is a multiple of 16 up to 128, block_tokens 16, 32, 64 or 128;
+ * k and v are 16-byte aligned. All four arrays are the caller's. */
+enum { SUPRA_ATTN_CACHE_INT8 = 0, SUPRA_ATTN_CACHE_E4M3 = 1 };
+typedef struct supra_attn_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t k_size, v_size;             /* bytes, >= blocks*H*block_tokens*D */
+  int64_t k_scale_size, v_scale_size; /* floats, >= blocks*H */
+  int32_t blocks, block_tokens, H, D;
+  int32_t format;   /* SUPRA_ATTN_CACHE_* */
+  int32_t reserved; /* 0 */
+} supra_attn_cache;
+
+/* The sequences of one call. All arrays are device memory, read when the call runs: their contents
+ * may change between calls, and between replays of a captured one. Token t of sequence b sits in
+ * block table[b*ld_table + t / block_tokens], slot t % block_tokens. The call's rows (queries, or
+ * K/V rows to write or read) of sequence b are rows row_start[b] .. row_start[b+1]-1 of its
+ * operands, or b*max_rows .. (b+1)*max_rows-1 when row_start is NULL; with n rows, row i stands
+ * at token lengths[b] - n + i (lengths count the tokens that the call writes).
+ * rows bounds row_start[B] (with row_start NULL it is B*max_rows), max_rows the rows of one
+ * sequence and max_len its length; operand rows at and after row_start[B] are neither read nor
+ * written. A sequence outside these bounds is left out (its output rows stay as they are), tokens
+ * in a block outside [0, blocks) are left out, and either is reported at sync
+ * (SUPRA_ATTN_EDEVICE). Table entries past a sequence's last block are not read. */
+typedef struct supra_attn_cache_batch {
+  const int32_t* lengths;   /* B */
+  const int32_t* table;     /* B rows of ld_table block numbers */
+  const int32_t* row_start; /* B + 1, ascending, or NULL */
+  int64_t lengths_size, table_size, row_start_size;
+  int64_t rows;
+  int32_t B, ld_table;
+  int32_t max_rows, max_len;
+} supra_attn_cache_batch;
+
+/* K/V rows beside the cache: row r of the keys at k[k_off + r*ldk + h*D + 0..D), values likewise. */
+typedef struct supra_attn_cache_rows_desc {
+  supra_attn_cache cache;
+  supra_attn_cache_batch seqs;
+  void* k; /* cache_write reads them, cache_read writes them */
+  void* v;
+  int64_t k_size, v_size, ldk, ldv, k_off, v_off;
+  int32_t type;   /* SUPRA_ATTN_T_* */
+  uint32_t flags; /* 0 */
+} supra_attn_cache_rows_desc;
+
+/* Quantises rows into the cache: the last n tokens of each sequence are written, and the tokens
+ * before them in the first touched block keep their values. Per block and head, over the block's
+ * written tokens,
+ *   s = max(amax|x|, 2^-100) * (1/qmax)         qmax 127 (INT8) or 448 (E4M3)
+ *   s = max(s, old scale)                       if the block already held earlier tokens
+ *   code = nearest (ties to even) to x * (1/s); the held codes become the nearest to
+ *   code * (old scale / s) when the scale grew
+ * s, 1/qmax, 1/s and the ratio are fp32; each product is rounded once, to the code. A value that is not
+ * finite makes its block's scale NaN (and its codes 0): the block then reads as NaN. Slots after a
+ * sequence's last token keep their bytes and stand for nothing. Blocks written by one call have to
+ * be distinct: a block given to two written tokens ranges of one call gets unspecified values. */
+SUPRA_ATTN_API int supra_attn_enqueue_cache_write(supra_attn_ctx* ctx, const supra_attn_cache_rows_desc* desc);
+SUPRA_ATTN_API int supra_attn_check_cache_write_desc(const supra_attn_cache_rows_desc* desc, char* msg, int32_t cap);
+/* Reads the last n tokens of each sequence back: code * scale, rounded to `type`. */
+SUPRA_ATTN_API int supra_attn_enqueue_cache_read(supra_attn_ctx* ctx, const supra_attn_cache_rows_desc* desc);
+SUPRA_ATTN_API int supra_attn_check_cache_read_desc(const supra_attn_cache_rows_desc* desc, char* msg, int32_t cap);
+
+/* Flags of a cache_attention call. */
+#define SUPRA_ATTN_CA_DEFAULT_SCALE 0x1u /* ignore .scale, use 1/sqrt(D) */
+#define SUPRA_ATTN_CA_CAUSAL 0x2u        /* row i of n sees tokens 0 .. length - n + i */
+
+/* Attention of query rows over the cache: softmax(scale * q k^T) v per head, over the sequence's
+ * tokens (causal: up to the row's own token). H query heads, a multiple of cache.H: heads
+ * g*H/cache.H .. (g+1)*H/cache.H-1 read the cache's head g. Row r, head h of the queries at
+ * q[q_off + r*ldq + h*D], of the result at out[o_off + r*ldo + h*D]. A row that sees no token
+ * (an empty sequence, or a causal row before the first token) is 0. The codes enter the products
+ * exactly; scores, softmax statistics and the sums over tokens are held in 32 bits, and
+ * SUPRA_ATTN_T_F32 requests keep FP32 accuracy (queries and probabilities as two 16-bit parts). */
+typedef struct supra_attn_cache_attn_desc {
+  supra_attn_cache cache;
+  supra_attn_cache_batch seqs;
+  const void* q;
+  void* out;
+  int64_t q_size, out_size, ldq, ldo, q_off, o_off;
+  int32_t H;
+  int32_t type; /* SUPRA_ATTN_T_* of q and out */
+  float scale;
+  uint32_t flags; /* SUPRA_ATTN_CA_* */
+} supra_attn_cache_attn_desc;
+SUPRA_ATTN_API int supra_attn_enqueue_cache_attention(supra_attn_ctx* ctx, const supra_attn_cache_attn_desc* desc);
+SUPRA_ATTN_API int supra_attn_check_cache_attention_desc(const supra_attn_cache_attn_desc* desc, char* msg,
+                                                         int32_t cap);
+/* The launches of these four calls take their descriptors as kernel arguments and use no memory of
+ * the context but its status word, so a flush of them alone (profiling off) may be captured into a
+ * CUDA graph on the context's stream, and graphs captured from one context may run at the same time
+ * where their own operands allow it. */
+
 /* ---- profiling (the reference's Profiler, app/gpu/device.js:91-99,222-233,272-325) -------- */
 /* When on, every grouped launch is bracketed by CUDA events on the launching stream and
  * aggregated by kernel name with its algorithmic FLOPs (4*Lq*Lk*D*H, app/gpu/ops.js:116) and

@@ -1,0 +1,179 @@
+// Device helpers shared by the kernels of the paged 8-bit K/V cache and the query/key norm: element
+// types, the cache's codes, and the bounds of a call's sequences.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace supra {
+
+// ---- element types ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Two values as one 32-bit word of a 16-bit type, the first in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t u);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+
+// N consecutive elements (N * sizeof(T) a multiple of 16). VEC: p is 16-byte aligned.
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void load_row(const T* p, float (&x)[N]) {
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_f32<T>(p[i]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + i);
+      x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 8) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + i);
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack2<T>(u[k]);
+        x[i + 2 * k] = f.x, x[i + 2 * k + 1] = f.y;
+      }
+    }
+  }
+}
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void store_row(T* p, const float (&x)[N]) {
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = from_f32<T>(x[i]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 8) {
+      uint4 v;
+      v.x = pack2<T>(x[i], x[i + 1]), v.y = pack2<T>(x[i + 2], x[i + 3]);
+      v.z = pack2<T>(x[i + 4], x[i + 5]), v.w = pack2<T>(x[i + 6], x[i + 7]);
+      *reinterpret_cast<uint4*>(p + i) = v;
+    }
+  }
+}
+
+// ---- the cache's codes -----------------------------------------------------------------------
+template <int FMT>
+constexpr float kQmax = FMT == kCacheInt8 ? 127.f : 448.f;
+constexpr float kAmaxFloor = 7.8886090522101181e-31f;  // 2^-100: keeps 1 / scale finite
+
+// Four codes of one 32-bit word as fp32 values (before the scale).
+template <int FMT>
+__device__ __forceinline__ void decode4(uint32_t u, float* x) {
+  if constexpr (FMT == kCacheInt8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(u >> (8 * i));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((u >> (16 * i)) & 0xffffu), __NV_E4M3);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+  }
+}
+
+// x * y rounded to odd: truncated, with the last bit set when anything was cut off. Rounding such
+// a value to fewer bits gives what rounding the exact product would, so the code below is the
+// nearest to the product itself and does not depend on how fp32 would round it first.
+__device__ __forceinline__ float mul_odd(float x, float y) {
+  const float p = __fmul_rz(x, y);
+  return fmaf(x, y, -p) != 0.f ? __uint_as_float(__float_as_uint(p) | 1u) : p;
+}
+
+// The codes nearest to four values, ties to even, as one 32-bit word; |x| <= kQmax (up to one fp32
+// rounding above it).
+template <int FMT>
+__device__ __forceinline__ uint32_t encode4(const float (&x)[4]) {
+  if constexpr (FMT == kCacheInt8) {
+    // adding 1.5 * 2^23 rounds to a whole number whose two's complement is in the low bits
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(x[i] + 12582912.f);
+    return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+  } else {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+  }
+}
+
+// ---- sequences ---------------------------------------------------------------------------------
+struct SeqView {
+  int64_t row0;  // first row of the operands
+  int32_t n;     // rows
+  int32_t len;   // tokens, the rows' own included
+};
+
+// Sequence b of a call, checked against the call's bounds; false (reported once) when outside.
+// rows_in_seq: the rows stand for tokens of the cache, so there are at most len.
+__device__ __forceinline__ bool seq_view(const CacheSeqs& s, int b, bool rows_in_seq, int32_t* status, SeqView& v) {
+  int64_t r0 = (int64_t)b * s.max_rows, r1 = r0 + s.max_rows;
+  if (s.row_start) {
+    r0 = s.row_start[b];
+    r1 = s.row_start[b + 1];
+  }
+  v.row0 = r0;
+  v.n = (int32_t)(r1 - r0);
+  v.len = s.lengths[b];
+  const bool ok = r0 >= 0 && r1 >= r0 && r1 <= s.rows && r1 - r0 <= s.max_rows && v.len >= 0 && v.len <= s.max_len &&
+                  (!rows_in_seq || v.n <= v.len);
+  if (!ok && threadIdx.x == 0) report_error(status, DEV_BAD_SEQ, 0, b);
+  return ok;
+}
+
+// Block number of block j of sequence b, or -1 (reported) when it is outside the cache.
+__device__ __forceinline__ int32_t block_of(const CacheSeqs& s, const CachePool& c, int b, int j, int32_t* status) {
+  const int32_t p = s.table[(int64_t)b * s.ld_table + j];
+  if (p >= 0 && p < c.blocks) return p;
+  report_error(status, DEV_BAD_BLOCK, 0, p);
+  return -1;
+}
+
+}  // namespace supra

@@ -1,0 +1,551 @@
+// Attention of few query rows over the paged 8-bit K/V cache (steps of single tokens, short drafts).
+//
+//   s_ij = scale * k_scale[block(j), h] * (q_i . code_j),  p_ij = exp2(s_ij - m_i)
+//   o_i  = sum_j p_ij v_scale[block(j), h] code'_j / sum_j p_ij
+// The cache's bytes are the bound: each is read from HBM once for all query rows that share its head,
+// and turned into 16-bit floats on the way to the tensor cores (mma.sync m16n8k16: the tile is 8
+// query rows wide, which the 128-row tcgen05 tile would pad 16-fold, and the tensor pipe is not
+// what bounds this kernel). Scores are formed transposed, S^T = K Q^T with tokens as the 16 rows of
+// the MMA, so that 8 query rows fill its 8 columns; P^T is turned in registers (movmatrix) into the B
+// operand of O^T += V^T P^T, and a row's statistics and its column of O^T live in the same lanes.
+// Codes are exact in fp16; the per-block scales multiply the scores and each block's partial sum in
+// fp32, which also keeps the long sum over blocks in fp32 registers, rounded to nearest.
+// q is multiplied by a power of two per row (its largest channel lands in [2^13, 2^14)) and rounded to
+// fp16, which is exact for bf16 and fp16 rows down to 2^-27 of their largest channel. fp32 rows use two
+// fp16 parts, hi + lo (22 bits), and so does p; each product is then two MMAs.
+//
+// One warp walks over a contiguous range of 32-token tiles, fed by its own ring of cp.async stages
+// (a padded row pitch keeps ldmatrix free of bank conflicts); 4 warps form a CTA and 1 to 16 CTAs a
+// cluster that splits one (sequence, cache head, 8 or 16 query rows). The cluster joins its parts
+// through distributed shared memory: no workspace, no atomics, the same order every time.
+#include <cooperative_groups.h>
+
+#include "cache.cuh"
+
+namespace supra {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kTile = 32;  // tokens of a warp's tile
+constexpr int kStages = 3;
+constexpr float kPShift = 12.f;  // p is formed as 2^12 p: its fp16 part keeps 2^-24 of p = 1 at 2^-12
+
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm2(uint32_t (&r)[2], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];"
+               : "=r"(r[0]), "=r"(r[1])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm2t(uint32_t (&r)[2], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];"
+               : "=r"(r[0]), "=r"(r[1])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t movm(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+// Two codes as fp16. kSel picks the bytes (i, j) of u: 0x4140 / 0x4342 neighbours, 0x4240 / 0x4341
+// every other byte.
+template <int FMT, uint32_t SEL>
+__device__ __forceinline__ uint32_t codes2(uint32_t u) {
+  if constexpr (FMT == kCacheInt8) {
+    // u holds codes + 128: 0x64 above a byte is the fp16 number 1024 + byte
+    const uint32_t w = __byte_perm(u, 0x64646464u, SEL);
+    const uint32_t off = 0x64806480u;  // 1152
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&off));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    constexpr uint32_t lo = SEL & 0xf, hi = (SEL >> 8) & 0xf;
+    const uint32_t w = __byte_perm(u, 0, lo | (hi << 4));
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+  }
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t prep(uint32_t u) {
+  return FMT == kCacheInt8 ? u ^ 0x80808080u : u;
+}
+
+// What a warp knows of a 16-token group of its tile: the K and V scale, and whether its block exists.
+struct Group {
+  float ks, vs;
+  int32_t dead, pad;
+};
+
+__host__ __device__ constexpr int pitch_of(int D) { return 16 * ((D >> 4) | 1); }
+constexpr int stage_bytes(int D) { return 2 * kTile * pitch_of(D) + 2 * (int)sizeof(Group); }
+
+// DT: head dim rounded up to 64 or 128. NT: groups of 8 query rows. SPLIT: two fp16 parts of q and p.
+// ONE: blocks of at least 32 tokens, so that a tile has one pair of scales.
+template <typename T, int FMT, int DT, int NT, bool ONE>
+__global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const __grid_constant__ CacheAttnLaunch L, int tiles) {
+  constexpr bool SPLIT = sizeof(T) == 4;
+  constexpr int CH = DT / 16;  // 16-channel chunks
+  constexpr int NR = 8 * NT;
+  namespace cg = cooperative_groups;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const CachePool& c = L.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int crank = (int)cluster.block_rank(), csize = (int)cluster.num_blocks();
+
+  // unit = (sequence, cache head, row tile); the whole cluster has the same one
+  int unit = blockIdx.x / csize;
+  const int rt = unit % tiles;
+  unit /= tiles;
+  const int hk = unit % c.H, b = unit / c.H;
+  SeqView q;
+  if (!seq_view(L.s, b, false, L.status, q)) return;
+  const int rows = q.n * L.G;  // packed (query, head of the group)
+  const int r0 = rt * NR;
+  if (r0 >= rows) return;
+  const int nrow = min(NR, rows - r0);
+  // tokens that some row of this tile sees
+  const int past = q.len - q.n;  // causal: query i sees tokens 0 .. past + i
+  const int i_last = (r0 + nrow - 1) / L.G, i_first = r0 / L.G;
+  const int seen = L.causal ? max(0, min(q.len, past + i_last + 1)) : q.len;
+  const int all = L.causal ? max(0, min(q.len, past + i_first + 1)) : q.len;  // every row sees these
+
+  const int D = c.D, ch = D >> 4, pitch = pitch_of(D);
+  const int tile_bytes = kTile * pitch;
+  const int sbytes = 2 * tile_bytes + 2 * (int)sizeof(Group);
+  uint8_t* ring = smem + warp * kStages * sbytes;
+
+  // ---- q fragments: lane (g, t) holds channels 16 k + 4 t .. + 3 of row g of each row group ----
+  uint32_t qh[NT][CH][2], ql[SPLIT ? NT : 1][SPLIT ? CH : 1][2];
+  float rs[NT][2];   // score factor of rows 2t, 2t + 1
+  int lim[NT][2];    // last token that they see
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float x[CH][4];
+    float top = 0.f;
+    const int r = 8 * n + g;
+    const bool live = r < nrow;
+    const int pr = r0 + min(r, nrow - 1);
+    const T* src = static_cast<const T*>(L.q) + (q.row0 + pr / L.G) * L.ldq + (int64_t)(hk * L.G + pr % L.G) * D;
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[k][e] = live && k < ch ? to_f32<T>(src[16 * k + 4 * t + e]) : 0.f;
+        top = fmaxf(top, fabsf(x[k][e]));
+      }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // 2^(13 - exponent of top), kept inside the fp32 range at both ends
+    const int ex = min(max((int)(__float_as_uint(top) >> 23), 27), 254) - 127;
+    const float up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
+    const float down = __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[k][e] *= up;
+      qh[n][k][0] = pack2<__half>(x[k][0], x[k][1]);
+      qh[n][k][1] = pack2<__half>(x[k][2], x[k][3]);
+      if constexpr (SPLIT) {
+        const float2 a = unpack2<__half>(qh[n][k][0]), d = unpack2<__half>(qh[n][k][1]);
+        ql[n][k][0] = pack2<__half>(x[k][0] - a.x, x[k][1] - a.y);
+        ql[n][k][1] = pack2<__half>(x[k][2] - d.x, x[k][3] - d.y);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      rs[n][e] = L.scale_log2 * __shfl_sync(0xffffffffu, down, (2 * t + e) * 4);
+      const int rr = min(8 * n + 2 * t + e, nrow - 1);
+      lim[n][e] = L.causal ? min(q.len - 1, past + (r0 + rr) / L.G) : q.len - 1;
+    }
+  }
+
+  float o[CH][NT][4];
+  float m[NT][2], l[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) m[n][e] = -INFINITY, l[n][e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < CH; ++k)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[k][n][e] = 0.f;
+
+  // ---- this warp's tiles ----
+  const int nt = (seen + kTile - 1) / kTile;
+  const int parts = csize * kWarps, part = crank * kWarps + warp;
+  const int share = nt / parts, extra = nt % parts;
+  const int t0 = part * share + min(part, extra);
+  const int cnt = share + (part < extra ? 1 : 0);
+
+  // Blocks of the next 16-token groups, one group per lane: the set in use, and the next one, whose
+  // loads are under way while the first is used up.
+  const int log2t = c.log2t;
+  auto page_at = [&](int grp) {  // grp: 16-token group of the sequence
+    const int j = (grp * 16) >> log2t;
+    if (grp * 16 >= seen) return -2;
+    const int32_t p = L.s.table[(int64_t)b * L.s.ld_table + j];
+    return p;
+  };
+  auto scales_at = [&](int p, float& ks, float& vs) {
+    ks = vs = 0.f;
+    if (p >= 0 && p < c.blocks) {
+      const int64_t u = (int64_t)p * c.H + hk;
+      ks = c.ks[u];
+      vs = c.vs[u];
+    }
+  };
+  int page = page_at(2 * t0 + lane), page_n = page_at(2 * t0 + 32 + lane);
+  float ks, vs, ks_n = 0.f, vs_n = 0.f;
+  scales_at(page, ks, vs);
+  auto issue = [&](int i) {  // loads the warp's tile i into its stage
+    if (i < cnt) {
+      const int w = i & 15;
+      if (w == 0 && i > 0) {
+        page = page_n, ks = ks_n, vs = vs_n;
+        page_n = page_at(2 * (t0 + i) + 32 + lane);
+      }
+      if (w == 8) scales_at(page_n, ks_n, vs_n);
+      uint8_t* st = ring + (i % kStages) * sbytes;
+      const int tok0 = (t0 + i) * kTile;
+      const int p0 = __shfl_sync(0xffffffffu, page, 2 * w), p1 = __shfl_sync(0xffffffffu, page, 2 * w + 1);
+      // lane: one 16-byte chunk of each of its rows, CH lanes a row
+      const int kc = lane % CH, rl = lane / CH;
+      if (kc < ch) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const int p = a ? p1 : p0, tok = tok0 + 16 * a + rl;
+          const bool have = p >= 0 && p < c.blocks;
+          const int64_t off = have ? ((((int64_t)p * c.H + hk) << log2t) + (tok & ((1 << log2t) - 1))) * D + 16 * kc : 0;
+          const uint8_t *gk = c.k + off, *gv = c.v + off;
+          uint8_t* to = st + (16 * a + rl) * pitch + 16 * kc;
+#pragma unroll
+          for (int r = 0; r < 16; r += 32 / CH) {
+            const bool in = have && tok + r < seen;
+            cp_async16(to + r * pitch, in ? gk + r * D : c.k, in ? 16 : 0);
+            cp_async16(to + tile_bytes + r * pitch, in ? gv + r * D : c.v, in ? 16 : 0);
+          }
+        }
+      }
+      if (lane >= 2 * w && lane < 2 * w + 2) {
+        const bool dead = page < 0 || page >= c.blocks;
+        Group* gr = reinterpret_cast<Group*>(st + 2 * tile_bytes) + (lane - 2 * w);
+        gr->ks = ks, gr->vs = vs, gr->dead = dead;
+        if (dead && page != -2) report_error(L.status, DEV_BAD_BLOCK, 1, page);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue(i);
+
+  for (int i = 0; i < cnt; ++i) {
+    cp_async_wait<kStages - 2>();
+    __syncwarp();
+    issue(i + kStages - 1);  // into the stage that the previous tile has left
+    uint8_t* st = ring + (i % kStages) * sbytes;
+    const Group* gr = reinterpret_cast<const Group*>(st + 2 * tile_bytes);
+    const uint32_t kb = smem_u32(st), vb = kb + (uint32_t)tile_bytes;
+    const int tok0 = (t0 + i) * kTile;
+
+    // S^T: two 16-token groups
+    float s[2][NT][4];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[a][n][e] = 0.f;
+      const uint32_t row = kb + (uint32_t)((16 * a + (lane & 15)) * pitch);
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        if (k >= ch) break;
+        uint32_t u[2];  // tokens 0-7 and 8-15 of the group, channels 16 k ..
+        ldsm2(u, row + 16 * k);
+        u[0] = prep<FMT>(u[0]), u[1] = prep<FMT>(u[1]);
+        const uint32_t f[4] = {codes2<FMT, 0x4140>(u[0]), codes2<FMT, 0x4140>(u[1]), codes2<FMT, 0x4342>(u[0]),
+                               codes2<FMT, 0x4342>(u[1])};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if constexpr (SPLIT) mma(s[a][n], f, ql[n][k]);
+          mma(s[a][n], f, qh[n][k]);
+        }
+      }
+    }
+    const float ks0 = gr[0].ks, ks1 = gr[1].ks;
+    const bool partial = tok0 + kTile > all || gr[0].dead || gr[1].dead;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[0][n][e] *= ks0 * rs[n][e & 1];
+        s[1][n][e] *= (ONE ? ks0 : ks1) * rs[n][e & 1];
+      }
+    if (partial) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (gr[a].dead || tok0 + 16 * a + 8 * (e >> 1) + g > lim[n][e & 1]) s[a][n][e] = -INFINITY;
+    }
+    // row maxima over the tile, statistics, P
+    float al[NT][2];
+    bool moved = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = fmaxf(fmaxf(s[0][n][e], s[0][n][e + 2]), fmaxf(s[1][n][e], s[1][n][e + 2]));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+        const float mn = fmaxf(m[n][e], x);
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        al[n][e] = ex2f(m[n][e] - ref);
+        moved = moved || mn != m[n][e];
+        m[n][e] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            s[a][n][e + 2 * y] = ex2f(s[a][n][e + 2 * y] - ref + kPShift);
+            sum += s[a][n][e + 2 * y];
+          }
+        l[n][e] = l[n][e] * al[n][e] + sum;
+      }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[k][n][e] *= al[n][e & 1];
+    }
+    uint32_t ph[2][NT][2], pl[SPLIT ? 2 : 1][SPLIT ? NT : 1][2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const float x0 = s[a][n][2 * y], x1 = s[a][n][2 * y + 1];
+          const uint32_t hi = pack2<__half>(x0, x1);
+          if constexpr (SPLIT) {
+            const float2 f = unpack2<__half>(hi);
+            pl[a][n][y] = movm(pack2<__half>(x0 - f.x, x1 - f.y));
+          }
+          ph[a][n][y] = movm(hi);
+        }
+    // O^T += vscale * (V^T P^T), each block's part from a fresh accumulator
+    const float vs0 = gr[0].vs, vs1 = gr[1].vs;
+    // A block whose scale is not finite reaches only the rows that see it.
+    const bool odd = !(fabsf(vs0) <= 3.4028234e38f) || !(fabsf(vs1) <= 3.4028234e38f);
+    bool sees[2][NT][2];
+    if (odd) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) sees[a][n][e] = tok0 + 16 * a <= lim[n][e];
+    }
+    const uint32_t vrow = vb + (uint32_t)((lane & 15) * pitch);
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      if (k >= ch) break;
+      float acc[NT][4];
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        if (a == 0 || !ONE) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+        }
+        uint32_t u[2];  // tokens 0-7 and 8-15 of the group, transposed: lane has tokens 2t, 2t + 1 and
+                        // channels 2g, 2g + 1 of the chunk, which are rows g and g + 8 of the MMA
+        ldsm2t(u, vrow + (uint32_t)(16 * a * pitch) + 16 * k);
+        u[0] = prep<FMT>(u[0]), u[1] = prep<FMT>(u[1]);
+        const uint32_t f[4] = {codes2<FMT, 0x4240>(u[0]), codes2<FMT, 0x4341>(u[0]), codes2<FMT, 0x4240>(u[1]),
+                               codes2<FMT, 0x4341>(u[1])};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if constexpr (SPLIT) mma(acc[n], f, pl[a][n]);
+          mma(acc[n], f, ph[a][n]);
+        }
+        if (a == 1 || !ONE) {
+          const float v = ONE ? vs0 : a ? vs1 : vs0;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (odd && !sees[ONE ? 0 : a][n][e & 1]) continue;
+              o[k][n][e] = fmaf(v, acc[n][e], o[k][n][e]);
+            }
+        }
+      }
+    }
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
+      l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
+      l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
+    }
+  __syncthreads();  // every warp has left its ring
+
+  // ---- join: the CTA's warps, then the cluster's CTAs ----
+  // shared memory: O of each warp [kWarps][NR][DT], then (m, l) [kWarps][NR]; the CTA's own sums
+  // [NR][DT] and (m, l) [NR] follow
+  float* wo = reinterpret_cast<float*>(smem);
+  float2* wml = reinterpret_cast<float2*>(wo + kWarps * NR * DT);
+  float* co = reinterpret_cast<float*>(wml + kWarps * NR);
+  float2* cml = reinterpret_cast<float2*>(co + NR * DT);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        wo[(warp * NR + 8 * n + 2 * t + (e & 1)) * DT + 16 * k + 2 * g + (e >> 1)] = o[k][n][e];
+    if (g == 0) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) wml[warp * NR + 8 * n + 2 * t + e] = make_float2(m[n][e], l[n][e]);
+    }
+  }
+  __syncthreads();
+  T* out = static_cast<T*>(L.o);
+  auto store = [&](int r, int d, float x) {
+    const int pr = r0 + r;
+    out[(q.row0 + pr / L.G) * L.ldo + (int64_t)(hk * L.G + pr % L.G) * D + d] = from_f32<T>(x);
+  };
+  for (int idx = threadIdx.x; idx < nrow * D; idx += kWarps * 32) {
+    const int r = idx / D, d = idx - r * D;
+    float mx = -INFINITY, sum = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, wml[w * NR + r].x);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float2 ml = wml[w * NR + r];
+      const float f = ex2f(ml.x - ref);
+      sum = fmaf(ml.y, f, sum);
+      x = fmaf(wo[(w * NR + r) * DT + d], f, x);
+    }
+    if (csize == 1) {
+      store(r, d, sum == 0.f ? 0.f : x / sum);
+    } else {
+      co[r * DT + d] = x;
+      if (d == 0) cml[r] = make_float2(mx, sum);
+    }
+  }
+  if (csize > 1) {
+    cluster.sync();
+    for (int idx = crank * kWarps * 32 + threadIdx.x; idx < nrow * D; idx += csize * kWarps * 32) {
+      const int r = idx / D, d = idx - r * D;
+      float mx = -INFINITY, sum = 0.f, x = 0.f;
+      for (int k = 0; k < csize; ++k) mx = fmaxf(mx, cluster.map_shared_rank(cml, k)[r].x);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      for (int k = 0; k < csize; ++k) {
+        const float2 ml = cluster.map_shared_rank(cml, k)[r];
+        const float f = ex2f(ml.x - ref);
+        sum = fmaf(ml.y, f, sum);
+        x = fmaf(cluster.map_shared_rank(co, k)[r * DT + d], f, x);
+      }
+      store(r, d, sum == 0.f ? 0.f : x / sum);
+    }
+    cluster.sync();  // no CTA leaves while another reads its shared memory
+  }
+}
+
+template <int NT>
+size_t smem_of(int D, int DT) {
+  const size_t ring = (size_t)kWarps * kStages * stage_bytes(D);
+  const size_t join = (size_t)(kWarps + 1) * (8 * NT) * (DT * sizeof(float) + sizeof(float2));
+  return ring > join ? ring : join;
+}
+
+template <typename T, int FMT, int DT, int NT, bool ONE>
+cudaError_t attn_as(const CacheAttnLaunch& L, cudaStream_t s) {
+  const int64_t rows = (int64_t)L.s.max_rows * L.G;
+  const int tiles = (int)((rows + 8 * NT - 1) / (8 * NT));
+  const int64_t units = (int64_t)L.s.B * L.c.H * tiles;
+  // CTAs that split one unit: enough to fill the SMs several times over, each left with at least 256
+  // tokens of the longest sequence
+  int split = 1;
+  while (split < 16 && units * split < 148 * 8 && (int64_t)L.s.max_len >= (int64_t)split * 2 * 256) split *= 2;
+  if (units * split > INT32_MAX) return cudaErrorInvalidValue;
+  auto kernel = cache_attn_kernel<T, FMT, DT, NT, ONE>;
+  const size_t smem = smem_of<NT>(L.c.D, DT);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of<NT>(DT, DT));
+  if (e == cudaSuccess && split > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * split));
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, L, tiles);
+}
+
+template <typename T, int FMT, int DT, int NT>
+cudaError_t attn_nt(const CacheAttnLaunch& L, cudaStream_t s) {
+  return L.c.log2t >= 5 ? attn_as<T, FMT, DT, NT, true>(L, s) : attn_as<T, FMT, DT, NT, false>(L, s);
+}
+template <typename T, int FMT>
+cudaError_t attn_fmt(const CacheAttnLaunch& L, cudaStream_t s) {
+  const bool wide = (int64_t)L.s.max_rows * L.G > 8;
+  if (L.c.D <= 64) return wide ? attn_nt<T, FMT, 64, 2>(L, s) : attn_nt<T, FMT, 64, 1>(L, s);
+  return wide ? attn_nt<T, FMT, 128, 2>(L, s) : attn_nt<T, FMT, 128, 1>(L, s);
+}
+template <typename T>
+cudaError_t attn_type(const CacheAttnLaunch& L, int format, cudaStream_t s) {
+  return format == kCacheInt8 ? attn_fmt<T, kCacheInt8>(L, s) : attn_fmt<T, kCacheE4m3>(L, s);
+}
+
+}  // namespace
+
+cudaError_t launch_cache_attn(const CacheAttnLaunch& L, int type, int format, cudaStream_t s) {
+  if (type == kTypeF32) return attn_type<float>(L, format, s);
+  if (type == kTypeF16) return attn_type<__half>(L, format, s);
+  return attn_type<__nv_bfloat16>(L, format, s);
+}
+const char* cache_attn_name(const CacheAttnLaunch& L, int type) {
+  (void)L;
+  return type == kTypeF32 ? "cache_attention_rows_fp32" : "cache_attention_rows";
+}
+
+}  // namespace supra

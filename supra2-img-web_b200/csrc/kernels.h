@@ -13,6 +13,9 @@ enum DevStatus : int32_t {
   DEV_OK = 0,
   DEV_TIMEOUT = 1,   // a bounded mbarrier / copy wait ran out
   DEV_BAD_TILE = 2,  // a tile index outside the launch's problem list
+  DEV_BAD_SEQ = 3,   // a sequence outside the bounds of its cache call (detail: its index)
+  DEV_BAD_BLOCK = 4, // a block number outside the cache (detail: the number)
+  DEV_BAD_POSITION = 5,  // a row's position outside the rotation table (detail: the row)
 };
 
 // One attention problem (all heads of one ops.attention call) as the fused kernels see it.
@@ -294,6 +297,74 @@ cudaError_t launch_ln_stats(const float* x, int32_t K, int32_t rows, float eps, 
 cudaError_t launch_norm_apply(const LinProb& P, float* dst, cudaStream_t s);
 cudaError_t launch_gn_stats(const float* x, int32_t K, int32_t rows_per_image, int32_t images, int32_t groups,
                             float eps, float2* stats, cudaStream_t s);
+
+// ---- query/key norm with rotation, and the paged 8-bit K/V cache --------------------------------
+// Element types (SUPRA_ATTN_T_*) and cache formats (SUPRA_ATTN_CACHE_*).
+constexpr int kTypeF32 = 0, kTypeF16 = 1, kTypeBf16 = 2;
+constexpr int kCacheInt8 = 0, kCacheE4m3 = 1;
+constexpr int kCacheMaxD = 128;
+
+// One operand of qk_norm (offsets applied), qk_norm.cu.
+struct QkOperand {
+  const void* x;
+  void* y;
+  const float* w;
+  int64_t ldx, ldy;
+  int32_t H;
+};
+struct QkNormLaunch {
+  QkOperand q, k;
+  const float* turns;
+  const int32_t* positions;
+  int32_t M, D, rot, n_turns;
+  float eps;
+  int32_t norm, interleaved;
+  int32_t* status;
+};
+// vec: every head row starts on a 16-byte boundary and D, rot / 2 (or rot, interleaved) split into
+// 16-byte pieces
+cudaError_t launch_qk_norm(const QkNormLaunch& L, int type, bool vec, cudaStream_t s);
+
+// The cache's pool and the sequences of a call as the kernels see them.
+struct CachePool {
+  uint8_t* k;
+  uint8_t* v;
+  float* ks;
+  float* vs;
+  int32_t blocks, H, D, log2t;  // log2 of the tokens of a block
+};
+struct CacheSeqs {
+  const int32_t* lengths;
+  const int32_t* table;
+  const int32_t* row_start;
+  int64_t rows;
+  int32_t B, ld_table, max_rows, max_len;
+};
+struct CacheRowsLaunch {
+  CachePool c;
+  CacheSeqs s;
+  void* k;  // offsets applied
+  void* v;
+  int64_t ldk, ldv;
+  int32_t* status;
+};
+// vec: every row of k and v starts on a 16-byte boundary
+cudaError_t launch_cache_write(const CacheRowsLaunch& L, int type, int format, bool vec, cudaStream_t s);
+cudaError_t launch_cache_read(const CacheRowsLaunch& L, int type, int format, bool vec, cudaStream_t s);
+
+struct CacheAttnLaunch {
+  CachePool c;
+  CacheSeqs s;
+  const void* q;
+  void* o;
+  int64_t ldq, ldo;
+  int32_t H, G;  // query heads, and query heads of one cache head
+  float scale_log2;
+  int32_t causal;
+  int32_t* status;
+};
+cudaError_t launch_cache_attn(const CacheAttnLaunch& L, int type, int format, cudaStream_t s);
+const char* cache_attn_name(const CacheAttnLaunch& L, int type);
 
 // Copies bytes (a multiple of 16, both addresses 16-byte aligned) from src, which may be pinned
 // host memory addressable by the device, to device memory dst (stage.cu).

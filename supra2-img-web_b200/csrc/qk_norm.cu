@@ -1,0 +1,204 @@
+// RMS norm of every query and key head with the position rotation in the same pass.
+//   n = x / sqrt(mean(x^2) + eps) * w;  (y_a, y_b) = (n_a cos - n_b sin, n_b cos + n_a sin)
+// Bound by the rows' bytes in and out. The vector form gives a head to a group of lanes, each with
+// one 16-byte piece: the sum of squares and the partner channels of the rotation go by shuffles, so
+// every element is read once, and a warp walks over the heads of one row with the row's turns and the
+// weights held in registers. Every lane stores only pieces that it loaded itself, so in-place calls
+// need no ordering. The scalar form (odd sizes and alignments) gives a head to a warp.
+#include "cache.cuh"
+
+namespace supra {
+namespace {
+
+template <typename T>
+struct Head {
+  const T* x;
+  T* y;
+  bool key;
+};
+template <typename T>
+__device__ __forceinline__ Head<T> head_of(const QkNormLaunch& L, int64_t row, int h) {
+  Head<T> r;
+  r.key = h >= L.q.H;
+  const QkOperand& o = r.key ? L.k : L.q;
+  const int64_t at = (int64_t)(r.key ? h - L.q.H : h) * L.D;
+  r.x = static_cast<const T*>(o.x) + row * o.ldx + at;
+  r.y = static_cast<T*>(o.y) + row * o.ldy + at;
+  return r;
+}
+
+// The row of the turns table for `row`, or null (reported) when its position is outside.
+__device__ __forceinline__ const float* turns_of(const QkNormLaunch& L, int64_t row, int lane, bool* ok) {
+  *ok = true;
+  if (L.rot == 0) return nullptr;
+  const int64_t p = L.positions ? (int64_t)L.positions[row] : row;
+  if (p < 0 || p >= L.n_turns) {
+    if (lane == 0) report_error(L.status, DEV_BAD_POSITION, 0, (int32_t)row);
+    *ok = false;
+    return nullptr;
+  }
+  return L.turns + p * L.rot;
+}
+
+// LPH lanes per head (a power of two), V elements per lane; `wpr` warps share a row's heads.
+template <typename T, int LPH>
+__global__ void __launch_bounds__(256) qk_norm_vec(const __grid_constant__ QkNormLaunch L, int wpr) {
+  constexpr int V = 16 / (int)sizeof(T);
+  constexpr int UNROLL = 4;
+  const int lane = threadIdx.x & 31, g = lane / LPH, l = lane % LPH;
+  const int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int64_t row = w / wpr;
+  if (row >= L.M) return;
+  bool ok;
+  const float* turns = turns_of(L, row, lane, &ok);
+  if (!ok) return;
+  const int e0 = l * V;                 // the lane's first channel
+  const bool on = e0 < L.D;             // lanes past the head only take part in the shuffles
+  const int half = L.rot >> 1;
+  const bool turn = on && e0 < L.rot;
+  // Interleaved: the lane's own pairs. Else the partner piece is half a rotation away, in the
+  // lane `away` from this one, and this lane's results are n cos -+ partner sin.
+  const bool second = !L.interleaved && e0 >= half;
+  const int peer = L.interleaved ? lane : g * LPH + (turn ? (second ? e0 - half : e0 + half) / V : l);
+  float co[V], si[V], wq[V], wk[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    co[i] = 1.f, si[i] = 0.f, wq[i] = 1.f, wk[i] = 1.f;
+    if (turn) {
+      const int p = L.interleaved ? (e0 + i) >> 1 : second ? e0 + i - half : e0 + i;
+      co[i] = turns[p];
+      si[i] = turns[half + p];
+      if (L.interleaved ? !(i & 1) : !second) si[i] = -si[i];
+    }
+    if (on && L.q.w) wq[i] = L.q.w[e0 + i];
+    if (on && L.k.w) wk[i] = L.k.w[e0 + i];
+  }
+  const int heads = L.q.H + L.k.H;
+  const int step = wpr * (32 / LPH);
+  const float inv_d = 1.f / (float)L.D;
+  // (whole warps stay in the loop: the shuffles need every lane)
+  for (int base = (int)(w - row * wpr) * (32 / LPH); base < heads; base += step * UNROLL) {
+    float x[UNROLL][V];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int h = base + u * step + g;
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[u][i] = 0.f;
+      if (on && h < heads) load_row<T, V, true>(head_of<T>(L, row, h).x + e0, x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      if (base + u * step >= heads) break;  // uniform over the warp
+      const int h = base + u * step + g;
+      const Head<T> hd = head_of<T>(L, row, min(h, heads - 1));
+      if (L.norm) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) ss = fmaf(x[u][i], x[u][i], ss);
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float r = 1.f / sqrtf(ss * inv_d + L.eps);
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[u][i] = x[u][i] * r * (hd.key ? wk[i] : wq[i]);
+      }
+      float y[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float other = L.interleaved ? x[u][i ^ 1] : __shfl_sync(0xffffffffu, x[u][i], peer);
+        y[i] = turn ? fmaf(x[u][i], co[i], other * si[i]) : x[u][i];
+      }
+      if (on && h < heads) store_row<T, V, true>(hd.y + e0, y);
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) qk_norm_scalar(const __grid_constant__ QkNormLaunch L) {
+  const int lane = threadIdx.x & 31;
+  const int heads = L.q.H + L.k.H;
+  const int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int64_t row = w / heads;
+  if (row >= L.M) return;
+  bool ok;
+  const float* turns = turns_of(L, row, lane, &ok);
+  if (!ok) return;
+  const Head<T> hd = head_of<T>(L, row, (int)(w - row * heads));
+  const float* wt = hd.key ? L.k.w : L.q.w;
+  const int half = L.rot >> 1;
+  float x[8], other[8];  // D <= 256
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int e = lane + 32 * i;
+    x[i] = other[i] = 0.f;
+    if (e < L.D) {
+      x[i] = to_f32<T>(hd.x[e]);
+      ss = fmaf(x[i], x[i], ss);
+      if (e < L.rot) other[i] = to_f32<T>(hd.x[L.interleaved ? e ^ 1 : e < half ? e + half : e - half]);
+    }
+  }
+  float r = 1.f;
+  if (L.norm) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    r = 1.f / sqrtf(ss * (1.f / (float)L.D) + L.eps);
+  }
+  __syncwarp();  // in place: every lane has read its partners before any lane stores
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int e = lane + 32 * i;
+    if (e >= L.D) break;
+    const float n = x[i] * r * (wt ? wt[e] : 1.f);
+    float y = n;
+    if (e < L.rot) {
+      const int p = L.interleaved ? e >> 1 : e < half ? e : e - half;
+      const int at = L.interleaved ? e ^ 1 : e < half ? e + half : e - half;
+      const float m = other[i] * r * (wt ? wt[at] : 1.f);
+      const bool first = L.interleaved ? !(e & 1) : e < half;
+      y = fmaf(n, turns[p], m * (first ? -turns[half + p] : turns[half + p]));
+    }
+    hd.y[e] = from_f32<T>(y);
+  }
+}
+
+template <typename T>
+cudaError_t norm_as(const QkNormLaunch& L, bool vec, cudaStream_t s) {
+  const int heads = L.q.H + L.k.H;
+  const int pieces = L.D * (int)sizeof(T) / 16;
+  if (vec && pieces <= 32) {
+    int lph = 1;
+    while (lph < pieces) lph *= 2;
+    // As many warps per row as bring 16 to every SM (few rows), at least one head group each.
+    const int groups = (heads + 32 / lph - 1) / (32 / lph);
+    int64_t wpr = (148 * 16 + L.M - 1) / L.M;
+    wpr = wpr < groups ? wpr : groups;
+    const int64_t grid = (L.M * wpr + 7) / 8;
+    if (grid > INT32_MAX) return cudaErrorInvalidValue;
+#define SUPRA_QK(N) \
+  case N: qk_norm_vec<T, N><<<(unsigned)grid, 256, 0, s>>>(L, (int)wpr); break;
+    switch (lph) {
+      SUPRA_QK(1)
+      SUPRA_QK(2)
+      SUPRA_QK(4)
+      SUPRA_QK(8)
+      SUPRA_QK(16)
+      SUPRA_QK(32)
+    }
+#undef SUPRA_QK
+  } else {
+    const int64_t grid = ((int64_t)L.M * heads + 7) / 8;
+    if (grid > INT32_MAX) return cudaErrorInvalidValue;
+    qk_norm_scalar<T><<<(unsigned)grid, 256, 0, s>>>(L);
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_qk_norm(const QkNormLaunch& L, int type, bool vec, cudaStream_t s) {
+  if (type == kTypeF32) return norm_as<float>(L, vec, s);
+  if (type == kTypeF16) return norm_as<__half>(L, vec, s);
+  return norm_as<__nv_bfloat16>(L, vec, s);
+}
+
+}  // namespace supra

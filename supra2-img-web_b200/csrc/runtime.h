@@ -5,6 +5,7 @@
 //   validate.cpp      argument checks of the attention and linear descriptors (ops.js:103-149)
 //   flush_attn.cpp    the attention groups of a flush: block, score-materialising and TMA kernels
 //   flush_linear.cpp  the linear groups of a flush: FFMA and tensor-core kernels
+//   cache_ops.cpp     argument checks and launches of the query/key norm and the 8-bit cache calls
 //   supra_attn.cpp    recording, flush/sync and the C ABI entry points
 #pragma once
 
@@ -100,12 +101,32 @@ class IntervalSet {
   mutable std::vector<ByteRange> v_, pend_, tmp_;
 };
 
-enum Path : int { PATH_FUSED = 0, PATH_GEMM = 1, PATH_TF32 = 2, PATH_FP32_TMA = 3, PATH_LINEAR = 4 };
+enum Path : int {
+  PATH_FUSED = 0,
+  PATH_GEMM = 1,
+  PATH_TF32 = 2,
+  PATH_FP32_TMA = 3,
+  PATH_LINEAR = 4,
+  PATH_CACHE = 5,  // the calls of cache_ops.cpp, one launch each
+};
+
+// A recorded qk_norm, cache_write, cache_read or cache_attention call: its launch descriptor.
+struct CacheCall {
+  enum Kind : int32_t { QK_NORM = 0, WRITE = 1, READ = 2, ATTENTION = 3 } kind;
+  int32_t type, format;
+  bool vec;
+  union {
+    supra::QkNormLaunch norm;
+    supra::CacheRowsLaunch rows;
+    supra::CacheAttnLaunch attn;
+  };
+};
 
 struct Queued {
   union {
     AttnProb p;          // attention problems
     supra::LinProb lin;  // PATH_LINEAR: the linear problem
+    size_t call;         // PATH_CACHE: index in the context's cache_calls
   };
   int path;
   int cfg;
@@ -179,9 +200,11 @@ struct CachedMap {
 // A validated problem with the byte ranges it reads and writes (hazard tracking).
 struct Checked {
   Queued q;
-  ByteRange reads[8];
+  ByteRange reads[10];
   int nreads = 0;
   ByteRange write;
+  ByteRange more_writes[3];  // cache_write: K, V and their scales; others write one range
+  int nmore = 0;
   bool empty = false;  // Lq == 0: nothing to do
 };
 
@@ -206,6 +229,7 @@ struct supra_attn_ctx {
   bool ring_ev_used[2] = {false, false};
 
   std::vector<supra::rt::Queued> queue;
+  std::vector<supra::rt::CacheCall> cache_calls;  // the recorded PATH_CACHE calls (Queued::call)
   supra::rt::IntervalSet qreads, qwrites;
   // enqueue_batch's working storage, kept across calls
   std::vector<supra::rt::Checked> batch_checked;
@@ -327,6 +351,12 @@ struct TcJob {
   const float* xl;
   int64_t ldxs;
 };
+
+// ---- cache_ops.cpp ----
+int check_qk_norm(supra_attn_ctx* c, const supra_attn_qk_norm_desc* d, Checked* out, CacheCall* call);
+int check_cache_rows(supra_attn_ctx* c, const supra_attn_cache_rows_desc* d, bool write, Checked* out, CacheCall* call);
+int check_cache_attn(supra_attn_ctx* c, const supra_attn_cache_attn_desc* d, Checked* out, CacheCall* call);
+int flush_cache(supra_attn_ctx* c, std::vector<const Queued*>& g);
 
 int flush_fused(supra_attn_ctx* c, std::vector<const Queued*>& g);
 int flush_gemm(supra_attn_ctx* c, std::vector<const Queued*>& g);

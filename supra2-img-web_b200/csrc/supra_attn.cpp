@@ -18,6 +18,8 @@
 // rest of the runtime is declared in runtime.h.
 #include "runtime.h"
 
+#include <new>
+
 using namespace supra::rt;
 
 namespace {
@@ -36,11 +38,13 @@ int do_flush(supra_attn_ctx* c) {
     rc = path == PATH_FUSED ? flush_fused(c, kv.second)
          : path == PATH_TF32 ? flush_tma(c, kv.second, true)
          : path == PATH_FP32_TMA ? flush_tma(c, kv.second, false)
+         : path == PATH_CACHE ? flush_cache(c, kv.second)
          : path == PATH_LINEAR ? (kv.second[0]->cfg ? flush_linear_tc(c, kv.second) : flush_linear(c, kv.second))
                              : flush_gemm(c, kv.second);
     if (rc) break;
   }
   c->queue.clear();
+  c->cache_calls.clear();
   c->qreads.clear();
   c->qwrites.clear();
   return rc;
@@ -59,6 +63,11 @@ int check_device_status(supra_attn_ctx* c, int32_t* device_status) {
   if (code == supra::DEV_TIMEOUT)
     return set_err(c, SUPRA_ATTN_ETIMEOUT, "device wait timed out (block %d, stage %d, detail %d)", blk, stage,
                    detail);
+  if (code == supra::DEV_BAD_SEQ)
+    return set_err(c, SUPRA_ATTN_EDEVICE, "cache: sequence %d has rows or a length outside the call's bounds", detail);
+  if (code == supra::DEV_BAD_BLOCK) return set_err(c, SUPRA_ATTN_EDEVICE, "cache: block %d is outside the cache", detail);
+  if (code == supra::DEV_BAD_POSITION)
+    return set_err(c, SUPRA_ATTN_EDEVICE, "qk_norm: the position of row %d is outside the rotation table", detail);
   return set_err(c, SUPRA_ATTN_EDEVICE, "device status %d (block %d, stage %d, detail %d)", code, blk, stage, detail);
 }
 
@@ -74,14 +83,59 @@ int record(supra_attn_ctx* c, const Checked& ck) {
   if (ck.empty) return SUPRA_ATTN_OK;
   bool hazard = c->qwrites.overlaps(ck.write.b, ck.write.e) || c->qreads.overlaps(ck.write.b, ck.write.e);
   for (int i = 0; i < ck.nreads && !hazard; ++i) hazard = c->qwrites.overlaps(ck.reads[i].b, ck.reads[i].e);
+  for (int i = 0; i < ck.nmore && !hazard; ++i)
+    hazard = c->qwrites.overlaps(ck.more_writes[i].b, ck.more_writes[i].e) ||
+             c->qreads.overlaps(ck.more_writes[i].b, ck.more_writes[i].e);
   if (hazard) {
     int rc = do_flush(c);
     if (rc) return rc;
   }
   for (int i = 0; i < ck.nreads; ++i) c->qreads.add(ck.reads[i].b, ck.reads[i].e);
   c->qwrites.add(ck.write.b, ck.write.e);
+  for (int i = 0; i < ck.nmore; ++i) c->qwrites.add(ck.more_writes[i].b, ck.more_writes[i].e);
   c->queue.push_back(ck.q);
   return SUPRA_ATTN_OK;
+}
+
+// Checks one call of cache_ops.cpp and records it; no C++ exception leaves the library.
+template <typename Check>
+int record_call(supra_attn_ctx* c, Check check) {
+  if (!c) return SUPRA_ATTN_EINVAL;
+  try {
+    Checked ck;
+    CacheCall call;
+    int rc = check(c, &ck, &call);
+    if (rc || ck.empty) return rc;
+    DeviceGuard g(c->device);
+    rc = record(c, ck);  // (may flush: the call's index is known only after it)
+    if (rc) return rc;
+    c->queue.back().call = c->cache_calls.size();
+    try {
+      c->cache_calls.push_back(call);
+    } catch (const std::bad_alloc&) {
+      c->queue.pop_back();  // (its byte ranges stay: at worst an early flush)
+      throw;
+    }
+    return SUPRA_ATTN_OK;
+  } catch (const std::bad_alloc&) {
+    return set_err(c, SUPRA_ATTN_ENOMEM, "out of host memory");
+  }
+}
+
+// The same checks without a context or a device.
+template <typename Check>
+int check_call(Check check, char* msg, int32_t cap) {
+  try {
+    supra_attn_ctx tmp;  // only its message field is used; no device state is touched
+    Checked ck;
+    CacheCall call;
+    const int rc = check(&tmp, &ck, &call);
+    if (msg && cap > 0) std::snprintf(msg, (size_t)cap, "%s", rc ? tmp.err.c_str() : "");
+    return rc;
+  } catch (const std::bad_alloc&) {
+    if (msg && cap > 0) std::snprintf(msg, (size_t)cap, "out of host memory");
+    return SUPRA_ATTN_ENOMEM;
+  }
 }
 
 // Merges r into the last few runs it overlaps or touches (reads), or appends it. Batches list
@@ -367,6 +421,46 @@ int supra_attn_check_linear_desc(const supra_attn_linear_desc* d, char* msg, int
   const int rc = validate_linear(&tmp, d, &ck);
   if (msg && cap > 0) std::snprintf(msg, (size_t)cap, "%s", rc ? tmp.err.c_str() : "");
   return rc;
+}
+
+int supra_attn_enqueue_qk_norm(supra_attn_ctx* c, const supra_attn_qk_norm_desc* d) {
+  return record_call(c, [d](supra_attn_ctx* x, Checked* ck, CacheCall* call) { return check_qk_norm(x, d, ck, call); });
+}
+
+int supra_attn_check_qk_norm_desc(const supra_attn_qk_norm_desc* d, char* msg, int32_t cap) {
+  return check_call([d](supra_attn_ctx* x, Checked* ck, CacheCall* call) { return check_qk_norm(x, d, ck, call); }, msg,
+                    cap);
+}
+
+int supra_attn_enqueue_cache_write(supra_attn_ctx* c, const supra_attn_cache_rows_desc* d) {
+  return record_call(
+      c, [d](supra_attn_ctx* x, Checked* ck, CacheCall* call) { return check_cache_rows(x, d, true, ck, call); });
+}
+
+int supra_attn_check_cache_write_desc(const supra_attn_cache_rows_desc* d, char* msg, int32_t cap) {
+  return check_call(
+      [d](supra_attn_ctx* x, Checked* ck, CacheCall* call) { return check_cache_rows(x, d, true, ck, call); }, msg, cap);
+}
+
+int supra_attn_enqueue_cache_read(supra_attn_ctx* c, const supra_attn_cache_rows_desc* d) {
+  return record_call(
+      c, [d](supra_attn_ctx* x, Checked* ck, CacheCall* call) { return check_cache_rows(x, d, false, ck, call); });
+}
+
+int supra_attn_check_cache_read_desc(const supra_attn_cache_rows_desc* d, char* msg, int32_t cap) {
+  return check_call(
+      [d](supra_attn_ctx* x, Checked* ck, CacheCall* call) { return check_cache_rows(x, d, false, ck, call); }, msg,
+      cap);
+}
+
+int supra_attn_enqueue_cache_attention(supra_attn_ctx* c, const supra_attn_cache_attn_desc* d) {
+  return record_call(c,
+                     [d](supra_attn_ctx* x, Checked* ck, CacheCall* call) { return check_cache_attn(x, d, ck, call); });
+}
+
+int supra_attn_check_cache_attention_desc(const supra_attn_cache_attn_desc* d, char* msg, int32_t cap) {
+  return check_call([d](supra_attn_ctx* x, Checked* ck, CacheCall* call) { return check_cache_attn(x, d, ck, call); },
+                    msg, cap);
 }
 
 int supra_attn_enqueue_batch(supra_attn_ctx* c, const supra_attn_desc* descs, int32_t n) {

@@ -8,6 +8,7 @@ ImportError if it has not been built; there is no fallback implementation.
 from ._lib import LIB_PATH, SupraAttnError, SupraAttnValueError, Desc, LinearDesc, SIGNATURES, lib
 from .ops import (GPU, Tensor, attention, make_desc, linear, make_linear_desc, position_bias, relative_bucket,
                   default_scale)
+from .cache import CacheBatch, KVCache, cache_attention, cache_read, cache_write, qk_norm, rotation_turns
 
 __all__ = [
     "LIB_PATH",
@@ -26,4 +27,11 @@ __all__ = [
     "position_bias",
     "relative_bucket",
     "default_scale",
+    "KVCache",
+    "CacheBatch",
+    "cache_write",
+    "cache_read",
+    "cache_attention",
+    "qk_norm",
+    "rotation_turns",
 ]

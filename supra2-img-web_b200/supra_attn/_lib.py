@@ -16,6 +16,10 @@ OK, EINVAL, ENOMEM, ECUDA, ETIMEOUT, EDEVICE, ESTATE = range(7)
 FP32, TF32, TF32X3 = 0, 1, 2
 F_DEFAULT_SCALE = 0x1
 F_T5_TABLE = 0x2
+T_F32, T_F16, T_BF16 = 0, 1, 2
+CACHE_INT8, CACHE_E4M3 = 0, 1
+QK_NO_NORM, QK_INTERLEAVED = 0x1, 0x2
+CA_DEFAULT_SCALE, CA_CAUSAL = 0x1, 0x2
 
 
 class Desc(C.Structure):
@@ -61,6 +65,59 @@ class LinearDesc(C.Structure):
     ]
 
 
+class QkOperand(C.Structure):
+    """supra_attn_qk_operand (include/supra_attn.h)."""
+
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("w", C.c_void_p),
+                ("x_size", C.c_int64), ("y_size", C.c_int64), ("w_size", C.c_int64),
+                ("ldx", C.c_int64), ("ldy", C.c_int64), ("x_off", C.c_int64), ("y_off", C.c_int64),
+                ("H", C.c_int32), ("reserved", C.c_int32)]
+
+
+class QkNormDesc(C.Structure):
+    """supra_attn_qk_norm_desc (include/supra_attn.h)."""
+
+    _fields_ = [("q", QkOperand), ("k", QkOperand), ("turns", C.c_void_p), ("positions", C.c_void_p),
+                ("turns_size", C.c_int64), ("positions_size", C.c_int64),
+                ("M", C.c_int32), ("D", C.c_int32), ("rot", C.c_int32), ("n_turns", C.c_int32),
+                ("type", C.c_int32), ("flags", C.c_uint32), ("eps", C.c_float), ("reserved", C.c_int32)]
+
+
+class Cache(C.Structure):
+    """supra_attn_cache (include/supra_attn.h)."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("k_size", C.c_int64), ("v_size", C.c_int64), ("k_scale_size", C.c_int64), ("v_scale_size", C.c_int64),
+                ("blocks", C.c_int32), ("block_tokens", C.c_int32), ("H", C.c_int32), ("D", C.c_int32),
+                ("format", C.c_int32), ("reserved", C.c_int32)]
+
+
+class CacheSeqs(C.Structure):
+    """supra_attn_cache_batch (include/supra_attn.h)."""
+
+    _fields_ = [("lengths", C.c_void_p), ("table", C.c_void_p), ("row_start", C.c_void_p),
+                ("lengths_size", C.c_int64), ("table_size", C.c_int64), ("row_start_size", C.c_int64),
+                ("rows", C.c_int64), ("B", C.c_int32), ("ld_table", C.c_int32),
+                ("max_rows", C.c_int32), ("max_len", C.c_int32)]
+
+
+class CacheRowsDesc(C.Structure):
+    """supra_attn_cache_rows_desc (include/supra_attn.h)."""
+
+    _fields_ = [("cache", Cache), ("seqs", CacheSeqs), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("k_size", C.c_int64), ("v_size", C.c_int64), ("ldk", C.c_int64), ("ldv", C.c_int64),
+                ("k_off", C.c_int64), ("v_off", C.c_int64), ("type", C.c_int32), ("flags", C.c_uint32)]
+
+
+class CacheAttnDesc(C.Structure):
+    """supra_attn_cache_attn_desc (include/supra_attn.h)."""
+
+    _fields_ = [("cache", Cache), ("seqs", CacheSeqs), ("q", C.c_void_p), ("out", C.c_void_p),
+                ("q_size", C.c_int64), ("out_size", C.c_int64), ("ldq", C.c_int64), ("ldo", C.c_int64),
+                ("q_off", C.c_int64), ("o_off", C.c_int64), ("H", C.c_int32), ("type", C.c_int32),
+                ("scale", C.c_float), ("flags", C.c_uint32)]
+
+
 class ProfileEntry(C.Structure):
     _fields_ = [("name", C.c_char * 48), ("launches", C.c_int64), ("ms", C.c_double), ("flops", C.c_double),
                 ("bytes", C.c_double)]
@@ -95,6 +152,14 @@ SIGNATURES = [
     ("supra_attn_attention_noalloc", C.c_int, [C.POINTER(Desc), C.c_void_p, C.c_char_p, C.c_int32]),
     ("supra_attn_enqueue_linear", C.c_int, [C.c_void_p, C.POINTER(LinearDesc)]),
     ("supra_attn_check_linear_desc", C.c_int, [C.POINTER(LinearDesc), C.c_char_p, C.c_int32]),
+    ("supra_attn_enqueue_qk_norm", C.c_int, [C.c_void_p, C.POINTER(QkNormDesc)]),
+    ("supra_attn_check_qk_norm_desc", C.c_int, [C.POINTER(QkNormDesc), C.c_char_p, C.c_int32]),
+    ("supra_attn_enqueue_cache_write", C.c_int, [C.c_void_p, C.POINTER(CacheRowsDesc)]),
+    ("supra_attn_check_cache_write_desc", C.c_int, [C.POINTER(CacheRowsDesc), C.c_char_p, C.c_int32]),
+    ("supra_attn_enqueue_cache_read", C.c_int, [C.c_void_p, C.POINTER(CacheRowsDesc)]),
+    ("supra_attn_check_cache_read_desc", C.c_int, [C.POINTER(CacheRowsDesc), C.c_char_p, C.c_int32]),
+    ("supra_attn_enqueue_cache_attention", C.c_int, [C.c_void_p, C.POINTER(CacheAttnDesc)]),
+    ("supra_attn_check_cache_attention_desc", C.c_int, [C.POINTER(CacheAttnDesc), C.c_char_p, C.c_int32]),
 ]
 
 

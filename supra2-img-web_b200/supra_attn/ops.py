@@ -33,11 +33,13 @@ ACTS = {None: 0, "gelu": 1, "gelu_tanh": 2, "silu": 3}  # SUPRA_ATTN_ACT_*
 class Tensor:
     """app/gpu/device.js:41-55 — {buf, shape, size, release()} over a device address."""
 
-    def __init__(self, gpu: "GPU", buf: int, shape, capacity: int, owned: bool = True, keepalive=None):
+    def __init__(self, gpu: "GPU", buf: int, shape, capacity: int, owned: bool = True, keepalive=None,
+                 dtype: str = "fp32"):
         self.gpu = gpu
         self.buf = buf
         self.shape = list(shape)
-        self.capacity = capacity  # floats addressable at buf (bounds for every call)
+        self.capacity = capacity  # elements addressable at buf (bounds for every call)
+        self.dtype = dtype        # a key of DTYPES; the reference's tensors are all "fp32"
         self.owned = owned
         self._keep = keepalive
 
@@ -54,6 +56,9 @@ class Tensor:
         self.buf = None
         self._keep = None
 
+
+# element types of a Tensor and the numpy type that holds them on the host (bf16: its 16 bits)
+DTYPES = {"fp32": np.float32, "fp16": np.float16, "bf16": np.uint16, "int32": np.int32, "uint8": np.uint8}
 
 CUDA_STREAM_LEGACY = 1  # cudaStreamLegacy: the legacy default stream as an explicit handle
 
@@ -80,6 +85,7 @@ class GPU:
                                           "(needs an sm_100 GPU and the CUDA driver)")
         self.ctx = ctx
         self.device = int(device)
+        self._held = []  # operands of recorded cache and norm calls, kept until they are on the stream
         if stream is not None:
             self.set_stream(stream)
 
@@ -99,15 +105,21 @@ class GPU:
         check(lib.supra_attn_set_stream(self.ctx, C.c_void_p(_stream_handle(stream))), self.ctx)
 
     # ---- tensors ----------------------------------------------------------------------------------
-    def empty(self, shape) -> Tensor:
+    def empty(self, shape, dtype: str = "fp32") -> Tensor:
+        if dtype not in DTYPES:
+            raise ValueError(f"dtype must be one of {sorted(DTYPES)}")
         n = 1
         for s in shape:
             n *= int(s)
         p = C.c_void_p()
-        check(lib.supra_attn_tensor_alloc(self.ctx, n, C.byref(p)), self.ctx)
-        return Tensor(self, p.value, shape, n)
+        # (the library counts floats)
+        check(lib.supra_attn_tensor_alloc(self.ctx, (n * np.dtype(DTYPES[dtype]).itemsize + 3) // 4, C.byref(p)),
+              self.ctx)
+        return Tensor(self, p.value, shape, n, dtype=dtype)
 
-    def from_array(self, arr, shape=None) -> Tensor:
+    def from_array(self, arr, shape=None, dtype: str = "fp32") -> Tensor:
+        if dtype != "fp32":
+            return self._from_array_as(arr, shape, dtype)
         a = np.ascontiguousarray(np.asarray(arr, dtype=np.float32)).reshape(-1)
         t = self.empty(list(shape) if shape is not None else [a.size])
         if t.size != a.size:
@@ -118,6 +130,24 @@ class GPU:
 
     fromArray = from_array
 
+    def _from_array_as(self, arr, shape, dtype: str) -> Tensor:
+        """from_array for the other element types; values must already be of the type (bf16: its bits)."""
+        if dtype not in DTYPES:
+            raise ValueError(f"dtype must be one of {sorted(DTYPES)}")
+        a = np.asarray(arr)
+        if a.size and not np.array_equal(a.astype(DTYPES[dtype]), a):
+            raise ValueError(f"from_array: values that {dtype} does not hold")
+        a = np.ascontiguousarray(a.astype(DTYPES[dtype])).reshape(-1)
+        t = self.empty(list(shape) if shape is not None else [a.size], dtype)
+        if t.size != a.size:
+            t.release()
+            raise ValueError(f"from_array: {a.size} values for shape {shape}")
+        b = np.zeros((a.nbytes + 3) // 4, dtype=np.float32)  # whole floats, as the library copies them
+        b.view(np.uint8)[:a.nbytes] = a.view(np.uint8)
+        check(lib.supra_attn_upload(self.ctx, C.c_void_p(t.buf), b.ctypes.data_as(C.c_void_p), b.size), self.ctx)
+        self.sync()  # (b is pageable memory of this call)
+        return t
+
     def write(self, t: Tensor, arr, offset: int = 0):
         a = np.ascontiguousarray(np.asarray(arr, dtype=np.float32)).reshape(-1)
         if offset < 0 or offset + a.size > t.capacity:
@@ -126,6 +156,8 @@ class GPU:
               self.ctx)
 
     def read(self, t, count: int | None = None) -> np.ndarray:
+        if isinstance(t, Tensor) and t.dtype != "fp32":
+            return self._read_as(t, count)
         buf, cap = _as_buf(t)
         n = cap if count is None and not isinstance(t, Tensor) else (t.size if count is None else int(count))
         if n > cap:
@@ -133,6 +165,18 @@ class GPU:
         out = np.empty(n, dtype=np.float32)
         check(lib.supra_attn_download(self.ctx, out.ctypes.data_as(C.c_void_p), C.c_void_p(buf), n), self.ctx)
         return out
+
+    def _read_as(self, t: Tensor, count: int | None) -> np.ndarray:
+        if not t.buf:
+            raise ValueError("tensor was released")
+        n = t.size if count is None else int(count)
+        if n > t.capacity:
+            raise ValueError("read: count exceeds the tensor")
+        nbytes = n * np.dtype(DTYPES[t.dtype]).itemsize
+        out = np.empty((nbytes + 3) // 4, dtype=np.float32)  # (allocations are whole floats)
+        check(lib.supra_attn_download(self.ctx, out.ctypes.data_as(C.c_void_p), C.c_void_p(t.buf), out.size), self.ctx)
+        self._held.clear()
+        return out.view(np.uint8)[:nbytes].view(DTYPES[t.dtype]).copy()
 
     def wrap(self, x, shape=None) -> Tensor:
         """A non-owning Tensor over a CUDA float32 torch tensor (kept alive by the Tensor)."""
@@ -149,10 +193,14 @@ class GPU:
 
     def flush(self):
         check(lib.supra_attn_flush(self.ctx), self.ctx)
+        self._held.clear()
 
     def sync(self) -> int:
         st = C.c_int32(0)
-        check(lib.supra_attn_sync(self.ctx, C.byref(st)), self.ctx)
+        try:
+            check(lib.supra_attn_sync(self.ctx, C.byref(st)), self.ctx)
+        finally:
+            self._held.clear()
         return st.value
 
     def pending(self) -> int:
@@ -185,6 +233,8 @@ def _as_buf(x):
     if isinstance(x, Tensor):
         if not x.buf:
             raise ValueError("tensor was released")
+        if x.dtype != "fp32":
+            raise ValueError(f"tensor must be fp32, not {x.dtype}")
         return x.buf, x.capacity
     if hasattr(x, "data_ptr") and hasattr(x, "is_cuda"):
         import torch
