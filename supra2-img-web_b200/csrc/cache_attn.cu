@@ -14,20 +14,22 @@
 // fp16, which is exact for bf16 and fp16 rows down to 2^-27 of their largest channel. fp32 rows use two
 // fp16 parts, hi + lo (22 bits), and so does p; each product is then two MMAs.
 //
-// One warp walks over a contiguous range of 32-token tiles, fed by its own ring of cp.async stages
-// (a padded row pitch keeps ldmatrix free of bank conflicts); 4 warps form a CTA and 1 to 16 CTAs a
-// cluster that splits one (sequence, cache head, 8 or 16 query rows). The cluster joins its parts
-// through distributed shared memory: no workspace, no atomics, the same order every time.
+// One warp walks over a contiguous range of 32-token tiles, fed by its own ring of TMA stages: a tile of K
+// or V is one box of the pool seen as [blocks * H * block_tokens, D] bytes (two boxes for 16-token
+// blocks), swizzled so that ldmatrix meets no bank conflicts, its channels past D filled with zeros. 4
+// warps form a CTA and 1 to 16 CTAs a cluster that splits one (sequence, cache head, 8 or 16 query
+// rows). The cluster joins its parts through distributed shared memory: no workspace, no atomics, the
+// same order every time.
 #include <cooperative_groups.h>
 
 #include "cache.cuh"
+#include "tcgen05.cuh"
 
 namespace supra {
 namespace {
 
-constexpr int kWarps = 4;
 constexpr int kTile = 32;  // tokens of a warp's tile
-constexpr int kStages = 3;
+constexpr int kStages = 2;
 constexpr float kPShift = 12.f;  // p is formed as 2^12 p: its fp16 part keeps 2^-24 of p = 1 at 2^-12
 
 __device__ __forceinline__ float ex2f(float x) {
@@ -41,15 +43,9 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ void ldsm2(uint32_t (&r)[2], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];"
-               : "=r"(r[0]), "=r"(r[1])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void ldsm2t(uint32_t (&r)[2], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];"
-               : "=r"(r[0]), "=r"(r[1])
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
 }
@@ -57,6 +53,14 @@ __device__ __forceinline__ uint32_t movm(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
+}
+// d = a b, without an accumulator to clear
+__device__ __forceinline__ void mma0(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
 }
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
   asm volatile(
@@ -66,26 +70,32 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
-// Two codes as fp16. kSel picks the bytes (i, j) of u: 0x4140 / 0x4342 neighbours, 0x4240 / 0x4341
-// every other byte.
-template <int FMT, uint32_t SEL>
-__device__ __forceinline__ uint32_t codes2(uint32_t u) {
-  if constexpr (FMT == kCacheInt8) {
-    // u holds codes + 128: 0x64 above a byte is the fp16 number 1024 + byte
-    const uint32_t w = __byte_perm(u, 0x64646464u, SEL);
-    const uint32_t off = 0x64806480u;  // 1152
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&off));
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    constexpr uint32_t lo = SEL & 0xf, hi = (SEL >> 8) & 0xf;
-    const uint32_t w = __byte_perm(u, 0, lo | (hi << 4));
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-    return (uint32_t)h.x | ((uint32_t)h.y << 16);
-  }
+// Codes of one word as fp16 pairs: bytes 0 and 2, bytes 1 and 3.
+__device__ __forceinline__ void e4m3x4(uint32_t u, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(u));
 }
 template <int FMT>
-__device__ __forceinline__ uint32_t prep(uint32_t u) {
-  return FMT == kCacheInt8 ? u ^ 0x80808080u : u;
+__device__ __forceinline__ void codes4(uint32_t u, uint32_t& even, uint32_t& odd) {
+  if constexpr (FMT == kCacheInt8) {
+    // 0x64 above a byte b is the fp16 number 1024 + b; with b = code + 128, 1152 off gives the code
+    const uint32_t a = (u & 0x00ff00ffu) ^ 0x64806480u, b = ((u >> 8) & 0x00ff00ffu) ^ 0x64806480u;
+    const uint32_t off = 0x64806480u;
+    const __half2 ha = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&off));
+    const __half2 hb = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&off));
+    even = *reinterpret_cast<const uint32_t*>(&ha);
+    odd = *reinterpret_cast<const uint32_t*>(&hb);
+  } else {
+    e4m3x4(__byte_perm(u, 0, 0x3120), even, odd);
+  }
+}
+// The same for operands whose order along the product is free (K, with q's channels in the same order):
+// INT8 as above, E4M3 bytes 0 and 1, bytes 2 and 3, which need no reordering.
+template <int FMT>
+__device__ __forceinline__ void codes4_any(uint32_t u, uint32_t& a, uint32_t& b) {
+  if constexpr (FMT == kCacheInt8) codes4<FMT>(u, a, b);
+  else e4m3x4(u, a, b);
 }
 
 // What a warp knows of a 16-token group of its tile: the K and V scale, and whether its block exists.
@@ -94,18 +104,28 @@ struct Group {
   int32_t dead, pad;
 };
 
-__host__ __device__ constexpr int pitch_of(int D) { return 16 * ((D >> 4) | 1); }
-constexpr int stage_bytes(int D) { return 2 * kTile * pitch_of(D) + 2 * (int)sizeof(Group); }
+constexpr int stage_bytes(int DT) { return 2 * kTile * DT; }
+// Shared memory of a warp besides its stages: a barrier and two groups per stage.
+constexpr int kWarpBytes = kStages * (8 + 2 * (int)sizeof(Group));
 
-// DT: head dim rounded up to 64 or 128. NT: groups of 8 query rows. SPLIT: two fp16 parts of q and p.
-// ONE: blocks of at least 32 tokens, so that a tile has one pair of scales.
-template <typename T, int FMT, int DT, int NT, bool ONE>
-__global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const __grid_constant__ CacheAttnLaunch L, int tiles) {
+// Byte offset in a tile (rows of DT bytes) of 16-byte chunk 0 of row r, as the TMA unit swizzles it:
+// 128-byte rows permute their chunks by r % 8, 64-byte rows by (r / 2) % 4. Chunk k is at ^ (16 k).
+template <int DT>
+__device__ __forceinline__ uint32_t chunk0_at(int r) {
+  return (uint32_t)(r * DT + ((DT == 128 ? r & 7 : (r >> 1) & 3) << 4));
+}
+
+// DT: head dim rounded up to 64 or 128 (the channels between are zero: no branches among the MMAs). NT: groups of 8 query rows. SPLIT: two fp16 parts of q and p. ONE: blocks of at least 32
+// tokens, so that a tile has one pair of scales. W: warps.
+template <typename T, int FMT, int DT, int NT, bool ONE, int W>
+__global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_kernel(const __grid_constant__ CacheAttnArgs L, const __grid_constant__ CUtensorMap mk,
+                                                            const __grid_constant__ CUtensorMap mv, int tiles) {
   constexpr bool SPLIT = sizeof(T) == 4;
   constexpr int CH = DT / 16;  // 16-channel chunks
   constexpr int NR = 8 * NT;
   namespace cg = cooperative_groups;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // swizzle atoms
   const CachePool& c = L.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -129,12 +149,18 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const __grid_co
   const int seen = L.causal ? max(0, min(q.len, past + i_last + 1)) : q.len;
   const int all = L.causal ? max(0, min(q.len, past + i_first + 1)) : q.len;  // every row sees these
 
-  const int D = c.D, ch = D >> 4, pitch = pitch_of(D);
-  const int tile_bytes = kTile * pitch;
-  const int sbytes = 2 * tile_bytes + 2 * (int)sizeof(Group);
+  constexpr int tile_bytes = kTile * DT, sbytes = stage_bytes(DT);
+  const int D = c.D, ch = D >> 4;
   uint8_t* ring = smem + warp * kStages * sbytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + W * kStages * sbytes) + warp * kStages;
+  Group* groups = reinterpret_cast<Group*>(smem + W * kStages * (sbytes + 8)) + warp * kStages * 2;
+  if (lane < kStages) mbar_init(full + lane, 1);
+  mbar_fence_init();
+  __syncwarp();
 
-  // ---- q fragments: lane (g, t) holds channels 16 k + 4 t .. + 3 of row g of each row group ----
+  // ---- q fragments: lane (g, t) holds channels 16 k + 4 t .. + 3 of row g of each row group, paired
+  // as codes4_any pairs K's ----
+  constexpr int P1 = FMT == kCacheInt8 ? 2 : 1;  // the channel beside the first
   uint32_t qh[NT][CH][2], ql[SPLIT ? NT : 1][SPLIT ? CH : 1][2];
   float rs[NT][2];   // score factor of rows 2t, 2t + 1
   int lim[NT][2];    // last token that they see
@@ -163,12 +189,12 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const __grid_co
     for (int k = 0; k < CH; ++k) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[k][e] *= up;
-      qh[n][k][0] = pack2<__half>(x[k][0], x[k][1]);
-      qh[n][k][1] = pack2<__half>(x[k][2], x[k][3]);
+      qh[n][k][0] = pack2<__half>(x[k][0], x[k][P1]);
+      qh[n][k][1] = pack2<__half>(x[k][3 - P1], x[k][3]);
       if constexpr (SPLIT) {
         const float2 a = unpack2<__half>(qh[n][k][0]), d = unpack2<__half>(qh[n][k][1]);
-        ql[n][k][0] = pack2<__half>(x[k][0] - a.x, x[k][1] - a.y);
-        ql[n][k][1] = pack2<__half>(x[k][2] - d.x, x[k][3] - d.y);
+        ql[n][k][0] = pack2<__half>(x[k][0] - a.x, x[k][P1] - a.y);
+        ql[n][k][1] = pack2<__half>(x[k][3 - P1] - d.x, x[k][3] - d.y);
       }
     }
 #pragma unroll
@@ -194,7 +220,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const __grid_co
 
   // ---- this warp's tiles ----
   const int nt = (seen + kTile - 1) / kTile;
-  const int parts = csize * kWarps, part = crank * kWarps + warp;
+  const int parts = csize * W, part = crank * W + warp;
   const int share = nt / parts, extra = nt % parts;
   const int t0 = part * share + min(part, extra);
   const int cnt = share + (part < extra ? 1 : 0);
@@ -220,76 +246,69 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const __grid_co
   float ks, vs, ks_n = 0.f, vs_n = 0.f;
   scales_at(page, ks, vs);
   auto issue = [&](int i) {  // loads the warp's tile i into its stage
-    if (i < cnt) {
-      const int w = i & 15;
-      if (w == 0 && i > 0) {
-        page = page_n, ks = ks_n, vs = vs_n;
-        page_n = page_at(2 * (t0 + i) + 32 + lane);
-      }
-      if (w == 8) scales_at(page_n, ks_n, vs_n);
-      uint8_t* st = ring + (i % kStages) * sbytes;
-      const int tok0 = (t0 + i) * kTile;
-      const int p0 = __shfl_sync(0xffffffffu, page, 2 * w), p1 = __shfl_sync(0xffffffffu, page, 2 * w + 1);
-      // lane: one 16-byte chunk of each of its rows, CH lanes a row
-      const int kc = lane % CH, rl = lane / CH;
-      if (kc < ch) {
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const int p = a ? p1 : p0, tok = tok0 + 16 * a + rl;
-          const bool have = p >= 0 && p < c.blocks;
-          const int64_t off = have ? ((((int64_t)p * c.H + hk) << log2t) + (tok & ((1 << log2t) - 1))) * D + 16 * kc : 0;
-          const uint8_t *gk = c.k + off, *gv = c.v + off;
-          uint8_t* to = st + (16 * a + rl) * pitch + 16 * kc;
-#pragma unroll
-          for (int r = 0; r < 16; r += 32 / CH) {
-            const bool in = have && tok + r < seen;
-            cp_async16(to + r * pitch, in ? gk + r * D : c.k, in ? 16 : 0);
-            cp_async16(to + tile_bytes + r * pitch, in ? gv + r * D : c.v, in ? 16 : 0);
-          }
-        }
-      }
-      if (lane >= 2 * w && lane < 2 * w + 2) {
-        const bool dead = page < 0 || page >= c.blocks;
-        Group* gr = reinterpret_cast<Group*>(st + 2 * tile_bytes) + (lane - 2 * w);
-        gr->ks = ks, gr->vs = vs, gr->dead = dead;
-        if (dead && page != -2) report_error(L.status, DEV_BAD_BLOCK, 1, page);
-      }
+    if (i >= cnt) return;
+    const int w = i & 15, st = i % kStages;
+    if (w == 0 && i > 0) {
+      page = page_n, ks = ks_n, vs = vs_n;
+      page_n = page_at(2 * (t0 + i) + 32 + lane);
     }
-    cp_async_commit();
+    if (w == 8) scales_at(page_n, ks_n, vs_n);
+    // the lanes that know the tile's groups describe them and load them (both by one, when they are
+    // in one block); a block outside the cache is not loaded
+    const int a = lane - 2 * w;
+    const bool mine = a == 0 || a == 1;
+    const bool dead = page < 0 || page >= c.blocks;
+    if (mine) {
+      Group* gr = groups + st * 2 + a;
+      gr->ks = ks, gr->vs = vs, gr->dead = dead;
+      if (dead && page != -2) report_error(L.status, DEV_BAD_BLOCK, 1, page);
+    }
+    const uint32_t live = __ballot_sync(0xffffffffu, (ONE ? a == 0 : mine) && !dead);
+    constexpr int box = ONE ? kTile : 16;
+    if (lane == 0) mbar_arrive_expect_tx(full + st, (uint32_t)(__popc(live) * 2 * box * DT));
+    __syncwarp();
+    if (live >> lane & 1) {
+      const int tok = (t0 + i) * kTile + 16 * a;
+      const int y = ((page * c.H + hk) << log2t) + (tok & ((1 << log2t) - 1));
+      uint8_t* to = ring + st * sbytes + 16 * a * DT;
+      tc::tma_load_2d(to, &mk, 0, y, full + st);
+      tc::tma_load_2d(to + tile_bytes, &mv, 0, y, full + st);
+    }
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) issue(i);
 
+  bool lost = false;
+  int lost_at = 0;
   for (int i = 0; i < cnt; ++i) {
-    cp_async_wait<kStages - 2>();
+    const int stg = i % kStages;
+    if (!mbar_wait_bounded(full + stg, (uint32_t)(i / kStages) & 1u)) {
+      if (lane == 0) report_error(L.status, DEV_TIMEOUT, 70, i);
+      lost = true, lost_at = i;
+      break;
+    }
     __syncwarp();
     issue(i + kStages - 1);  // into the stage that the previous tile has left
-    uint8_t* st = ring + (i % kStages) * sbytes;
-    const Group* gr = reinterpret_cast<const Group*>(st + 2 * tile_bytes);
-    const uint32_t kb = smem_u32(st), vb = kb + (uint32_t)tile_bytes;
+    const Group* gr = groups + stg * 2;
+    const uint32_t kb = smem_u32(ring + stg * sbytes) + chunk0_at<DT>(lane), vb = kb + (uint32_t)tile_bytes;
     const int tok0 = (t0 + i) * kTile;
 
     // S^T: two 16-token groups
     float s[2][NT][4];
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
+    for (int k = 0; k < CH; ++k) {
+      uint32_t u[4];  // tokens 0-7, 8-15 of the first and the second group, channels 16 k ..
+      ldsm4(u, kb ^ (uint32_t)(16 * k));
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[a][n][e] = 0.f;
-      const uint32_t row = kb + (uint32_t)((16 * a + (lane & 15)) * pitch);
-#pragma unroll
-      for (int k = 0; k < CH; ++k) {
-        if (k >= ch) break;
-        uint32_t u[2];  // tokens 0-7 and 8-15 of the group, channels 16 k ..
-        ldsm2(u, row + 16 * k);
-        u[0] = prep<FMT>(u[0]), u[1] = prep<FMT>(u[1]);
-        const uint32_t f[4] = {codes2<FMT, 0x4140>(u[0]), codes2<FMT, 0x4140>(u[1]), codes2<FMT, 0x4342>(u[0]),
-                               codes2<FMT, 0x4342>(u[1])};
+      for (int a = 0; a < 2; ++a) {
+        uint32_t f[4];
+        codes4_any<FMT>(u[2 * a], f[0], f[2]);
+        codes4_any<FMT>(u[2 * a + 1], f[1], f[3]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+          if (k == 0) mma0(s[a][n], f, qh[n][k]);
+          else mma(s[a][n], f, qh[n][k]);
           if constexpr (SPLIT) mma(s[a][n], f, ql[n][k]);
-          mma(s[a][n], f, qh[n][k]);
         }
       }
     }
@@ -323,8 +342,8 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const __grid_co
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
         const float mn = fmaxf(m[n][e], x);
-        const float ref = mn == -INFINITY ? 0.f : mn;
-        al[n][e] = ex2f(m[n][e] - ref);
+        const float ref = (mn == -INFINITY ? 0.f : mn) - kPShift;
+        al[n][e] = ex2f(m[n][e] - kPShift - ref);
         moved = moved || mn != m[n][e];
         m[n][e] = mn;
         float sum = 0.f;
@@ -332,7 +351,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const __grid_co
         for (int a = 0; a < 2; ++a)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            s[a][n][e + 2 * y] = ex2f(s[a][n][e + 2 * y] - ref + kPShift);
+            s[a][n][e + 2 * y] = ex2f(s[a][n][e + 2 * y] - ref);
             sum += s[a][n][e + 2 * y];
           }
         l[n][e] = l[n][e] * al[n][e] + sum;
@@ -362,55 +381,62 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const __grid_co
         }
     // O^T += vscale * (V^T P^T), each block's part from a fresh accumulator
     const float vs0 = gr[0].vs, vs1 = gr[1].vs;
-    // A block whose scale is not finite reaches only the rows that see it.
+    // A block whose scale is not finite reaches only the rows that see it: the others' p and partial sum
+    // are 0, and so is their factor.
     const bool odd = !(fabsf(vs0) <= 3.4028234e38f) || !(fabsf(vs1) <= 3.4028234e38f);
-    bool sees[2][NT][2];
-    if (odd) {
+    float vf[ONE ? 1 : 2][NT][2];
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < (ONE ? 1 : 2); ++a)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) sees[a][n][e] = tok0 + 16 * a <= lim[n][e];
+        for (int e = 0; e < 2; ++e) vf[a][n][e] = odd && tok0 + 16 * a > lim[n][e] ? 0.f : a ? vs1 : vs0;
+    // Bytes after the last token may be anything, NaN codes among them, and 0 * NaN is not 0: the lane's
+    // tokens 2t, 2t + 1 of each eight are the halves of its words.
+    uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+    const bool cut = FMT == kCacheE4m3 && (tok0 + kTile > seen || gr[0].dead || gr[1].dead);
+    if (cut) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int tok = tok0 + 8 * j + 2 * t;
+        keep[j] = gr[j >> 1].dead ? 0u : (tok < seen ? 0xffffu : 0u) | (tok + 1 < seen ? 0xffff0000u : 0u);
+      }
     }
-    const uint32_t vrow = vb + (uint32_t)((lane & 15) * pitch);
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      if (k >= ch) break;
       float acc[NT][4];
+      uint32_t u[4];  // as for K, transposed: the lane has tokens 2t, 2t + 1 of each eight and channels 2g,
+                      // 2g + 1 of the chunk, which are rows g and g + 8 of the MMA
+      ldsm4t(u, vb ^ (uint32_t)(16 * k));
+      if (cut) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] &= keep[j];
+      }
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
-        if (a == 0 || !ONE) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-        }
-        uint32_t u[2];  // tokens 0-7 and 8-15 of the group, transposed: lane has tokens 2t, 2t + 1 and
-                        // channels 2g, 2g + 1 of the chunk, which are rows g and g + 8 of the MMA
-        ldsm2t(u, vrow + (uint32_t)(16 * a * pitch) + 16 * k);
-        u[0] = prep<FMT>(u[0]), u[1] = prep<FMT>(u[1]);
-        const uint32_t f[4] = {codes2<FMT, 0x4240>(u[0]), codes2<FMT, 0x4341>(u[0]), codes2<FMT, 0x4240>(u[1]),
-                               codes2<FMT, 0x4341>(u[1])};
+        uint32_t f[4];
+        codes4<FMT>(u[2 * a], f[0], f[1]);
+        codes4<FMT>(u[2 * a + 1], f[2], f[3]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+          if (a == 0 || !ONE) mma0(acc[n], f, ph[a][n]);
+          else mma(acc[n], f, ph[a][n]);
           if constexpr (SPLIT) mma(acc[n], f, pl[a][n]);
-          mma(acc[n], f, ph[a][n]);
         }
         if (a == 1 || !ONE) {
-          const float v = ONE ? vs0 : a ? vs1 : vs0;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (odd && !sees[ONE ? 0 : a][n][e & 1]) continue;
-              o[k][n][e] = fmaf(v, acc[n][e], o[k][n][e]);
-            }
+            for (int e = 0; e < 4; ++e) o[k][n][e] = fmaf(vf[ONE ? 0 : a][n][e & 1], acc[n][e], o[k][n][e]);
         }
       }
     }
   }
-  cp_async_wait<0>();
+  // (every copy has landed: each was waited for, but after a wait that ran out, when those in flight are
+  // given their time before the ring is used again)
+  if (lost) {
+    for (int i = lost_at; i < min(cnt, lost_at + kStages); ++i) mbar_wait_bounded(full + i % kStages, (uint32_t)(i / kStages) & 1u);
+  }
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -422,11 +448,11 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const __grid_co
   __syncthreads();  // every warp has left its ring
 
   // ---- join: the CTA's warps, then the cluster's CTAs ----
-  // shared memory: O of each warp [kWarps][NR][DT], then (m, l) [kWarps][NR]; the CTA's own sums
+  // shared memory: O of each warp [W][NR][DT], then (m, l) [W][NR]; the CTA's own sums
   // [NR][DT] and (m, l) [NR] follow
   float* wo = reinterpret_cast<float*>(smem);
-  float2* wml = reinterpret_cast<float2*>(wo + kWarps * NR * DT);
-  float* co = reinterpret_cast<float*>(wml + kWarps * NR);
+  float2* wml = reinterpret_cast<float2*>(wo + W * NR * DT);
+  float* co = reinterpret_cast<float*>(wml + W * NR);
   float2* cml = reinterpret_cast<float2*>(co + NR * DT);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -446,14 +472,14 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const __grid_co
     const int pr = r0 + r;
     out[(q.row0 + pr / L.G) * L.ldo + (int64_t)(hk * L.G + pr % L.G) * D + d] = from_f32<T>(x);
   };
-  for (int idx = threadIdx.x; idx < nrow * D; idx += kWarps * 32) {
+  for (int idx = threadIdx.x; idx < nrow * D; idx += W * 32) {
     const int r = idx / D, d = idx - r * D;
     float mx = -INFINITY, sum = 0.f, x = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, wml[w * NR + r].x);
+    for (int w = 0; w < W; ++w) mx = fmaxf(mx, wml[w * NR + r].x);
     const float ref = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float2 ml = wml[w * NR + r];
       const float f = ex2f(ml.x - ref);
       sum = fmaf(ml.y, f, sum);
@@ -468,7 +494,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const __grid_co
   }
   if (csize > 1) {
     cluster.sync();
-    for (int idx = crank * kWarps * 32 + threadIdx.x; idx < nrow * D; idx += csize * kWarps * 32) {
+    for (int idx = crank * W * 32 + threadIdx.x; idx < nrow * D; idx += csize * W * 32) {
       const int r = idx / D, d = idx - r * D;
       float mx = -INFINITY, sum = 0.f, x = 0.f;
       for (int k = 0; k < csize; ++k) mx = fmaxf(mx, cluster.map_shared_rank(cml, k)[r].x);
@@ -485,31 +511,28 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attn_kernel(const __grid_co
   }
 }
 
-template <int NT>
-size_t smem_of(int D, int DT) {
-  const size_t ring = (size_t)kWarps * kStages * stage_bytes(D);
-  const size_t join = (size_t)(kWarps + 1) * (8 * NT) * (DT * sizeof(float) + sizeof(float2));
-  return ring > join ? ring : join;
+template <int NT, int W>
+constexpr size_t smem_of(int DT) {
+  const size_t ring = (size_t)W * (kStages * stage_bytes(DT) + kWarpBytes);
+  const size_t join = (size_t)(W + 1) * (8 * NT) * (DT * sizeof(float) + sizeof(float2));
+  return (ring > join ? ring : join) + 1024;  // (the base is moved to a 1024-byte boundary)
 }
 
-template <typename T, int FMT, int DT, int NT, bool ONE>
-cudaError_t attn_as(const CacheAttnLaunch& L, cudaStream_t s) {
+template <typename T, int FMT, int DT, int NT, bool ONE, int W>
+cudaError_t attn_as(const CacheAttnLaunch& L, int split, cudaStream_t s) {
   const int64_t rows = (int64_t)L.s.max_rows * L.G;
   const int tiles = (int)((rows + 8 * NT - 1) / (8 * NT));
   const int64_t units = (int64_t)L.s.B * L.c.H * tiles;
-  // CTAs that split one unit: enough to fill the SMs several times over, each left with at least 256
-  // tokens of the longest sequence
-  int split = 1;
-  while (split < 16 && units * split < 148 * 8 && (int64_t)L.s.max_len >= (int64_t)split * 2 * 256) split *= 2;
   if (units * split > INT32_MAX) return cudaErrorInvalidValue;
-  auto kernel = cache_attn_kernel<T, FMT, DT, NT, ONE>;
-  const size_t smem = smem_of<NT>(L.c.D, DT);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of<NT>(DT, DT));
+  auto kernel = cache_attn_kernel<T, FMT, DT, NT, ONE, W>;
+  constexpr size_t smem = smem_of<NT, W>(DT);
+  static_assert(smem <= 227 * 1024, "shared memory");
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e == cudaSuccess && split > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * split));
-  cfg.blockDim = dim3(kWarps * 32);
+  cfg.blockDim = dim3(W * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -518,12 +541,26 @@ cudaError_t attn_as(const CacheAttnLaunch& L, cudaStream_t s) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, L, tiles);
+  return cudaLaunchKernelEx(&cfg, kernel, L, L.mk, L.mv, tiles);
+}
+
+template <typename T, int FMT, int DT, int NT, bool ONE>
+cudaError_t attn_one(const CacheAttnLaunch& L, cudaStream_t s) {
+  const int64_t rows = (int64_t)L.s.max_rows * L.G;
+  const int64_t units = (int64_t)L.s.B * L.c.H * ((rows + 8 * NT - 1) / (8 * NT));
+  // CTAs that split one unit: enough to fill the SMs several times over, each left with at least 256
+  // tokens of the longest sequence
+  int split = 1;
+  while (split < 16 && units * split < 148 * 8 && (int64_t)L.s.max_len >= (int64_t)split * 2 * 256) split *= 2;
+  if constexpr (NT == 1) {
+    if (units * split <= 148) return attn_as<T, FMT, DT, NT, ONE, 8>(L, split, s);
+  }
+  return attn_as<T, FMT, DT, NT, ONE, 4>(L, split, s);
 }
 
 template <typename T, int FMT, int DT, int NT>
 cudaError_t attn_nt(const CacheAttnLaunch& L, cudaStream_t s) {
-  return L.c.log2t >= 5 ? attn_as<T, FMT, DT, NT, true>(L, s) : attn_as<T, FMT, DT, NT, false>(L, s);
+  return L.c.log2t >= 5 ? attn_one<T, FMT, DT, NT, true>(L, s) : attn_one<T, FMT, DT, NT, false>(L, s);
 }
 template <typename T, int FMT>
 cudaError_t attn_fmt(const CacheAttnLaunch& L, cudaStream_t s) {

@@ -362,7 +362,7 @@ int check_cache_attn(supra_attn_ctx* c, const supra_attn_cache_attn_desc* d, Che
   call->kind = CacheCall::ATTENTION;
   call->type = d->type;
   call->format = d->cache.format;
-  CacheAttnLaunch& L = call->attn;
+  CacheAttnArgs& L = call->attn;
   int rc = check_type(c, what, d->type);
   if (!rc) rc = check_cache(c, what, d->cache, &L.c);
   if (!rc) rc = check_seqs(c, what, d->seqs, d->cache.block_tokens, &L.s);
@@ -371,6 +371,8 @@ int check_cache_attn(supra_attn_ctx* c, const supra_attn_cache_attn_desc* d, Che
     return set_err(c, SUPRA_ATTN_EINVAL, "%s: H=%d must be a multiple of the cache's H=%d", what, d->H, d->cache.H);
   const float scale = d->flags & SUPRA_ATTN_CA_DEFAULT_SCALE ? (float)(1.0 / std::sqrt((double)d->cache.D)) : d->scale;
   if (!std::isfinite(scale)) return set_err(c, SUPRA_ATTN_EINVAL, "%s: scale must be finite", what);
+  if (((int64_t)d->cache.blocks * d->cache.H << L.c.log2t) > INT32_MAX)
+    return set_err(c, SUPRA_ATTN_EINVAL, "%s: blocks*H*block_tokens must be below 2^31", what);
   const int es = esize(d->type);
   const int64_t width = (int64_t)d->H * d->cache.D, rows = d->seqs.rows;
   rc = check_rows(c, what, "q", d->q, d->q_size, d->ldq, d->q_off, rows, width, es);
@@ -426,10 +428,17 @@ int flush_cache(supra_attn_ctx* c, std::vector<const Queued*>& g) {
         break;
       }
       case CacheCall::ATTENTION: {
-        call.attn.status = c->d_status;
-        name = cache_attn_name(call.attn, call.type);
+        CacheAttnLaunch L;
+        static_cast<CacheAttnArgs&>(L) = call.attn;
+        L.status = c->d_status;
+        name = cache_attn_name(L, call.type);
+        const int64_t tokens = ((int64_t)L.c.blocks * L.c.H) << L.c.log2t;
+        const int cols = cache_attn_box_cols(L.c.D), rows = cache_attn_box_rows(L.c.log2t);
+        if (!encode_byte_map(&L.mk, L.c.k, tokens, L.c.D, cols, rows) ||
+            !encode_byte_map(&L.mv, L.c.v, tokens, L.c.D, cols, rows))
+          return set_err(c, SUPRA_ATTN_ECUDA, "cuTensorMapEncodeTiled failed");
         ProfScope ps(c, name, q->flops, q->bytes);
-        e = launch_cache_attn(call.attn, call.type, call.format, c->stream);
+        e = launch_cache_attn(L, call.type, call.format, c->stream);
         break;
       }
     }

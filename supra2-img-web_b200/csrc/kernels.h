@@ -352,7 +352,7 @@ struct CacheRowsLaunch {
 cudaError_t launch_cache_write(const CacheRowsLaunch& L, int type, int format, bool vec, cudaStream_t s);
 cudaError_t launch_cache_read(const CacheRowsLaunch& L, int type, int format, bool vec, cudaStream_t s);
 
-struct CacheAttnLaunch {
+struct CacheAttnArgs {
   CachePool c;
   CacheSeqs s;
   const void* q;
@@ -363,6 +363,13 @@ struct CacheAttnLaunch {
   int32_t causal;
   int32_t* status;
 };
+// Boxes of the K and V pools, seen as [blocks * H * block_tokens, D] bytes: cache_attn_box_cols(D)
+// columns (zeros past D) with the swizzle of that many bytes, and rows of a tile inside one block.
+struct CacheAttnLaunch : CacheAttnArgs {
+  CUtensorMap mk, mv;
+};
+inline int cache_attn_box_cols(int D) { return D <= 64 ? 64 : 128; }
+inline int cache_attn_box_rows(int log2t) { return log2t >= 5 ? 32 : 16; }
 cudaError_t launch_cache_attn(const CacheAttnLaunch& L, int type, int format, cudaStream_t s);
 const char* cache_attn_name(const CacheAttnLaunch& L, int type);
 
