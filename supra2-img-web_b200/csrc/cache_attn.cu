@@ -19,8 +19,12 @@
 // blocks), swizzled so that ldmatrix meets no bank conflicts, its channels past D filled with zeros. 4
 // warps form a CTA and 1 to 16 CTAs a cluster that splits one (sequence, cache head, 8 or 16 query
 // rows). The cluster joins its parts through distributed shared memory: no workspace, no atomics, the
-// same order every time.
+// same order every time. Where so few units meet so long a cache that 16 CTAs each leave SMs idle, the
+// CTAs are launched without clusters, as many as fill the SMs, write their parts to a workspace that
+// lives from the launch to the join, and a second kernel joins them in order.
 #include <cooperative_groups.h>
+
+#include <algorithm>
 
 #include "cache.cuh"
 #include "tcgen05.cuh"
@@ -130,7 +134,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   cg::cluster_group cluster = cg::this_cluster();
-  const int crank = (int)cluster.block_rank(), csize = (int)cluster.num_blocks();
+  const int csize = L.splits, crank = blockIdx.x % csize;  // (the rank in the cluster, where there is one)
 
   // unit = (sequence, cache head, row tile); the whole cluster has the same one
   int unit = blockIdx.x / csize;
@@ -487,12 +491,16 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
     }
     if (csize == 1) {
       store(r, d, sum == 0.f ? 0.f : x / sum);
+    } else if (L.ws_o) {
+      const int64_t at = (int64_t)blockIdx.x * NR + r;
+      L.ws_o[at * D + d] = x;
+      if (d == 0) L.ws_ml[at] = make_float2(mx, sum);
     } else {
       co[r * DT + d] = x;
       if (d == 0) cml[r] = make_float2(mx, sum);
     }
   }
-  if (csize > 1) {
+  if (csize > 1 && !L.ws_o) {
     cluster.sync();
     for (int idx = crank * W * 32 + threadIdx.x; idx < nrow * D; idx += csize * W * 32) {
       const int r = idx / D, d = idx - r * D;
@@ -511,6 +519,57 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
   }
 }
 
+// Joins the workspace's parts of one row of one unit, always in the same order: warp w takes splits w, w + 8,
+// .. (lane: 4 channels), then the warps are added up.
+template <typename T>
+__global__ void __launch_bounds__(256) cache_attn_join(const __grid_constant__ CacheAttnArgs L, int tiles, int NR) {
+  __shared__ float4 po[8][32];
+  __shared__ float2 pml[8];
+  const CachePool& c = L.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int unit = blockIdx.x;
+  const int64_t part0 = (int64_t)unit * L.splits;
+  const int rt = unit % tiles;
+  unit /= tiles;
+  const int hk = unit % c.H, b = unit / c.H;
+  SeqView q;
+  if (!seq_view(L.s, b, false, L.status, q)) return;
+  const int pr = rt * NR + blockIdx.y;
+  if (pr >= q.n * L.G) return;
+  float mx = -INFINITY, sum = 0.f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = warp; s < L.splits; s += 8) {
+    const int64_t at = (part0 + s) * NR + blockIdx.y;
+    const float2 ml = L.ws_ml[at];
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (4 * lane < c.D) v = *reinterpret_cast<const float4*>(L.ws_o + at * c.D + 4 * lane);
+    const float mn = fmaxf(mx, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+    const float f = ex2f(mx - ref), g = ex2f(ml.x - ref);
+    mx = mn;
+    sum = sum * f + ml.y * g;
+    x.x = x.x * f + v.x * g, x.y = x.y * f + v.y * g, x.z = x.z * f + v.z * g, x.w = x.w * f + v.w * g;
+  }
+  po[warp][lane] = x;
+  if (lane == 0) pml[warp] = make_float2(mx, sum);
+  __syncthreads();
+  if (threadIdx.x >= c.D) return;
+  const int d = threadIdx.x;
+  mx = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) mx = fmaxf(mx, pml[w].x);
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float y = 0.f;
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const float f = ex2f(pml[w].x - ref);
+    sum = fmaf(pml[w].y, f, sum);
+    y = fmaf(reinterpret_cast<const float*>(po[w])[d], f, y);
+  }
+  static_cast<T*>(L.o)[(q.row0 + pr / L.G) * L.ldo + (int64_t)(hk * L.G + pr % L.G) * c.D + d] =
+      from_f32<T>(sum == 0.f ? 0.f : y / sum);
+}
+
 template <int NT, int W>
 constexpr size_t smem_of(int DT) {
   const size_t ring = (size_t)W * (kStages * stage_bytes(DT) + kWarpBytes);
@@ -518,70 +577,80 @@ constexpr size_t smem_of(int DT) {
   return (ring > join ? ring : join) + 1024;  // (the base is moved to a 1024-byte boundary)
 }
 
-template <typename T, int FMT, int DT, int NT, bool ONE, int W>
-cudaError_t attn_as(const CacheAttnLaunch& L, int split, cudaStream_t s) {
-  const int64_t rows = (int64_t)L.s.max_rows * L.G;
-  const int tiles = (int)((rows + 8 * NT - 1) / (8 * NT));
-  const int64_t units = (int64_t)L.s.B * L.c.H * tiles;
-  if (units * split > INT32_MAX) return cudaErrorInvalidValue;
-  auto kernel = cache_attn_kernel<T, FMT, DT, NT, ONE, W>;
-  constexpr size_t smem = smem_of<NT, W>(DT);
+constexpr int kW = 4;  // warps of a CTA
+
+template <typename T, int FMT, int DT, int NT, bool ONE>
+cudaError_t attn_as(const CacheAttnLaunch& L, const CacheAttnPlan& P, cudaStream_t s) {
+  auto kernel = cache_attn_kernel<T, FMT, DT, NT, ONE, kW>;
+  constexpr size_t smem = smem_of<NT, kW>(DT);
   static_assert(smem <= 227 * 1024, "shared memory");
+  const int cluster = P.ws_bytes ? 1 : P.splits;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e == cudaSuccess && split > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess && cluster > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units * split));
-  cfg.blockDim = dim3(W * 32);
+  cfg.gridDim = dim3((unsigned)(P.units * P.splits));
+  cfg.blockDim = dim3(kW * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)split;
+  at[0].val.clusterDim.x = (unsigned)cluster;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, L, L.mk, L.mv, tiles);
-}
-
-template <typename T, int FMT, int DT, int NT, bool ONE>
-cudaError_t attn_one(const CacheAttnLaunch& L, cudaStream_t s) {
-  const int64_t rows = (int64_t)L.s.max_rows * L.G;
-  const int64_t units = (int64_t)L.s.B * L.c.H * ((rows + 8 * NT - 1) / (8 * NT));
-  // CTAs that split one unit: enough to fill the SMs several times over, each left with at least 256
-  // tokens of the longest sequence
-  int split = 1;
-  while (split < 16 && units * split < 148 * 8 && (int64_t)L.s.max_len >= (int64_t)split * 2 * 256) split *= 2;
-  if constexpr (NT == 1) {
-    if (units * split <= 148) return attn_as<T, FMT, DT, NT, ONE, 8>(L, split, s);
-  }
-  return attn_as<T, FMT, DT, NT, ONE, 4>(L, split, s);
+  const CacheAttnArgs& A = L;
+  e = cudaLaunchKernelEx(&cfg, kernel, A, L.mk, L.mv, P.tiles);
+  if (e != cudaSuccess || !P.ws_bytes) return e;
+  const int rows = (int)std::min<int64_t>((int64_t)L.s.max_rows * L.G, 8 * NT);
+  cache_attn_join<T><<<dim3((unsigned)P.units, (unsigned)rows), 256, 0, s>>>(A, P.tiles, 8 * NT);
+  return cudaGetLastError();
 }
 
 template <typename T, int FMT, int DT, int NT>
-cudaError_t attn_nt(const CacheAttnLaunch& L, cudaStream_t s) {
-  return L.c.log2t >= 5 ? attn_one<T, FMT, DT, NT, true>(L, s) : attn_one<T, FMT, DT, NT, false>(L, s);
+cudaError_t attn_nt(const CacheAttnLaunch& L, const CacheAttnPlan& P, cudaStream_t s) {
+  return L.c.log2t >= 5 ? attn_as<T, FMT, DT, NT, true>(L, P, s) : attn_as<T, FMT, DT, NT, false>(L, P, s);
 }
 template <typename T, int FMT>
-cudaError_t attn_fmt(const CacheAttnLaunch& L, cudaStream_t s) {
-  const bool wide = (int64_t)L.s.max_rows * L.G > 8;
-  if (L.c.D <= 64) return wide ? attn_nt<T, FMT, 64, 2>(L, s) : attn_nt<T, FMT, 64, 1>(L, s);
-  return wide ? attn_nt<T, FMT, 128, 2>(L, s) : attn_nt<T, FMT, 128, 1>(L, s);
+cudaError_t attn_fmt(const CacheAttnLaunch& L, const CacheAttnPlan& P, cudaStream_t s) {
+  if (L.c.D <= 64) return P.nt == 2 ? attn_nt<T, FMT, 64, 2>(L, P, s) : attn_nt<T, FMT, 64, 1>(L, P, s);
+  return P.nt == 2 ? attn_nt<T, FMT, 128, 2>(L, P, s) : attn_nt<T, FMT, 128, 1>(L, P, s);
 }
 template <typename T>
-cudaError_t attn_type(const CacheAttnLaunch& L, int format, cudaStream_t s) {
-  return format == kCacheInt8 ? attn_fmt<T, kCacheInt8>(L, s) : attn_fmt<T, kCacheE4m3>(L, s);
+cudaError_t attn_type(const CacheAttnLaunch& L, const CacheAttnPlan& P, int format, cudaStream_t s) {
+  return format == kCacheInt8 ? attn_fmt<T, kCacheInt8>(L, P, s) : attn_fmt<T, kCacheE4m3>(L, P, s);
 }
 
 }  // namespace
 
-cudaError_t launch_cache_attn(const CacheAttnLaunch& L, int type, int format, cudaStream_t s) {
-  if (type == kTypeF32) return attn_type<float>(L, format, s);
-  if (type == kTypeF16) return attn_type<__half>(L, format, s);
-  return attn_type<__nv_bfloat16>(L, format, s);
+CacheAttnPlan plan_cache_attn(const CacheAttnArgs& L) {
+  CacheAttnPlan P = {};
+  const int64_t rows = (int64_t)L.s.max_rows * L.G;
+  P.nt = rows > 8 ? 2 : 1;
+  P.tiles = (int)((rows + 8 * P.nt - 1) / (8 * P.nt));
+  P.units = (int64_t)L.s.B * L.c.H * P.tiles;
+  // CTAs that split one unit: enough to fill the SMs several times over, each left with at least 256
+  // tokens of the longest sequence
+  P.splits = 1;
+  while (P.splits < 16 && P.units * P.splits < 148 * 8 && L.s.max_len >= P.splits * 2 * 256) P.splits *= 2;
+  // Without clusters: one wave of three CTAs per SM, each left with 512 tokens. Worth the second launch
+  // where it is well over 16 CTAs a unit.
+  const int64_t wide = std::min<int64_t>(148 * 3 / std::max<int64_t>(P.units, 1), L.s.max_len / 512);
+  if (wide >= 20) {
+    P.splits = (int)wide;
+    P.ws_bytes = (size_t)(P.units * wide * 8 * P.nt) * (L.c.D * sizeof(float) + sizeof(float2));
+  }
+  return P;
 }
-const char* cache_attn_name(const CacheAttnLaunch& L, int type) {
-  (void)L;
+
+cudaError_t launch_cache_attn(const CacheAttnLaunch& L, const CacheAttnPlan& P, int type, int format, cudaStream_t s) {
+  if (P.units * P.splits > INT32_MAX) return cudaErrorInvalidValue;
+  if (type == kTypeF32) return attn_type<float>(L, P, format, s);
+  if (type == kTypeF16) return attn_type<__half>(L, P, format, s);
+  return attn_type<__nv_bfloat16>(L, P, format, s);
+}
+const char* cache_attn_name(const CacheAttnPlan& P, int type) {
+  (void)P;
   return type == kTypeF32 ? "cache_attention_rows_fp32" : "cache_attention_rows";
 }
 

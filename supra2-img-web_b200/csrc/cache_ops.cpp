@@ -148,6 +148,32 @@ int check_overlap(supra_attn_ctx* c, const char* what, const Checked& ck) {
   return SUPRA_ATTN_OK;
 }
 
+// Device memory for one launch, ordered on the context's stream and given back after it. It comes from a
+// pool of the context that keeps what it has; inside a stream capture it becomes the graph's own, so
+// no two graphs share it.
+int scratch_alloc(supra_attn_ctx* c, size_t bytes, void** p) {
+  cudaError_t e = cudaSuccess;
+  if (!c->async_pool) {
+    cudaMemPoolProps props = {};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = c->device;
+    e = cudaMemPoolCreate(&c->async_pool, &props);
+    if (e != cudaSuccess) {
+      c->async_pool = nullptr;
+      return cuda_err(c, e, "cache_attention: memory pool");
+    }
+    uint64_t keep = UINT64_MAX;
+    cudaMemPoolSetAttribute(c->async_pool, cudaMemPoolAttrReleaseThreshold, &keep);
+  }
+  e = cudaMallocFromPoolAsync(p, bytes, c->async_pool, c->stream);
+  if (e == cudaErrorMemoryAllocation) {
+    cudaGetLastError();
+    return set_err(c, SUPRA_ATTN_ENOMEM, "cache_attention: workspace of %zu bytes failed", bytes);
+  }
+  return e == cudaSuccess ? SUPRA_ATTN_OK : cuda_err(c, e, "cache_attention: workspace");
+}
+
 void queue_entry(Checked* out, double flops, double bytes) {
   std::memset(&out->q, 0, sizeof out->q);
   out->q.path = PATH_CACHE;
@@ -431,14 +457,30 @@ int flush_cache(supra_attn_ctx* c, std::vector<const Queued*>& g) {
         CacheAttnLaunch L;
         static_cast<CacheAttnArgs&>(L) = call.attn;
         L.status = c->d_status;
-        name = cache_attn_name(L, call.type);
+        const CacheAttnPlan plan = plan_cache_attn(L);
+        name = cache_attn_name(plan, call.type);
         const int64_t tokens = ((int64_t)L.c.blocks * L.c.H) << L.c.log2t;
         const int cols = cache_attn_box_cols(L.c.D), rows = cache_attn_box_rows(L.c.log2t);
         if (!encode_byte_map(&L.mk, L.c.k, tokens, L.c.D, cols, rows) ||
             !encode_byte_map(&L.mv, L.c.v, tokens, L.c.D, cols, rows))
           return set_err(c, SUPRA_ATTN_ECUDA, "cuTensorMapEncodeTiled failed");
-        ProfScope ps(c, name, q->flops, q->bytes);
-        e = launch_cache_attn(L, call.type, call.format, c->stream);
+        L.splits = plan.splits;
+        void* ws = nullptr;
+        if (plan.ws_bytes) {
+          int rc = scratch_alloc(c, plan.ws_bytes, &ws);
+          if (rc) return rc;
+          L.ws_o = static_cast<float*>(ws);
+          L.ws_ml = reinterpret_cast<float2*>(L.ws_o + plan.units * plan.splits * 8 * plan.nt * L.c.D);
+          c->launches += 1;  // the join
+        }
+        {
+          ProfScope ps(c, name, q->flops, q->bytes);
+          e = launch_cache_attn(L, plan, call.type, call.format, c->stream);
+        }
+        if (ws) {
+          const cudaError_t f = cudaFreeAsync(ws, c->stream);
+          if (e == cudaSuccess) e = f;
+        }
         break;
       }
     }

@@ -243,6 +243,7 @@ struct supra_attn_ctx {
   std::unordered_map<void*, size_t> pool_live;
   std::unordered_set<void*> host_live;
 
+  cudaMemPool_t async_pool = nullptr;  // cache_attention's workspaces (cache_ops.cpp)
   float* scratch = nullptr;
   size_t scratch_cap = 0;
   size_t scratch_budget = size_t(64) << 20;  // per chunk of score-materialising units

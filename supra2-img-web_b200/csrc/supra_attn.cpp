@@ -286,6 +286,7 @@ int supra_attn_destroy(supra_attn_ctx* c) {
     for (void* p : kv.second) cudaFree(p);
   for (auto& kv : c->pool_live) cudaFree(kv.first);
   for (void* p : c->host_live) cudaFreeHost(p);
+  if (c->async_pool) cudaMemPoolDestroy(c->async_pool);
   if (c->scratch) cudaFree(c->scratch);
   if (c->gn_stats) cudaFree(c->gn_stats);
   if (c->lin_split) cudaFree(c->lin_split);

@@ -285,6 +285,46 @@ def test_attention_split_along_the_cache(gpu, T, lengths, rows, dtype):
     check_attention(gpu, "e4m3", dtype, T, 1, 2, 128, lengths, rows, False, seed=4)
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_attention_split_over_many_ctas(gpu, dtype):
+    """Few rows over a cache so long that the parts are joined through a workspace."""
+    check_attention(gpu, "int8", dtype, 64, 1, 2, 64, [11000, 300, 0], [1, 1, 1], True, seed=20)
+    check_attention(gpu, "e4m3", dtype, 16, 1, 8, 128, [10753], [3], True, seed=21)
+
+
+def test_captured_split_over_many_ctas(gpu):
+    """The workspace inside a capture is the graph's own: two graphs and eager calls give the same bits."""
+    rng = np.random.default_rng(22)
+    p = Pool(gpu, rng, "int8", 128, 1, 64, [12000])
+    side = torch.cuda.Stream()
+    ctx = supra_attn.GPU(0, stream=side)
+    cache = supra_attn.KVCache(ctx, p.blocks, 1, 64, block_tokens=128, format="int8", k=p.d[0], v=p.d[1], k_scale=p.d[2], v_scale=p.d[3])
+    seqs = supra_attn.CacheBatch(ctx, p.d_len, p.d_table)
+    q = torch.randn(1, 128, device="cuda")
+    outs = [torch.zeros(1, 128, device="cuda") for _ in range(3)]
+    torch.cuda.synchronize()
+    supra_attn.cache_attention(ctx, cache, seqs, q=q, H=2, out=outs[2])
+    ctx.sync()
+    graphs = []
+    for o in outs[:2]:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            supra_attn.cache_attention(ctx, cache, seqs, q=q, H=2, out=o)
+            ctx.flush()
+    others = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):  # both at once, each on a stream of its own
+        for g, s in zip(graphs, others):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[2])
+    ref, pv, av, st, sm = oc.attention("int8", p.kc, p.ks, p.vc, p.vs, q.cpu().double().numpy().reshape(1, 2, 64), [12000], [0, 1], p.table,
+                                       0.125, False)
+    assert (np.abs(outs[2].cpu().double().numpy().reshape(1, 2, 64) - ref) <= attention_bound("fp32", 64, 12000, ref, pv, av, st, sm)).all()
+    del graphs
+    ctx.close()
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_attention_scale_and_sharp_scores(gpu, dtype):
     check_attention(gpu, "int8", dtype, 64, 2, 2, 64, [300, 40], [5, 33], True, scale=0.25, seed=5, sharp=4.0)
