@@ -522,14 +522,14 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
 // Joins the workspace's parts of one row of one unit, always in the same order: warp w takes splits w, w + 8,
 // .. (lane: 4 channels), then the warps are added up.
 template <typename T>
-__global__ void __launch_bounds__(256) cache_attn_join(const __grid_constant__ CacheAttnArgs L, int tiles, int NR) {
+__global__ void __launch_bounds__(256) cache_attn_join(const __grid_constant__ CacheAttnArgs L, int tiles, int NR, bool last_first) {
   __shared__ float4 po[8][32];
   __shared__ float2 pml[8];
   const CachePool& c = L.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int unit = blockIdx.x;
   const int64_t part0 = (int64_t)unit * L.splits;
-  const int rt = unit % tiles;
+  const int rt = last_first ? tiles - 1 - unit % tiles : unit % tiles;
   unit /= tiles;
   const int hk = unit % c.H, b = unit / c.H;
   SeqView q;
@@ -601,10 +601,7 @@ cudaError_t attn_as(const CacheAttnLaunch& L, const CacheAttnPlan& P, cudaStream
   cfg.numAttrs = 1;
   const CacheAttnArgs& A = L;
   e = cudaLaunchKernelEx(&cfg, kernel, A, L.mk, L.mv, P.tiles);
-  if (e != cudaSuccess || !P.ws_bytes) return e;
-  const int rows = (int)std::min<int64_t>((int64_t)L.s.max_rows * L.G, 8 * NT);
-  cache_attn_join<T><<<dim3((unsigned)P.units, (unsigned)rows), 256, 0, s>>>(A, P.tiles, 8 * NT);
-  return cudaGetLastError();
+  return e;
 }
 
 template <typename T, int FMT, int DT, int NT>
@@ -613,8 +610,8 @@ cudaError_t attn_nt(const CacheAttnLaunch& L, const CacheAttnPlan& P, cudaStream
 }
 template <typename T, int FMT>
 cudaError_t attn_fmt(const CacheAttnLaunch& L, const CacheAttnPlan& P, cudaStream_t s) {
-  if (L.c.D <= 64) return P.nt == 2 ? attn_nt<T, FMT, 64, 2>(L, P, s) : attn_nt<T, FMT, 64, 1>(L, P, s);
-  return P.nt == 2 ? attn_nt<T, FMT, 128, 2>(L, P, s) : attn_nt<T, FMT, 128, 1>(L, P, s);
+  if (L.c.D <= 64) return P.nr == 16 ? attn_nt<T, FMT, 64, 2>(L, P, s) : attn_nt<T, FMT, 64, 1>(L, P, s);
+  return P.nr == 16 ? attn_nt<T, FMT, 128, 2>(L, P, s) : attn_nt<T, FMT, 128, 1>(L, P, s);
 }
 template <typename T>
 cudaError_t attn_type(const CacheAttnLaunch& L, const CacheAttnPlan& P, int format, cudaStream_t s) {
@@ -626,31 +623,44 @@ cudaError_t attn_type(const CacheAttnLaunch& L, const CacheAttnPlan& P, int form
 CacheAttnPlan plan_cache_attn(const CacheAttnArgs& L) {
   CacheAttnPlan P = {};
   const int64_t rows = (int64_t)L.s.max_rows * L.G;
-  P.nt = rows > 8 ? 2 : 1;
-  P.tiles = (int)((rows + 8 * P.nt - 1) / (8 * P.nt));
+  P.tc = rows > 64;
+  P.nr = P.tc ? cache_attn_tc_rows(L.c.D) : rows > 8 ? 16 : 8;
+  P.tiles = (int)((rows + P.nr - 1) / P.nr);
   P.units = (int64_t)L.s.B * L.c.H * P.tiles;
-  // CTAs that split one unit: enough to fill the SMs several times over, each left with at least 256
-  // tokens of the longest sequence
   P.splits = 1;
-  while (P.splits < 16 && P.units * P.splits < 148 * 8 && L.s.max_len >= P.splits * 2 * 256) P.splits *= 2;
-  // Without clusters: one wave of three CTAs per SM, each left with 512 tokens. Worth the second launch
-  // where it is well over 16 CTAs a unit.
-  const int64_t wide = std::min<int64_t>(148 * 3 / std::max<int64_t>(P.units, 1), L.s.max_len / 512);
-  if (wide >= 20) {
-    P.splits = (int)wide;
-    P.ws_bytes = (size_t)(P.units * wide * 8 * P.nt) * (L.c.D * sizeof(float) + sizeof(float2));
+  const int wave = P.tc ? (L.c.D <= 64 ? 148 * 2 : 148) : 148 * 3;  // CTAs that run at once
+  const int64_t wide = std::min<int64_t>(wave / std::max<int64_t>(P.units, 1), L.s.max_len / 512);
+  if (P.tc) {
+    // fewer units than run at once, each with many tiles of tokens: split them
+    if (wide >= 2) P.splits = (int)wide;
+  } else {
+    // CTAs of a cluster that split one unit: enough to fill the SMs several times over, each left with
+    // at least 256 tokens of the longest sequence
+    while (P.splits < 16 && P.units * P.splits < 148 * 8 && L.s.max_len >= P.splits * 2 * 256) P.splits *= 2;
+    // Without clusters: one wave of three CTAs per SM, each left with 512 tokens. Worth the second
+    // launch where it is well over 16 CTAs a unit.
+    if (wide >= 20) P.splits = (int)wide;
   }
+  if (P.splits > (P.tc ? 1 : 16)) P.ws_bytes = (size_t)(P.units * P.splits * P.nr) * (L.c.D * sizeof(float) + sizeof(float2));
   return P;
 }
 
 cudaError_t launch_cache_attn(const CacheAttnLaunch& L, const CacheAttnPlan& P, int type, int format, cudaStream_t s) {
   if (P.units * P.splits > INT32_MAX) return cudaErrorInvalidValue;
-  if (type == kTypeF32) return attn_type<float>(L, P, format, s);
-  if (type == kTypeF16) return attn_type<__half>(L, P, format, s);
-  return attn_type<__nv_bfloat16>(L, P, format, s);
+  cudaError_t e = P.tc ? launch_cache_attn_tc(L, P, type, format, s)
+                  : type == kTypeF32 ? attn_type<float>(L, P, format, s)
+                  : type == kTypeF16 ? attn_type<__half>(L, P, format, s)
+                                     : attn_type<__nv_bfloat16>(L, P, format, s);
+  if (e != cudaSuccess || !P.ws_bytes) return e;
+  const dim3 grid((unsigned)P.units, (unsigned)std::min<int64_t>((int64_t)L.s.max_rows * L.G, P.nr));
+  const CacheAttnArgs& A = L;
+  if (type == kTypeF32) cache_attn_join<float><<<grid, 256, 0, s>>>(A, P.tiles, P.nr, P.tc);
+  else if (type == kTypeF16) cache_attn_join<__half><<<grid, 256, 0, s>>>(A, P.tiles, P.nr, P.tc);
+  else cache_attn_join<__nv_bfloat16><<<grid, 256, 0, s>>>(A, P.tiles, P.nr, P.tc);
+  return cudaGetLastError();
 }
 const char* cache_attn_name(const CacheAttnPlan& P, int type) {
-  (void)P;
+  if (P.tc) return type == kTypeF32 ? "cache_attention_tc_fp32" : "cache_attention_tc";
   return type == kTypeF32 ? "cache_attention_rows_fp32" : "cache_attention_rows";
 }
 

@@ -427,7 +427,7 @@ int check_cache_attn(supra_attn_ctx* c, const supra_attn_cache_attn_desc* d, Che
   L.H = d->H;
   L.scale_log2 = scale * kLog2e;
   L.causal = d->flags & SUPRA_ATTN_CA_CAUSAL ? 1 : 0;
-  call->vec = vec_rows(d->q, d->ldq, d->q_off, es) && vec_rows(d->out, d->ldo, d->o_off, es);
+  L.vec = vec_rows(d->q, d->ldq, d->q_off, es) && vec_rows(d->out, d->ldo, d->o_off, es);
   return SUPRA_ATTN_OK;
 }
 
@@ -460,9 +460,9 @@ int flush_cache(supra_attn_ctx* c, std::vector<const Queued*>& g) {
         const CacheAttnPlan plan = plan_cache_attn(L);
         name = cache_attn_name(plan, call.type);
         const int64_t tokens = ((int64_t)L.c.blocks * L.c.H) << L.c.log2t;
-        const int cols = cache_attn_box_cols(L.c.D), rows = cache_attn_box_rows(L.c.log2t);
-        if (!encode_byte_map(&L.mk, L.c.k, tokens, L.c.D, cols, rows) ||
-            !encode_byte_map(&L.mv, L.c.v, tokens, L.c.D, cols, rows))
+        const int cols = cache_attn_box_cols(L.c.D), rows = cache_attn_box_rows(L.c.log2t, plan.tc);
+        if (!encode_byte_map(&L.mk, L.c.k, tokens, L.c.D, cols, rows, !plan.tc) ||
+            !encode_byte_map(&L.mv, L.c.v, tokens, L.c.D, cols, rows, !plan.tc))
           return set_err(c, SUPRA_ATTN_ECUDA, "cuTensorMapEncodeTiled failed");
         L.splits = plan.splits;
         void* ws = nullptr;
@@ -470,7 +470,7 @@ int flush_cache(supra_attn_ctx* c, std::vector<const Queued*>& g) {
           int rc = scratch_alloc(c, plan.ws_bytes, &ws);
           if (rc) return rc;
           L.ws_o = static_cast<float*>(ws);
-          L.ws_ml = reinterpret_cast<float2*>(L.ws_o + plan.units * plan.splits * 8 * plan.nt * L.c.D);
+          L.ws_ml = reinterpret_cast<float2*>(L.ws_o + plan.units * plan.splits * plan.nr * L.c.D);
           c->launches += 1;  // the join
         }
         {

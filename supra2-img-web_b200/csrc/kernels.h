@@ -361,6 +361,7 @@ struct CacheAttnArgs {
   int32_t H, G;  // query heads, and query heads of one cache head
   float scale_log2;
   int32_t causal;
+  int32_t vec;  // rows of q and out start on 16-byte boundaries
   int32_t* status;
   // CTAs that share a unit (a sequence's rows of one cache head), and where they put their parts for
   // the join kernel (null: joined through distributed shared memory)
@@ -369,22 +370,27 @@ struct CacheAttnArgs {
   float2* ws_ml;
 };
 // Boxes of the K and V pools, seen as [blocks * H * block_tokens, D] bytes: cache_attn_box_cols(D)
-// columns (zeros past D) with the swizzle of that many bytes, and rows of a tile inside one block.
+// columns (zeros past D) and rows inside one block: for the rows kernel up to 32 with the swizzle of the
+// box's width, for the tensor-core kernel whole blocks without one.
 struct CacheAttnLaunch : CacheAttnArgs {
   CUtensorMap mk, mv;
 };
 inline int cache_attn_box_cols(int D) { return D <= 64 ? 64 : 128; }
-inline int cache_attn_box_rows(int log2t) { return log2t >= 5 ? 32 : 16; }
+inline int cache_attn_box_rows(int log2t, bool tc) { return tc ? 1 << log2t : log2t >= 5 ? 32 : 16; }
 // How a call is split, from its sizes alone.
 struct CacheAttnPlan {
-  int nt, tiles;     // groups of 8 rows in a row tile, row tiles of a sequence and cache head
+  bool tc;           // the tensor-core kernel (cache_attn_tc.cu)
+  int nr, tiles;     // rows of a row tile, row tiles of a sequence and cache head
   int64_t units;
   int splits;
-  size_t ws_bytes;   // workspace: parts of O (units * splits * 8 nt * D floats), then (m, l) of each row
+  size_t ws_bytes;   // workspace: parts of O (units * splits * nr * D floats), then (m, l) of each row
 };
 CacheAttnPlan plan_cache_attn(const CacheAttnArgs& L);
 cudaError_t launch_cache_attn(const CacheAttnLaunch& L, const CacheAttnPlan& P, int type, int format, cudaStream_t s);
 const char* cache_attn_name(const CacheAttnPlan& P, int type);
+// cache_attn_tc.cu, and the rows of its row tiles
+cudaError_t launch_cache_attn_tc(const CacheAttnLaunch& L, const CacheAttnPlan& P, int type, int format, cudaStream_t s);
+int cache_attn_tc_rows(int D);
 
 // Copies bytes (a multiple of 16, both addresses 16-byte aligned) from src, which may be pinned
 // host memory addressable by the device, to device memory dst (stage.cu).

@@ -272,9 +272,10 @@ namespace rt {
 
 // ---- runtime.cpp ----
 bool encode_map(CUtensorMap* m, const MapKey& k);
-// [rows, cols] bytes without padding, boxes of box_cols (64 or 128, swizzled over as many bytes) x
-// box_rows, zeros past the ends.
-bool encode_byte_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int box_cols, int box_rows);
+// [rows, cols] bytes without padding, boxes of box_cols (64 or 128) x box_rows, zeros past the ends;
+// swizzle: over as many bytes as the box is wide.
+bool encode_byte_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int box_cols, int box_rows,
+                     bool swizzle);
 // The slot in `maps` (the tensor maps of the launch being packed, map epoch c->map_epoch) of the
 // map for k: encoded once per context and cached, appended to maps at its first use in the epoch.
 int map_slot(supra_attn_ctx* c, const MapKey& k, std::vector<CUtensorMap>& maps, int32_t* out);

@@ -205,7 +205,9 @@ def test_write_of_values_that_are_not_finite(gpu):
 #   p: e^ds and ex2's own 2^-22; then 2^12 p is rounded to fp16 (2^-12 of it; two parts: 2^-22), and where
 #     it (or its second part) is below 2^-14, where fp16 numbers are 2^-24 apart, by up to 2^-25: 2^-37 of
 #     the largest p, which is 1 and at most the sum of all, for each token: 2^-37 sum |v| of the quotient,
-#     however small p is (it shows where the tokens with large p have v = 0);
+#     however small p is (it shows where the tokens with large p have v = 0). Where many rows share a tile
+#     it is 2^15 p times its block's V scale over the tile's largest, no less than 2^-3 for fp32 (2^-37
+#     again) and 2^-8 for the others: 2^-32;
 #   sums over tokens: a rounding for each 16 tokens, (tokens / 16 + 40) u of sum p|v|;
 #   the quotient: the error of sum p relative to itself is the same, so both count: twice;
 #   the result's own rounding: eps / 2 of its type (fp16 numbers below 2^-14 are 2^-24 apart: 2^-25).
@@ -216,7 +218,7 @@ def attention_bound(dtype, D, tokens, out, pv, av, st, sm):
         ds = ds + 2.0 ** -22 * st
     p = (2.0 ** -22 if dtype == "fp32" else 2.0 ** -12) + 2.0 ** -21
     rel = 2 * (np.expm1(ds) + p + (tokens / 16 + 40) * u)
-    err = rel[..., None] * pv + 2.0 ** -37 * av
+    err = rel[..., None] * pv + 2.0 ** (-37 if dtype == "fp32" else -32) * av
     return err + torch.finfo(TYPES[dtype]).eps / 2 * (np.abs(out) + err) + (2.0 ** -25 if dtype == "fp16" else 1e-37)
 
 
@@ -283,6 +285,55 @@ def test_attention(gpu, case, dtype, fmt):
 def test_attention_split_along_the_cache(gpu, T, lengths, rows, dtype):
     check_attention(gpu, "int8", dtype, T, 1, 2, 64, lengths, rows, True, seed=3)
     check_attention(gpu, "e4m3", dtype, T, 1, 2, 128, lengths, rows, False, seed=4)
+
+
+TILE_CASES = [
+    # many query rows: T, Hk, G, D, lengths, rows, causal
+    (64, 1, 1, 64, [128], [256], False),
+    (64, 2, 1, 64, [1, 33, 129, 0], [130, 128, 127, 40], False),
+    (128, 1, 4, 128, [700, 40], [100, 33], True),
+    (32, 2, 3, 96, [300, 290], [90, 290], True),
+    (16, 1, 2, 32, [77, 500], [77, 300], True),
+    (16, 1, 5, 128, [130], [60], False),
+    (64, 1, 8, 80, [64, 1000], [64, 37], True),
+]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("case", TILE_CASES, ids=lambda c: "-".join(str(x) for x in c[:4]))
+def test_attention_of_many_rows(gpu, case, dtype, fmt):
+    T, Hk, G, D, lengths, rows, causal = case
+    check_attention(gpu, fmt, dtype, T, Hk, G, D, lengths, rows, causal, seed=23)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_of_many_rows_over_a_long_cache(gpu, D, dtype):
+    """So few row tiles that the tokens are split among CTAs."""
+    check_attention(gpu, "int8", dtype, 64, 1, 2, D, [4099, 700, 0], [40, 20, 3], True, seed=24)
+
+
+@pytest.mark.parametrize("rows", [3, 70])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_attention_of_blocks_of_unlike_size(gpu, dtype, rows):
+    """V scales far apart inside one tile: a row that sees only the small ones keeps their precision. Blocks
+    of zeros and negative scales are taken as they are."""
+    def spread(p):
+        for i, page in enumerate(p.table[0]):
+            p.vs[page] *= 2.0 ** (-10 * (6 - i)) if i < 7 else 0.0 if i == 7 else -1.0
+
+    for T, D in ((16, 64), (16, 128), (32, 64), (64, 128)):
+        got = check_attention(gpu, "int8", dtype, T, 1, 1, D, [11 * T], [11 * T if rows > 3 else 3], True, seed=25, mutate=spread)
+        if rows > 3:
+            assert np.abs(got[:T]).max() < 2.0 ** -50  # the first block's own size
+
+    def negative(p):
+        p.ks[p.table[0][1]] *= -1
+        p.vs[p.table[0][2]] *= -1
+
+    for T in (32, 128):
+        check_attention(gpu, "e4m3", dtype, T, 1, 2, 64, [3 * T + 5], [rows], True, seed=26, mutate=negative)
 
 
 @pytest.mark.parametrize("dtype", sorted(TYPES))
