@@ -25,6 +25,7 @@
 // Every wait is bounded; on a timeout the CTA records the failure, waits for its own copies and MMAs, frees its
 // TMEM and leaves.
 #include <algorithm>
+#include <type_traits>
 
 #include "cache.cuh"
 #include "tcgen05.cuh"
@@ -136,6 +137,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Four codes as two fp16 pairs in their order.
 template <int FMT>
 __device__ __forceinline__ void codes_in_order(uint32_t u, uint32_t& lo, uint32_t& hi) {
@@ -218,6 +225,9 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
   if (warp == 0) {
     tc::tmem_alloc(&B->tmem, Y::COLS);
     tc::tmem_relinquish();
+  } else if (warp == 1 && lane == 0) {
+    tc::prefetch_map(&mk);
+    tc::prefetch_map(&mv);
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -239,15 +249,27 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       const int32_t page = in ? L.s.table[(int64_t)b * L.s.ld_table + (tok >> log2t)] : -1;
       const bool live = in && page >= 0 && page < c.blocks;
       if (in && !live) report_error(L.status, DEV_BAD_BLOCK, 2, page);
+      const bool first = (tok & ((1 << log2t) - 1)) == 0;  // one box per block of the tile
+      const uint32_t boxes = __ballot_sync(0xffffffffu, live && first);
+      const uint32_t dead = __ballot_sync(0xffffffffu, in && !live);
+      const int box_rows = min(kN, 1 << log2t);
+      if (lane == 0) {
+        mt.dead = (int32_t)dead;
+        mbar_arrive_expect_tx(&B->raw[st], (uint32_t)(__popc(boxes) * 2 * box_rows * DT));
+      }
+      __syncwarp();
+      if (boxes >> lane & 1) {
+        const int y = ((page * c.H + hk) << log2t) + (tok & ((1 << log2t) - 1));
+        uint8_t* to = base + Y::RAWS + st * 2 * Y::RAWB + 16 * lane * DT;
+        tc::tma_load_2d(to, &mk, 0, y, &B->raw[st]);
+        tc::tma_load_2d(to + Y::RAWB, &mv, 0, y, &B->raw[st]);
+      }
       float ks = 0.f, vs = 0.f;
       if (live) {
         const int64_t u = (int64_t)page * c.H + hk;
         ks = c.ks[u];
         vs = c.vs[u];
       }
-      const uint32_t dead = __ballot_sync(0xffffffffu, in && !live);
-      const bool first = (tok & ((1 << log2t) - 1)) == 0;  // one box per block of the tile
-      const uint32_t boxes = __ballot_sync(0xffffffffu, live && first);
       const float av = fabsf(vs);
       float top = live && av <= 3.4028234e38f ? av : 0.f;
       float low = live && av <= 3.4028234e38f ? av : 3.4028234e38f;
@@ -266,20 +288,9 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         mt.lr[lane] = ratio == 1.f ? 0.f : log2f(ratio);
         mt.ir[lane] = 1.f / ratio;
       }
-      const int box_rows = min(kN, 1 << log2t);
-      __syncwarp();
       if (lane == 0) {
         mt.top = top;
-        mt.dead = (int32_t)dead;
         mt.subs = apart ? kN >> log2t : 1;
-        mbar_arrive_expect_tx(&B->raw[st], (uint32_t)(__popc(boxes) * 2 * box_rows * DT));
-      }
-      __syncwarp();
-      if (boxes >> lane & 1) {
-        const int y = ((page * c.H + hk) << log2t) + (tok & ((1 << log2t) - 1));
-        uint8_t* to = base + Y::RAWS + st * 2 * Y::RAWB + 16 * lane * DT;
-        tc::tma_load_2d(to, &mk, 0, y, &B->raw[st]);
-        tc::tma_load_2d(to + Y::RAWB, &mv, 0, y, &B->raw[st]);
       }
     };
     int loaded = j0;
@@ -449,72 +460,83 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         const float v0 = mt.vs[lo >> 4];
         const float f = hi <= lo ? 0.f : subs > 1 ? v0 : v0 < 0.f ? -mt.top : mt.top;
 
-        // the row's maximum
+        // the row's maximum: the largest score of each 16 tokens (32, when blocks hold as many) times their
+        // factor
         float mx = -INFINITY;
+        auto largest = [](const float* s) {
+          float u = max3(s[0], s[1], s[2]), w = max3(s[3], s[4], s[5]);
+#pragma unroll
+          for (int e = 6; e < 14; e += 4) u = max3(u, s[e], s[e + 1]), w = max3(w, s[e + 2], s[e + 3]);
+          u = max3(u, s[14], s[15]);
+          return fmaxf(u, w);
+        };
         for (int ch = 0; ch < nch; ++ch) {
           float s[32];
           tc::tmem_ld32(tl + 32 * ch, s);
+          const float k0 = mt.ks[2 * ch] * rs, k1 = mt.ks[2 * ch + 1] * rs;
           tc::tmem_wait_ld();
           if (partial) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               const int col = 32 * ch + e;
-              if (col < lo || col >= hi || (deadm >> (2 * ch + (e >> 4)) & 1)) s[e] = -INFINITY;
+              if (col < lo || col >= hi || (deadm >> (2 * ch + (e >> 4)) & 1)) s[e] = k0 < 0.f ? INFINITY : -INFINITY;
             }
           }
+          if (k0 < 0.f || k1 < 0.f) {  // (a negative K scale, which no write makes: score by score)
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float k = mt.ks[2 * ch + g] * rs;
-            float a = s[16 * g];
-            if (!(k < 0.f)) {
-#pragma unroll
-              for (int e = 1; e < 16; ++e) a = fmaxf(a, s[16 * g + e]);
-            } else {  // (a negative K scale, which no write makes)
-              a = INFINITY;
-#pragma unroll
-              for (int e = 0; e < 16; ++e) a = fminf(a, s[16 * g + e] == -INFINITY ? INFINITY : s[16 * g + e]);
+            for (int e = 0; e < 32; ++e) {
+              const float y = fabsf(s[e]) < INFINITY ? s[e] * (e < 16 ? k0 : k1) : -INFINITY;
+              mx = fmaxf(mx, y);
             }
-            if (fabsf(a) < INFINITY) mx = fmaxf(mx, a * k);
-            else if (a == INFINITY && !(k < 0.f)) mx = INFINITY;
+          } else {
+            const float a0 = largest(s), a1 = largest(s + 16);
+            mx = max3(mx, a0 * k0, a1 * k1);  // (-inf times a factor of 0 is NaN, which the maximum leaves out)
           }
         }
         const float mn = fmaxf(m, mx);
         const float ref = mn == -INFINITY ? 0.f : mn;
         const float al = ex2f(m - ref);
+        const bool moved = mn != m;
         m = mn;
         // p, its sum, and P into the columns of the scores it comes from
         float sum = 0.f;
         for (int ch = 0; ch < nch; ++ch) {
           float s[32];
           tc::tmem_ld32(tl + 32 * ch, s);
+          const float k0 = mt.ks[2 * ch] * rs, k1 = mt.ks[2 * ch + 1] * rs;
+          const float h0 = kPShift - ref + mt.lr[2 * ch], h1 = kPShift - ref + mt.lr[2 * ch + 1];
+          const float i0 = mt.ir[2 * ch], i1 = mt.ir[2 * ch + 1];
           tc::tmem_wait_ld();
           uint32_t ph[16], pl[SPLIT ? 16 : 1];
+          float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          auto form = [&](auto masked) {
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const int grp = 2 * ch + g;
-            const float k = mt.ks[grp] * rs, shift = kPShift - ref + mt.lr[grp];
-            float part = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              float2 x = __ffma2_rn(make_float2(s[16 * g + e], s[16 * g + e + 1]), make_float2(k, k), make_float2(shift, shift));
-              if (partial) {
-                const int col = 16 * grp + e;
-                const bool dd = deadm >> grp & 1;
+            for (int e = 0; e < 32; e += 2) {
+              const float k = e < 16 ? k0 : k1, h = e < 16 ? h0 : h1;
+              float2 x = __ffma2_rn(make_float2(s[e], s[e + 1]), make_float2(k, k), make_float2(h, h));
+              if constexpr (decltype(masked)::value) {
+                const int col = 32 * ch + e;
+                const bool dd = deadm >> (2 * ch + (e >> 4)) & 1;
                 if (col < lo || col >= hi || dd) x.x = -INFINITY;
                 if (col + 1 < lo || col + 1 >= hi || dd) x.y = -INFINITY;
               }
               x.x = ex2f(x.x);
               x.y = ex2f(x.y);
-              part += x.x + x.y;
-              const int w = 8 * g + (e >> 1);
+              part[e >> 4] = __fadd2_rn(part[e >> 4], x);
+              const int w = e >> 1;
               ph[w] = pack2<__half>(x.x, x.y);
               if constexpr (SPLIT) {
                 const float2 f = unpack2<__half>(ph[w]);
-                pl[w] = pack2<__half>(x.x - f.x, x.y - f.y);
+                const float2 d = __ffma2_rn(f, make_float2(-1.f, -1.f), x);
+                pl[w] = pack2<__half>(d.x, d.y);
               }
             }
-            sum += part == 0.f ? 0.f : part * mt.ir[grp];  // (the ratio of a block that no visible token is in may be NaN)
-          }
+          };
+          if (partial) form(std::true_type{});
+          else form(std::false_type{});
+          const float p0 = part[0].x + part[0].y, p1 = part[1].x + part[1].y;
+          // (the ratio of a block that no visible token is in may be NaN)
+          sum += (p0 == 0.f ? 0.f : p0 * i0) + (p1 == 0.f ? 0.f : p1 * i1);
           tmem_st16(tl + 32 * ch, ph);
           if constexpr (SPLIT) tmem_st16(tl + 32 * ch + 16, pl);
         }
@@ -531,6 +553,13 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
           if (!lastsub) issue_s(j, false);
           else if (j + 1 < j1) issue_s(j + 1, true);
         }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int e = 0; e < DT; e += 2) {
+            const float2 w = __fmul2_rn(make_float2(o[e], o[e + 1]), make_float2(al, al));
+            o[e] = w.x, o[e + 1] = w.y;
+          }
+        }
 #pragma unroll
         for (int e = 0; e < DT; e += 32) {
           float a[32];
@@ -538,8 +567,7 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
           tc::tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const float2 w = __fmul2_rn(make_float2(o[e + i], o[e + i + 1]), make_float2(al, al));
-            const float2 y = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(f, f), w);
+            const float2 y = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(f, f), make_float2(o[e + i], o[e + i + 1]));
             o[e + i] = y.x, o[e + i + 1] = y.y;
           }
         }
@@ -575,19 +603,21 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       }
       __syncwarp();
       const int per = c.D / V8;  // pieces that exist
-      T* out = static_cast<T*>(L.o);
-      for (int v = lane; v < 32 * PER; v += 32) {
-        const int rr = (tr & ~31) + v / PER, p = v % PER;
-        const int row = rt * kM + rr;
-        if (row >= nrow || p >= per) continue;
-        const int pk = r0 + row;
-        T* to = out + (q.row0 + pk / L.G) * L.ldo + (int64_t)(hk * L.G + pk % L.G) * c.D + p * V8;
-        const T* from = reinterpret_cast<const T*>(Qs + rr * (PER * 16) + ((p ^ (rr & 7)) << 4));
+      // each row's address is known to its own thread
+      T* mine_out = live ? static_cast<T*>(L.o) + (q.row0 + qi) * L.ldo + head : nullptr;
+      constexpr int RPI = 32 / PER;  // rows of an iteration
+#pragma unroll 4
+      for (int i = 0; i < 32; i += (RPI > 0 ? RPI : 1)) {
+        const int rl = i + (RPI > 0 ? lane / PER : 0), p = lane % PER;
+        T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine_out), rl));
+        const T* from = reinterpret_cast<const T*>(Qs + ((tr & ~31) + rl) * (PER * 16) + ((p ^ (rl & 7)) << 4));
+        if (!to || p >= per) continue;
+        to += p * V8;
         if (L.vec) {
           *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
         } else {
 #pragma unroll
-          for (int i = 0; i < V8; ++i) to[i] = from[i];
+          for (int e = 0; e < V8; ++e) to[e] = from[e];
         }
       }
     }
