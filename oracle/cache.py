@@ -89,13 +89,14 @@ def read(fmt, codes, scale, lengths, row_start, table):
 
 
 def attention(fmt, kc, ks, vc, vs, q, lengths, row_start, table, scale, causal):
-    """q [R, H, D] float64 -> (out [R, H, D], sums of p|v| [R, H, D], sums of |v| [R, H, D],
-    largest score term sum [R, H], largest |score| [R, H]), all float64; the last four bound rounding
-    errors."""
+    """q [R, H, D] float64 -> (out [R, H, D], sums of p|v| [R, H, D], what the smallest steps of p
+    are worth [2, R, H, D], largest score term sum [R, H], largest |score| [R, H]), all float64; the last
+    four bound rounding errors. Steps of p itself: sum |v|; steps of p times its V scale, relative to
+    the row's largest: max(p v_scale) * sum |code|."""
     T, Hk = kc.shape[2], kc.shape[1]
     R, H, D = q.shape
     G = H // Hk
-    out, pv, av = (np.zeros((R, H, D)) for _ in range(3))
+    out, pv, av = np.zeros((R, H, D)), np.zeros((R, H, D)), np.zeros((2, R, H, D))
     st, sm = np.zeros((R, H)), np.zeros((R, H))
     for b in range(len(lengths)):
         L, n = lengths[b], row_start[b + 1] - row_start[b]
@@ -104,6 +105,8 @@ def attention(fmt, kc, ks, vc, vs, q, lengths, row_start, table, scale, causal):
         pages = [table[b][j] for j in range((L + T - 1) // T)]
         k = (decode(fmt, kc[pages]) * ks[pages].astype(np.float64)[:, :, None, None]).transpose(1, 0, 2, 3).reshape(Hk, -1, D)[:, :L]
         v = (decode(fmt, vc[pages]) * vs[pages].astype(np.float64)[:, :, None, None]).transpose(1, 0, 2, 3).reshape(Hk, -1, D)[:, :L]
+        vc_of = decode(fmt, vc[pages]).transpose(1, 0, 2, 3).reshape(Hk, -1, D)[:, :L]
+        vs_of = np.abs(np.repeat(vs[pages].astype(np.float64), T, axis=0).T[:, :L])
         for i in range(n):
             seen = min(L, L - n + i + 1) if causal else L
             if seen <= 0:
@@ -117,7 +120,8 @@ def attention(fmt, kc, ks, vc, vs, q, lengths, row_start, table, scale, causal):
                     p /= p.sum()
                 out[r, h] = p @ vv
                 pv[r, h] = p @ np.abs(vv)
-                av[r, h] = np.abs(vv).sum(0)
+                av[0, r, h] = np.abs(vv).sum(0)
+                av[1, r, h] = (p * vs_of[h // G, :seen]).max() * np.abs(vc_of[h // G, :seen]).sum(0)
                 st[r, h] = abs(scale) * (np.abs(kk) @ np.abs(q[r, h])).max()
                 sm[r, h] = np.abs(s).max()
     return out, pv, av, st, sm

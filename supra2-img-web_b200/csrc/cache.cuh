@@ -144,6 +144,24 @@ __device__ __forceinline__ uint32_t encode4(const float (&x)[4]) {
   }
 }
 
+// ---- waits -----------------------------------------------------------------------------------
+// Waits for the phase with the given parity, for about two seconds at most; gives up at once when
+// *abort is set (abort may be null). The limit is counted in SM clocks and looked at only every 64
+// tries: a read of the global timer takes about 1500 cycles, more than most of these waits.
+constexpr long long kWaitLimitClocks = 4000000000ll;
+__device__ __forceinline__ bool mbar_wait_clocked(uint64_t* bar, uint32_t parity, volatile int32_t* abort) {
+  long long t0 = 0;
+  for (uint32_t it = 0;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 63u) == 63u) {
+      if (abort && *abort) return false;
+      const long long t = clock64();
+      if (t0 == 0) t0 = t;
+      else if (t - t0 > kWaitLimitClocks) return false;
+    }
+  }
+}
+
 // ---- sequences ---------------------------------------------------------------------------------
 struct SeqView {
   int64_t row0;  // first row of the operands

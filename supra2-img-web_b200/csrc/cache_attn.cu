@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
   int lost_at = 0;
   for (int i = 0; i < cnt; ++i) {
     const int stg = i % kStages;
-    if (!mbar_wait_bounded(full + stg, (uint32_t)(i / kStages) & 1u)) {
+    if (!mbar_wait_clocked(full + stg, (uint32_t)(i / kStages) & 1u, nullptr)) {
       if (lane == 0) report_error(L.status, DEV_TIMEOUT, 70, i);
       lost = true, lost_at = i;
       break;
@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
   // (every copy has landed: each was waited for, but after a wait that ran out, when those in flight are
   // given their time before the ring is used again)
   if (lost) {
-    for (int i = lost_at; i < min(cnt, lost_at + kStages); ++i) mbar_wait_bounded(full + i % kStages, (uint32_t)(i / kStages) & 1u);
+    for (int i = lost_at; i < min(cnt, lost_at + kStages); ++i) mbar_wait_clocked(full + i % kStages, (uint32_t)(i / kStages) & 1u, nullptr);
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -529,8 +529,10 @@ __global__ void __launch_bounds__(256) cache_attn_join(const __grid_constant__ C
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int unit = blockIdx.x;
   const int64_t part0 = (int64_t)unit * L.splits;
-  const int rt = last_first ? tiles - 1 - unit % tiles : unit % tiles;
-  unit /= tiles;
+  // (the tensor-core kernel orders its units by row tile, the last ones first)
+  const int heads = L.s.B * c.H;
+  const int rt = last_first ? tiles - 1 - unit / heads : unit % tiles;
+  unit = last_first ? unit % heads : unit / tiles;
   const int hk = unit % c.H, b = unit / c.H;
   SeqView q;
   if (!seq_view(L.s, b, false, L.status, q)) return;

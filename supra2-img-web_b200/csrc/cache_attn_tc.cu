@@ -2,26 +2,29 @@
 // attention of an image's patches to a prompt, chunks of new tokens against their history).
 //
 // The mathematics of cache_attn.cu for tiles of 128 packed query rows (query, head of the group) against
-// tiles of up to 128 tokens:
+// tiles of 64 tokens:
 //   S = Q C_k^T      tcgen05.mma kind::f16, Q (smem, fp16) x K codes (smem, fp16), fp32 in TMEM
-//   P = 2^(S c - m)  softmax threads, one row each: c = scale * k_scale of the token's block
-//   O += f (P C_v)   tcgen05.mma kind::f16, P from TMEM x V codes (smem, MN-major); the tile's product
-//                    goes into a fresh accumulator and is added to O in fp32 registers
+//   P = 2^(S c + log2 v - m)   softmax threads, one row each: c = scale * k_scale and v = v_scale of the
+//                    token's block, m the row's largest exponent so far
+//   O += P C_v       tcgen05.mma kind::f16, P from TMEM x V codes (smem, MN-major)
+//   o = O / sum(P / v)
 // Codes are exact in fp16, so 8-bit K and V cost the tensor cores nothing but their conversion: four
 // converter warps turn the raw bytes, which the TMA unit brings in block by block, into the swizzled
-// operand tiles, once for all rows of the CTA. The V scales of a tile's blocks differ: p carries each
-// block's scale over the tile's largest, as an exponent (added to m, so it costs nothing per element;
-// the row's sum divides it out again per 32 tokens), and the largest multiplies the tile's product. A
-// tile whose scales lie far apart (2^8, for fp32 rows 2^3) is taken block by block instead, so that a row
-// that sees only its small ones keeps their precision.
-// q carries a power of two per row (cache_attn.cu); fp32 rows and their p use two fp16 parts, and each
-// product two MMAs.
+// operand tiles, once for all rows of the CTA. P carries the V scale as an exponent, which costs nothing
+// per score, and m follows the product of both, so each row's P is as large as fp16 allows whatever the
+// scales of the blocks that it sees; only the sum divides the scale out again, once per 16 tokens.
+// q carries a power of two per row (cache_attn.cu).
+// 16-bit rows keep O in TMEM, where m moves only when a tile exceeds it by 2^8 (then the softmax threads
+// rescale O there). fp32 rows use two fp16 parts of q and p (each product two MMAs), move m exactly, and
+// add each tile's product to O in fp32 registers, rounded to nearest, so that the error does not grow
+// with the number of tiles.
 //
-// Head dims up to 64: one row tile per CTA, two CTAs per SM (128 + 64 TMEM columns each, 256 allocated).
-// Up to 128: two row tiles per CTA that share the converted tiles, one CTA per SM (2 x 256 columns),
-// registers moved from the converters to the softmax threads. Either way one row tile's softmax runs
-// while the tensor cores work for the other. The softmax, 16 exponentials per cycle and SM, bounds the
-// kernel: 128 x 128 scores take 1024 cycles of it and 2 x 256 (head dim 64) or 2 x 512 (128) of MMA.
+// Head dims up to 64: one row tile per CTA, two CTAs per SM (192 TMEM columns each, 256 allocated). Up to
+// 128: two row tiles per CTA that share the converted tiles, one CTA per SM (2 x 256 columns). fp32 rows
+// move registers from the converters to the softmax threads. K, V and their raw bytes have two stages
+// each, and so has S: a row tile's next scores are formed while its softmax threads work on the present
+// ones, and its last product behind them, so that neither MMA nor conversion is waited for. What bounds
+// the kernel is the softmax: 16 exponentials per cycle and SM, and about five instructions a score.
 // Every wait is bounded; on a timeout the CTA records the failure, waits for its own copies and MMAs, frees its
 // TMEM and leaves.
 #include <algorithm>
@@ -34,12 +37,12 @@ namespace supra {
 namespace {
 
 constexpr int kM = 128;  // rows of a row tile
-constexpr int kN = 128;  // tokens of a tile
-// p is formed as 2^15 p (fp16 ends at 65504). With its block's ratio r the smallest step of its fp16 form is
-// 2^-40 / r of the row's largest p: blocks further apart than this are taken one by one.
-constexpr float kPShift = 15.f;
+constexpr int kN = 64;   // tokens of a tile
+// P is formed as 2^kPShift P (fp16 ends at 65504). 16-bit rows: m may lag the row's largest exponent by kLag.
 template <bool SPLIT>
-constexpr float kApart = SPLIT ? 0.125f : 0.00390625f;  // 2^-3, 2^-8
+constexpr float kPShift = SPLIT ? 15.f : 7.f;
+constexpr float kLag = 8.f;
+constexpr float kScaleFloor = 7.7037197775489434e-34f;  // 2^-110, below any scale that a write makes
 constexpr int kMeta = 4;  // tiles whose scales are kept at once
 
 template <int DT, bool SPLIT>
@@ -48,43 +51,46 @@ struct Cfg {
   static constexpr int SOFT = 128 * RT;        // softmax threads
   static constexpr int THREADS = SOFT + 128;
   static constexpr int PER_SM = DT == 64 ? 2 : 1;
-  static constexpr int RAW = DT == 128 && SPLIT ? 1 : 2;  // raw stages
   static constexpr int PARTS = SPLIT ? 2 : 1;
+  static constexpr int CHUNK = SPLIT && DT == 128 ? 32 : 64;  // scores that a thread holds at once
+  static constexpr int REGS_SOFT = DT == 64 ? 168 : 208, REGS_CONV = 88;  // (SPLIT) 128 or 168 at launch
   static constexpr int SLABS = DT / 64;                       // 64-channel slabs of an operand tile
-  static constexpr uint32_t SLAB = kM * 128;                  // 128 rows of 128 bytes
-  static constexpr uint32_t QPART = SLABS * SLAB;             // one part of one row tile
+  static constexpr uint32_t QSLAB = kM * 128;                 // 128 rows of 128 bytes
+  static constexpr uint32_t QPART = SLABS * QSLAB;            // one part of one row tile
+  static constexpr uint32_t SLAB = kN * 128;                  // of K or V
+  static constexpr uint32_t TILE = SLABS * SLAB;              // K or V, one stage
   static constexpr uint32_t Q = 0;                            // [RT][PARTS]
-  static constexpr uint32_t K = Q + RT * PARTS * QPART;
-  static constexpr uint32_t V = K + SLABS * SLAB;
-  static constexpr uint32_t RAWS = V + SLABS * SLAB;          // [RAW][K, V][kN][DT] bytes
+  static constexpr uint32_t K = Q + RT * PARTS * QPART;       // [2]
+  static constexpr uint32_t V = K + 2 * TILE;                 // [2]
+  static constexpr uint32_t RAWS = V + 2 * TILE;              // [2][K, V][kN][DT] bytes
   static constexpr uint32_t RAWB = kN * DT;
-  static constexpr uint32_t META = RAWS + RAW * 2 * RAWB;     // [kMeta] TileMeta
-  static constexpr uint32_t BAR = META + kMeta * 192;
-  static constexpr uint32_t SMEM = BAR + 128 + 1024;          // + alignment of the base
-  static constexpr uint32_t COL_ACC = kN;                     // S and P, then the tile's product
+  static constexpr uint32_t RS = RAWS + 4 * RAWB;             // score factor of each row
+  static constexpr uint32_t META = RS + RT * kM * 4;          // [kMeta] TileMeta
+  static constexpr uint32_t BAR = META + kMeta * 64;
+  static constexpr uint32_t SMEM = BAR + 192 + 1024;          // + alignment of the base
+  static constexpr uint32_t COL_ACC = 2 * kN;                 // two buffers of S and P, then the tile's product
   static constexpr uint32_t COLS = DT == 64 ? 256 : 512;
   static constexpr uint32_t COL_RT = 256;
   static_assert(SMEM <= (PER_SM == 2 ? 113u : 227u) * 1024, "shared memory");
 };
 
-struct TileMeta {  // of a tile's eight 16-token groups
-  float ks[8];
-  float vs[8];
-  float lr[8];   // log2 of |vs| over top, and its inverse ratio: what p carries, and its sum does not
-  float ir[8];
-  float top;     // the largest finite |vs|
+struct TileMeta {  // of a tile's four 16-token groups
+  float ks[4];
+  float lv[4];   // log2 |v_scale|
+  float iv[4];   // 1 / |v_scale|
   int32_t dead;  // groups whose block does not exist (bits), tokens past the end not among them
-  int32_t subs;  // 1, or the number of blocks the tile is taken in
-  int32_t pad[13];
+  int32_t neg;   // groups with a negative V scale (bits), which no write makes
+  int32_t odd;   // the tile has dead or negative groups: taken score by score
+  int32_t pad;
 };
-static_assert(sizeof(TileMeta) == 192, "META");
+static_assert(sizeof(TileMeta) == 64, "META");
 
 struct Bars {
-  uint64_t raw[2], k_full, v_full, k_empty, v_empty, s_full[2], pv_full[2], drain[2];
+  uint64_t raw[2], k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2][2], pv_full[2], drain[2];
   uint32_t tmem;
   int32_t abort;
 };
-static_assert(sizeof(Bars) <= 128, "BAR");
+static_assert(sizeof(Bars) <= 192, "BAR");
 
 // status[2] of a wait that ran out
 enum TcWait : int32_t { W_RAW = 80, W_K_FULL = 81, W_V_FULL = 82, W_K_EMPTY = 83, W_V_EMPTY = 84, W_S = 85, W_PV = 86 };
@@ -97,22 +103,35 @@ __device__ __forceinline__ float ex2f(float x) {
 
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int32_t* abort, int32_t* status, int32_t id,
                                          int32_t detail) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = global_ns();
-  for (uint32_t it = 1;; ++it) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 63u) == 0u) {
-      if (*abort) return false;
-      if (global_ns() - t0 > kWaitLimitNs) {
-        report_error(status, DEV_TIMEOUT, id, detail);
-        *abort = 1;
-        return false;
-      }
-    }
+  if (mbar_wait_clocked(bar, parity, abort)) return true;
+  if (!*abort) {
+    report_error(status, DEV_TIMEOUT, id, detail);
+    *abort = 1;
   }
+  return false;
 }
 
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+
+// The barrier of a role's threads, and whether all of them are well: whoever gave up a wait still arrives, and
+// all leave together.
+__device__ __forceinline__ bool bar_and(int id, int n, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)ok), "r"(id), "r"(n)
+      : "memory");
+  return r != 0;
+}
+
+// One lane of a converged warp, the same in every call; the branch it guards is uniform to the compiler, so
+// the MMA operands stay in uniform registers (a branch on a thread's number cost ~190 cycles per MMA).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
 
 // kind::f16, fp16 operands, fp32 accumulator
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -184,15 +203,14 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
   Bars* B = reinterpret_cast<Bars*>(base + Y::BAR);
   volatile int32_t* abort = &B->abort;
   const CachePool& c = L.c;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;  // (uniform)
 
   // unit = (row tile, sequence, cache head), the longest causal row tiles first; the CTAs that split a
   // unit's tokens are neighbours
-  int unit = blockIdx.x / L.splits;
-  const int split = blockIdx.x % L.splits;
-  const int rt0 = tiles - 1 - unit % tiles;
-  unit /= tiles;
-  const int hk = unit % c.H, b = unit / c.H;
+  const int unit = blockIdx.x / L.splits, split = blockIdx.x % L.splits;
+  const int heads = L.s.B * c.H;
+  const int rt0 = tiles - 1 - unit / heads;
+  const int hk = unit % heads % c.H, b = unit % heads / c.H;
   SeqView q;
   if (!seq_view(L.s, b, false, L.status, q)) return;
   const int rows = q.n * L.G;  // packed (query, head of the group)
@@ -208,14 +226,14 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
   const int j0 = (int)((int64_t)nt * split / L.splits), j1 = (int)((int64_t)nt * (split + 1) / L.splits);
 
   if (threadIdx.x == 0) {
-    mbar_init(&B->raw[0], 1);
-    mbar_init(&B->raw[1], 1);
-    mbar_init(&B->k_full, 128);
-    mbar_init(&B->v_full, 128);
-    mbar_init(&B->k_empty, RT);
-    mbar_init(&B->v_empty, RT);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&B->s_full[i], 1);
+      mbar_init(&B->raw[i], 1);
+      mbar_init(&B->k_full[i], 128);
+      mbar_init(&B->v_full[i], 128);
+      mbar_init(&B->k_empty[i], RT);
+      mbar_init(&B->v_empty[i], RT);
+      mbar_init(&B->s_full[i][0], 1);
+      mbar_init(&B->s_full[i][1], 1);
       mbar_init(&B->pv_full[i], 1);
       mbar_init(&B->drain[i], 1);
     }
@@ -236,379 +254,470 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
 
   if (warp >= 4 * RT) {
     // ---------------- converters ----------------
-    if constexpr (RT == 2) reg_dec<88>();
+    if constexpr (SPLIT) reg_dec<Y::REGS_CONV>();
     const int ct = threadIdx.x - Y::SOFT;
     const int log2t = c.log2t;
-    // Tile j's blocks into raw stage j % RAW and its scales into meta[j % kMeta] (the first warp).
+    // The first warp knows the blocks of 8 tiles at a time, a 16-token group per lane, and loads the next
+    // 8 tiles' while it uses them up.
+    const int g0 = j0 * (kN / 16);
+    auto page_at = [&](int grp) {
+      return grp * 16 < seen && grp < j1 * (kN / 16) ? L.s.table[(int64_t)b * L.s.ld_table + ((grp * 16) >> log2t)] : -2;
+    };
+    auto scales_at = [&](int p, float& ks, float& vs) {
+      ks = vs = 0.f;
+      if (p >= 0 && p < c.blocks) {
+        const int64_t u = (int64_t)p * c.H + hk;
+        ks = c.ks[u];
+        vs = c.vs[u];
+      }
+    };
+    int page = -2, page_n = -2;
+    float ks = 0.f, vs = 0.f, ks_n = 0.f, vs_n = 0.f, lv = 0.f, iv = 1.f;
+    auto logs = [&] {
+      const float av = fmaxf(fabsf(vs), kScaleFloor);
+      lv = vs == vs ? log2f(av) : vs;
+      iv = vs == vs ? 1.f / av : vs;
+    };
+    if (ct < 32) {
+      page = page_at(g0 + lane);
+      page_n = page_at(g0 + 32 + lane);
+    }
+    // Tile j's blocks into its raw stage and its scales into meta[j % kMeta].
     auto load = [&](int j) {
       if (j >= j1) return;
-      const int st = (j - j0) % Y::RAW;
-      TileMeta& mt = meta[(j - j0) % kMeta];
-      const int tok = j * kN + 16 * lane;  // lanes 0-7: the tile's groups
-      const bool in = lane < 8 && tok < seen;
-      const int32_t page = in ? L.s.table[(int64_t)b * L.s.ld_table + (tok >> log2t)] : -1;
-      const bool live = in && page >= 0 && page < c.blocks;
-      if (in && !live) report_error(L.status, DEV_BAD_BLOCK, 2, page);
-      const bool first = (tok & ((1 << log2t) - 1)) == 0;  // one box per block of the tile
+      const int n = j - j0, st = n & 1, w = 4 * (n & 7);
+      if ((n & 7) == 0 && n > 0) {
+        page = page_n, ks = ks_n, vs = vs_n;
+        page_n = page_at(g0 + 4 * n + 32 + lane);
+        logs();
+      }
+      if ((n & 7) == 4) scales_at(page_n, ks_n, vs_n);
+      TileMeta& mt = meta[n % kMeta];
+      const int a = lane - w;  // lanes w .. w + 3: the tile's groups
+      const bool mine = a >= 0 && a < 4;
+      const bool live = mine && page >= 0 && page < c.blocks;
+      if (mine && !live && page != -2) report_error(L.status, DEV_BAD_BLOCK, 2, page);
+      const bool first = log2t >= 6 ? a == 0 : ((16 * a) & ((1 << log2t) - 1)) == 0;  // one box per block of the tile
       const uint32_t boxes = __ballot_sync(0xffffffffu, live && first);
-      const uint32_t dead = __ballot_sync(0xffffffffu, in && !live);
+      const uint32_t dead = __ballot_sync(0xffffffffu, mine && !live && page != -2) >> w;
       const int box_rows = min(kN, 1 << log2t);
       if (lane == 0) {
-        mt.dead = (int32_t)dead;
+        mt.dead = (int32_t)(dead & 15u);  // (before the arrival: the converters read it)
         mbar_arrive_expect_tx(&B->raw[st], (uint32_t)(__popc(boxes) * 2 * box_rows * DT));
       }
       __syncwarp();
       if (boxes >> lane & 1) {
-        const int y = ((page * c.H + hk) << log2t) + (tok & ((1 << log2t) - 1));
-        uint8_t* to = base + Y::RAWS + st * 2 * Y::RAWB + 16 * lane * DT;
+        const int y = ((page * c.H + hk) << log2t) + ((j * kN + 16 * a) & ((1 << log2t) - 1));
+        uint8_t* to = base + Y::RAWS + st * 2 * Y::RAWB + 16 * a * DT;
         tc::tma_load_2d(to, &mk, 0, y, &B->raw[st]);
         tc::tma_load_2d(to + Y::RAWB, &mv, 0, y, &B->raw[st]);
       }
-      float ks = 0.f, vs = 0.f;
-      if (live) {
-        const int64_t u = (int64_t)page * c.H + hk;
-        ks = c.ks[u];
-        vs = c.vs[u];
+      if (n == 0) {  // (the first scales are fetched behind the first copies)
+        scales_at(page, ks, vs);
+        logs();
       }
-      const float av = fabsf(vs);
-      float top = live && av <= 3.4028234e38f ? av : 0.f;
-      float low = live && av <= 3.4028234e38f ? av : 3.4028234e38f;
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-      }
-      // (a tile with a negative scale, which no write makes, goes block by block too)
-      const bool neg = __any_sync(0xffffffffu, live && vs < 0.f);
-      const bool apart = log2t < 7 && (low < top * kApart<SPLIT> || neg);
-      if (lane < 8) {
-        const float ratio = apart || av == top || !live ? 1.f : av / top;
-        mt.ks[lane] = ks;
-        mt.vs[lane] = vs;
-        mt.lr[lane] = ratio == 1.f ? 0.f : log2f(ratio);
-        mt.ir[lane] = 1.f / ratio;
+      const uint32_t neg = __ballot_sync(0xffffffffu, live && vs < 0.f) >> w;
+      const uint32_t kneg = __ballot_sync(0xffffffffu, live && ks < 0.f) >> w;
+      if (mine) {
+        mt.ks[a] = ks;
+        mt.lv[a] = lv;
+        mt.iv[a] = iv;
       }
       if (lane == 0) {
-        mt.top = top;
-        mt.subs = apart ? kN >> log2t : 1;
+        mt.neg = (int32_t)(neg & 15u);
+        mt.odd = ((dead | neg | kneg) & 15u) != 0;
       }
     };
     int loaded = j0;
     if (ct < 32) {
-      for (; loaded < j0 + Y::RAW; ++loaded) load(loaded);
+      for (; loaded < j0 + 2; ++loaded) load(loaded);
     }
-    constexpr int CPR = DT / 16;  // 16-byte pieces per row
+    constexpr int CPR = DT / 16;              // 16-byte pieces per row
+    constexpr int NP = kN * CPR / 128;        // pieces of a thread, 128 / CPR rows apart
     const int pc = ct % CPR, pr = ct / CPR;
     bool ok = true;
     for (int j = j0; j < j1; ++j) {
-      const int n = j - j0, st = n % Y::RAW;
-      if (!(ok = wait_for(&B->raw[st], (uint32_t)(n / Y::RAW) & 1u, abort, L.status, W_RAW, j))) break;
+      const int n = j - j0, st = n & 1;
+      const uint32_t ph = (uint32_t)(n >> 1) & 1u;
+      ok = wait_for(&B->raw[st], ph, abort, L.status, W_RAW, j);
       const int tok0 = j * kN;
       const int nrows = min(kN, (seen - tok0 + 31) & ~31);
-      const uint32_t dead = (uint32_t)meta[n % kMeta].dead;
+      const uint32_t dead = FMT == kCacheE4m3 ? (uint32_t)meta[n % kMeta].dead : 0u;
       // bytes past the last token (or of a block that does not exist) may be NaN codes: zeros instead
       const bool cut = FMT == kCacheE4m3 && (tok0 + nrows > seen || dead);
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        if (n > 0 && !(ok = wait_for(kv ? &B->v_empty : &B->k_empty, (uint32_t)(n - 1) & 1u, abort, L.status, kv ? W_V_EMPTY : W_K_EMPTY, j)))
-          break;
-        const uint8_t* src = base + Y::RAWS + (st * 2 + kv) * Y::RAWB;
-        uint8_t* dst = base + (kv ? Y::V : Y::K);
-#pragma unroll 4
-        for (int r = pr; r < nrows; r += 128 / CPR) {
-          uint4 w = *reinterpret_cast<const uint4*>(src + r * DT + 16 * pc);
-          if (cut && (tok0 + r >= seen || (dead >> (r >> 4) & 1))) w = make_uint4(0, 0, 0, 0);
+        const uint8_t* src = base + Y::RAWS + (st * 2 + kv) * Y::RAWB + pr * DT + 16 * pc;
+        uint4 w[NP];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) w[i] = *reinterpret_cast<const uint4*>(src + i * (128 / CPR) * DT);
+        if (cut) {
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            const int r = pr + i * (128 / CPR);
+            if (tok0 + r >= seen || (dead >> (r >> 4) & 1)) w[i] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        if (ok && n >= 2)
+          ok = wait_for(kv ? &B->v_empty[st] : &B->k_empty[st], ph ^ 1u, abort, L.status, kv ? W_V_EMPTY : W_K_EMPTY, j);
+        if (!ok) break;
+        uint8_t* dst = base + (kv ? Y::V : Y::K) + st * Y::TILE + (pc >> 2) * Y::SLAB;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int r = pr + i * (128 / CPR), k = 2 * (pc & 3);
           uint4 x, y;
-          codes_in_order<FMT>(w.x, x.x, x.y);
-          codes_in_order<FMT>(w.y, x.z, x.w);
-          codes_in_order<FMT>(w.z, y.x, y.y);
-          codes_in_order<FMT>(w.w, y.z, y.w);
-          uint8_t* row = dst + (pc >> 2) * Y::SLAB + r * 128;
-          const int k = 2 * (pc & 3);
-          *reinterpret_cast<uint4*>(row + ((k ^ (r & 7)) << 4)) = x;
-          *reinterpret_cast<uint4*>(row + (((k + 1) ^ (r & 7)) << 4)) = y;
+          codes_in_order<FMT>(w[i].x, x.x, x.y);
+          codes_in_order<FMT>(w[i].y, x.z, x.w);
+          codes_in_order<FMT>(w[i].z, y.x, y.y);
+          codes_in_order<FMT>(w[i].w, y.z, y.w);
+          *reinterpret_cast<uint4*>(dst + r * 128 + ((k ^ (r & 7)) << 4)) = x;
+          *reinterpret_cast<uint4*>(dst + r * 128 + (((k + 1) ^ (r & 7)) << 4)) = y;
         }
         fence_proxy_async_smem();
-        mbar_arrive(kv ? &B->v_full : &B->k_full);
+        mbar_arrive(kv ? &B->v_full[st] : &B->k_full[st]);
       }
-      if (!ok) break;
-      bar_sync(1, 128);  // every converter has left the raw stage
+      if (!(ok = bar_and(1, 128, ok))) break;  // every converter has left the raw stage
       if (ct < 32 && loaded < j1) load(loaded++);
     }
     if (!ok && ct == 0) {  // copies in flight land before the CTA may leave
-      for (int j = j0; j < min(loaded, j1); ++j) mbar_wait_bounded(&B->raw[(j - j0) % Y::RAW], (uint32_t)((j - j0) / Y::RAW) & 1u);
+      for (int j = j0; j < min(loaded, j1); ++j) mbar_wait_clocked(&B->raw[(j - j0) & 1], (uint32_t)((j - j0) >> 1) & 1u, nullptr);
     }
   } else {
     // ---------------- softmax, MMA issue, epilogue: one row per thread ----------------
-    if constexpr (RT == 2) reg_inc<208>();
+    if constexpr (SPLIT) reg_inc<Y::REGS_SOFT>();
     const int rt = warp >> 2, tr = threadIdx.x & 127;
     const int r = rt * kM + tr;  // row of the CTA
     const bool live = r < nrow;
     const int prow = r0 + min(r, nrow - 1);
     const int qi = prow / L.G;
     const int64_t head = (int64_t)(hk * L.G + prow % L.G) * c.D;
-    const int lim = !live ? -1 : L.causal ? min(q.len - 1, past + qi) : q.len - 1;  // the last token the row sees
+    // the last token the row sees (a row past the last one goes along with that one)
+    const int lim = L.causal ? min(q.len - 1, past + qi) : q.len - 1;
     const uint32_t tl = tmem + (uint32_t)rt * Y::COL_RT + ((uint32_t)((warp & 3) * 32) << 16);  // this warp's lanes
     uint8_t* Qs = base + Y::Q + rt * Y::PARTS * Y::QPART;
 
-    // q, times a power of two that brings its largest channel into [2^13, 2^14) (and the sign of the scale)
-    float rs;
+    // q, times a power of two that brings its row's largest channel into [2^13, 2^14) (and the sign of the
+    // scale): PER lanes load a row together, 16 bytes each
+    constexpr int V8 = 16 / (int)sizeof(T);         // channels of a piece
+    constexpr int PER = DT / V8;                    // pieces of a row: 8, 16 or 32
+    constexpr int RPI = 32 / PER;                   // rows of a warp's load
+    float* rsm = reinterpret_cast<float*>(base + Y::RS) + rt * kM;
     {
-      const T* src = static_cast<const T*>(L.q) + (q.row0 + qi) * L.ldq + head;
-      const bool vec = L.vec != 0;
-      auto load8 = [&](int e, float (&x)[8]) {
-        if (!live || e >= c.D) {
+      const T* mine = live ? static_cast<const T*>(L.q) + (q.row0 + qi) * L.ldq + head : nullptr;
+      const int p = lane % PER, e = p * V8;
+      constexpr int UN = 4;  // loads under way
+      for (int i0 = 0; i0 < 32; i0 += UN * RPI) {
+        float x[UN][V8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = 0.f;
-        } else if (vec) {
-          load_row<T, 8, true>(src + e, x);
-        } else {
-          load_row<T, 8, false>(src + e, x);
-        }
-      };
-      float top = 0.f;
-#pragma unroll 4
-      for (int e = 0; e < DT; e += 8) {
-        float x[8];
-        load8(e, x);
+        for (int u = 0; u < UN; ++u) {
+          const int rl = i0 + u * RPI + lane / PER;
+          const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), rl & 31));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
-      }
-      const int ex = min(max((int)(__float_as_uint(top) >> 23), 27), 254) - 127;
-      const float up = __uint_as_float(((uint32_t)(13 - ex + 127) << 23) | (L.scale_log2 < 0.f ? 0x80000000u : 0u));
-      rs = fabsf(L.scale_log2) * __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
-#pragma unroll 4
-      for (int e = 0; e < DT; e += 8) {
-        float x[8];
-        load8(e, x);
-        uint32_t h[4], l[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[2 * i] *= up, x[2 * i + 1] *= up;
-          h[i] = pack2<__half>(x[2 * i], x[2 * i + 1]);
-          if constexpr (SPLIT) {
-            const float2 f = unpack2<__half>(h[i]);
-            l[i] = pack2<__half>(x[2 * i] - f.x, x[2 * i + 1] - f.y);
+          for (int i = 0; i < V8; ++i) x[u][i] = 0.f;
+          if (src && e < c.D) {
+            if (L.vec) load_row<T, V8, true>(src + e, x[u]);
+            else load_row<T, V8, false>(src + e, x[u]);
           }
         }
-        uint8_t* at = Qs + (e >> 6) * Y::SLAB + tr * 128 + ((((e >> 3) & 7) ^ (tr & 7)) << 4);
-        *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
-        if constexpr (SPLIT) *reinterpret_cast<uint4*>(at + Y::QPART) = make_uint4(l[0], l[1], l[2], l[3]);
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+          const int row = (tr & ~31) + i0 + u * RPI + lane / PER;
+          float top = 0.f;
+#pragma unroll
+          for (int i = 0; i < V8; ++i) top = fmaxf(top, fabsf(x[u][i]));
+#pragma unroll
+          for (int o = PER / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const int ex = min(max((int)(__float_as_uint(top) >> 23), 27), 254) - 127;
+          const float up = __uint_as_float(((uint32_t)(13 - ex + 127) << 23) | (L.scale_log2 < 0.f ? 0x80000000u : 0u));
+          if (p == 0) rsm[row] = fabsf(L.scale_log2) * __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
+          uint32_t h[V8 / 2], lo[V8 / 2];
+#pragma unroll
+          for (int i = 0; i < V8 / 2; ++i) {
+            const float y0 = x[u][2 * i] * up, y1 = x[u][2 * i + 1] * up;
+            h[i] = pack2<__half>(y0, y1);
+            const float2 f = unpack2<__half>(h[i]);
+            lo[i] = SPLIT ? pack2<__half>(y0 - f.x, y1 - f.y) : 0u;
+          }
+          uint8_t* at = Qs + (e >> 6) * Y::QSLAB + row * 128 + ((((e >> 3) & 7) ^ (row & 7)) << 4) + (e & 7) * 2;
+          if constexpr (V8 == 8) {
+            *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+          } else {
+            *reinterpret_cast<uint2*>(at) = make_uint2(h[0], h[1]);
+            *reinterpret_cast<uint2*>(at + Y::QPART) = make_uint2(lo[0], lo[1]);
+          }
+        }
       }
       fence_proxy_async_smem();
     }
     bar_sync(2 + rt, 128);
+    const float rs = rsm[tr];
 
     bool ok = true;
-    // S of tile j (its first n tokens) into the row tile's S columns, by the row tile's first thread.
-    auto issue_s = [&](int j, bool first) {
-      if (first && !wait_for(&B->k_full, (uint32_t)(j - j0) & 1u, abort, L.status, W_K_FULL, j)) return;
+    // By one lane of the row tile's first warp: the scores of tile j into the S buffer of its parity, and P's
+    // product with V. Each releases its operand's stage.
+    const bool issuer = (warp & 3) == 0;
+    const uint64_t dq = tc::smem_desc(base + Y::Q + rt * Y::PARTS * Y::QPART, 16, 1024, tc::kLayoutSW128);
+    const uint64_t dk = tc::smem_desc(base + Y::K, 16, 1024, tc::kLayoutSW128);
+    // V is MN-major: 64-channel slabs SLAB apart (LBO), 8-token groups 1024 B apart (SBO)
+    const uint64_t dv = tc::smem_desc(base + Y::V, Y::SLAB, 1024, tc::kLayoutSW128);
+    const uint32_t trt = tmem + (uint32_t)rt * Y::COL_RT;
+    auto issue_s = [&](int j) {
+      const int n = j - j0, st = n & 1;
+      if (!wait_for(&B->k_full[st], (uint32_t)(n >> 1) & 1u, abort, L.status, W_K_FULL, j)) return;
       tc::fence_after_sync();
-      const int n = min(kN, (seen - j * kN + 31) & ~31);
-      const uint32_t id = idesc_f16(n, false);
-      const uint32_t d = tmem + (uint32_t)rt * Y::COL_RT;
+      const uint32_t id = idesc_f16(min(kN, (seen - j * kN + 31) & ~31), false);
+      const uint32_t d = trt + (uint32_t)(st * kN);
+      const uint64_t dks = dk + (uint64_t)(st * (Y::TILE >> 4));
 #pragma unroll
       for (int p = 0; p < Y::PARTS; ++p)
 #pragma unroll
-        for (int k = 0; k < DT / 16; ++k) {
-          const uint64_t a = tc::smem_desc(Qs + p * Y::QPART + (k >> 2) * Y::SLAB + (k & 3) * 32, 16, 1024, tc::kLayoutSW128);
-          const uint64_t w = tc::smem_desc(base + Y::K + (k >> 2) * Y::SLAB + (k & 3) * 32, 16, 1024, tc::kLayoutSW128);
-          mma_ss(d, a, w, id, p + k > 0);
-        }
-      tc::commit(&B->s_full[rt]);
+        for (int k = 0; k < DT / 16; ++k)
+          mma_ss(d, dq + ((p * Y::QPART + (k >> 2) * Y::QSLAB + (k & 3) * 32) >> 4), dks + (((k >> 2) * Y::SLAB + (k & 3) * 32) >> 4), id,
+                 p + k > 0);
+      tc::commit(&B->s_full[rt][st]);
+      tc::commit(&B->k_empty[st]);
     };
-    auto issue_pv = [&](int j, bool first, bool last) {
-      if (first && !wait_for(&B->v_full, (uint32_t)(j - j0) & 1u, abort, L.status, W_V_FULL, j)) return;
+    auto issue_pv = [&](int j) {
+      const int n = j - j0, st = n & 1;
+      if (!wait_for(&B->v_full[st], (uint32_t)(n >> 1) & 1u, abort, L.status, W_V_FULL, j)) return;
       tc::fence_after_sync();
       const int steps = (min(kN, seen - j * kN) + 15) >> 4;
       constexpr uint32_t id = idesc_f16(DT, true);
-      const uint32_t s0 = tmem + (uint32_t)rt * Y::COL_RT, d = s0 + Y::COL_ACC;
-      for (int k = 0; k < steps; ++k) {
-        // V is MN-major: 64-channel slabs SLAB apart (LBO), 8-token groups 1024 B apart (SBO)
-        const uint64_t w = tc::smem_desc(base + Y::V + k * 2048, Y::SLAB, 1024, tc::kLayoutSW128);
+      const uint32_t s0 = trt + (uint32_t)(st * kN), d = trt + Y::COL_ACC;
+      const uint64_t dvs = dv + (uint64_t)(st * (Y::TILE >> 4));
+#pragma unroll
+      for (int k = 0; k < kN / 16; ++k) {
+        if (k >= steps) break;
         const uint32_t a = s0 + 32 * (k >> 1) + 8 * (k & 1);  // P of 32 tokens: 16 columns, then its low part
-        mma_ts(d, a, w, id, k > 0);
-        if constexpr (SPLIT) mma_ts(d, a + 16, w, id, 1);
+        mma_ts(d, a, dvs + ((k * 2048) >> 4), id, k > 0 || (!SPLIT && n > 0));
+        if constexpr (SPLIT) mma_ts(d, a + 16, dvs + ((k * 2048) >> 4), id, 1);
       }
       tc::commit(&B->pv_full[rt]);
-      if (last) tc::commit(&B->v_empty);
+      tc::commit(&B->v_empty[st]);
     };
 
-    float o[DT];
+    constexpr int OR = SPLIT ? DT / 2 : 1;
+    float2 o[OR];  // fp32 rows: O
 #pragma unroll
-    for (int e = 0; e < DT; ++e) o[e] = 0.f;
+    for (int e = 0; e < OR; ++e) o[e] = make_float2(0.f, 0.f);
     float m = -INFINITY, l = 0.f;
-    int it = 0;  // passes: tiles, or parts of tiles
-    if (j0 < j1 && tr == 0) issue_s(j0, true);
-    for (int j = j0; j < j1 && ok; ++j) {
-      const TileMeta& mt = meta[(j - j0) % kMeta];
-      const int tok0 = j * kN;
-      const int ncol = min(kN, seen - tok0), nch = (ncol + 31) >> 5;
-      int subs = 1;
-      for (int sub = 0; sub < subs && ok; ++sub, ++it) {
-        if (!(ok = wait_for(&B->s_full[rt], (uint32_t)it & 1u, abort, L.status, W_S, j))) break;
-        tc::fence_after_sync();
-        if (sub == 0) subs = mt.subs;  // (written before the tile's K was converted)
-        if (tr == 0 && sub + 1 == subs) tc::commit(&B->k_empty);  // the tile's last scores are formed
-        // columns of this pass that the row sees: [lo, hi)
-        const int lo = subs > 1 ? sub << c.log2t : 0;
-        const int end = subs > 1 ? min(ncol, (sub + 1) << c.log2t) : ncol;
-        const int hi = min(end, lim - tok0 + 1);
-        const bool partial = subs > 1 || tok0 + ncol > all || (ncol & 31) || mt.dead;
-        const uint32_t deadm = (uint32_t)mt.dead;
-        // what the product is multiplied by: a row that sees none of it has a product of 0 and takes 0
-        const float v0 = mt.vs[lo >> 4];
-        const float f = hi <= lo ? 0.f : subs > 1 ? v0 : v0 < 0.f ? -mt.top : mt.top;
-
-        // the row's maximum: the largest score of each 16 tokens (32, when blocks hold as many) times their
-        // factor
-        float mx = -INFINITY;
-        auto largest = [](const float* s) {
-          float u = max3(s[0], s[1], s[2]), w = max3(s[3], s[4], s[5]);
+    auto product_done = [&](int n) {  // of the tile n after the CTA's first
+      return __all_sync(0xffffffffu, wait_for(&B->pv_full[rt], (uint32_t)n & 1u, abort, L.status, W_PV, n));
+    };
+    auto add_product = [&] {
+      tc::fence_after_sync();
 #pragma unroll
-          for (int e = 6; e < 14; e += 4) u = max3(u, s[e], s[e + 1]), w = max3(w, s[e + 2], s[e + 3]);
-          u = max3(u, s[14], s[15]);
-          return fmaxf(u, w);
-        };
-        for (int ch = 0; ch < nch; ++ch) {
-          float s[32];
-          tc::tmem_ld32(tl + 32 * ch, s);
-          const float k0 = mt.ks[2 * ch] * rs, k1 = mt.ks[2 * ch + 1] * rs;
-          tc::tmem_wait_ld();
-          if (partial) {
+      for (int e = 0; e < DT; e += 32) {
+        float a[32];
+        tc::tmem_ld32(tl + Y::COL_ACC + e, a);
+        tc::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int col = 32 * ch + e;
-              if (col < lo || col >= hi || (deadm >> (2 * ch + (e >> 4)) & 1)) s[e] = k0 < 0.f ? INFINITY : -INFINITY;
-            }
-          }
-          if (k0 < 0.f || k1 < 0.f) {  // (a negative K scale, which no write makes: score by score)
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float y = fabsf(s[e]) < INFINITY ? s[e] * (e < 16 ? k0 : k1) : -INFINITY;
-              mx = fmaxf(mx, y);
-            }
-          } else {
-            const float a0 = largest(s), a1 = largest(s + 16);
-            mx = max3(mx, a0 * k0, a1 * k1);  // (-inf times a factor of 0 is NaN, which the maximum leaves out)
-          }
+        for (int i = 0; i < 16; ++i) {
+          float2& x = o[SPLIT ? e / 2 + i : 0];
+          x = __fadd2_rn(make_float2(a[2 * i], a[2 * i + 1]), x);
         }
-        const float mn = fmaxf(m, mx);
-        const float ref = mn == -INFINITY ? 0.f : mn;
-        const float al = ex2f(m - ref);
-        const bool moved = mn != m;
-        m = mn;
-        // p, its sum, and P into the columns of the scores it comes from
-        float sum = 0.f;
-        for (int ch = 0; ch < nch; ++ch) {
-          float s[32];
-          tc::tmem_ld32(tl + 32 * ch, s);
-          const float k0 = mt.ks[2 * ch] * rs, k1 = mt.ks[2 * ch + 1] * rs;
-          const float h0 = kPShift - ref + mt.lr[2 * ch], h1 = kPShift - ref + mt.lr[2 * ch + 1];
-          const float i0 = mt.ir[2 * ch], i1 = mt.ir[2 * ch + 1];
-          tc::tmem_wait_ld();
-          uint32_t ph[16], pl[SPLIT ? 16 : 1];
-          float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          auto form = [&](auto masked) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float k = e < 16 ? k0 : k1, h = e < 16 ? h0 : h1;
-              float2 x = __ffma2_rn(make_float2(s[e], s[e + 1]), make_float2(k, k), make_float2(h, h));
-              if constexpr (decltype(masked)::value) {
-                const int col = 32 * ch + e;
-                const bool dd = deadm >> (2 * ch + (e >> 4)) & 1;
-                if (col < lo || col >= hi || dd) x.x = -INFINITY;
-                if (col + 1 < lo || col + 1 >= hi || dd) x.y = -INFINITY;
-              }
-              x.x = ex2f(x.x);
-              x.y = ex2f(x.y);
-              part[e >> 4] = __fadd2_rn(part[e >> 4], x);
-              const int w = e >> 1;
-              ph[w] = pack2<__half>(x.x, x.y);
-              if constexpr (SPLIT) {
-                const float2 f = unpack2<__half>(ph[w]);
-                const float2 d = __ffma2_rn(f, make_float2(-1.f, -1.f), x);
-                pl[w] = pack2<__half>(d.x, d.y);
-              }
-            }
-          };
-          if (partial) form(std::true_type{});
-          else form(std::false_type{});
-          const float p0 = part[0].x + part[0].y, p1 = part[1].x + part[1].y;
-          // (the ratio of a block that no visible token is in may be NaN)
-          sum += (p0 == 0.f ? 0.f : p0 * i0) + (p1 == 0.f ? 0.f : p1 * i1);
-          tmem_st16(tl + 32 * ch, ph);
-          if constexpr (SPLIT) tmem_st16(tl + 32 * ch + 16, pl);
-        }
-        l = l * al + sum;
-        tc::tmem_wait_st();
-        tc::fence_before_sync();
-        bar_sync(2 + rt, 128);
-        const bool lastsub = sub + 1 == subs;
-        if (tr == 0) issue_pv(j, sub == 0, lastsub);
-        if (!(ok = wait_for(&B->pv_full[rt], (uint32_t)it & 1u, abort, L.status, W_PV, j))) break;
-        tc::fence_after_sync();
-        // the next scores, while this product is added to O
-        if (tr == 0) {
-          if (!lastsub) issue_s(j, false);
-          else if (j + 1 < j1) issue_s(j + 1, true);
-        }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-          for (int e = 0; e < DT; e += 2) {
-            const float2 w = __fmul2_rn(make_float2(o[e], o[e + 1]), make_float2(al, al));
-            o[e] = w.x, o[e + 1] = w.y;
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < DT; e += 32) {
-          float a[32];
-          tc::tmem_ld32(tl + Y::COL_ACC + e, a);
-          tc::tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float2 y = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(f, f), make_float2(o[e + i], o[e + i + 1]));
-            o[e + i] = y.x, o[e + i + 1] = y.y;
-          }
-        }
-        tc::fence_before_sync();
       }
+    };
+    if (j0 < j1 && issuer && elect_one()) issue_s(j0);
+    __syncwarp();
+    for (int j = j0; j < j1; ++j) {
+      const int n = j - j0;
+      const TileMeta& mt = meta[n % kMeta];
+      const int tok0 = j * kN;
+      // (a warp that gives up a wait goes on to the barrier, where all leave together)
+      if (!__all_sync(0xffffffffu, wait_for(&B->s_full[rt][n & 1], (uint32_t)(n >> 1) & 1u, abort, L.status, W_S, j))) {
+        ok = bar_and(2 + rt, 128, false);
+        break;
+      }
+      tc::fence_after_sync();
+      const uint32_t ts = tl + (uint32_t)((n & 1) * kN);
+      constexpr int CH = Y::CHUNK;
+      float s[CH];
+      auto load_s = [&](int c0) {
+        if constexpr (CH == 64) tc::tmem_ld64(ts, s);
+        else tc::tmem_ld32(ts + c0, s);
+        tc::tmem_wait_ld();
+      };
+      // The common tile, all of it seen by every row of the warp, and any other, score by score.
+      const bool plain = !mt.odd && __all_sync(0xffffffffu, lim >= tok0 + kN - 1);
+      uint64_t vis = ~0ull;  // the columns that the row sees
+      if (!plain) {
+        const int hi = min(max(lim - tok0 + 1, 0), kN);
+        vis = hi == kN ? ~0ull : (1ull << hi) - 1ull;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (mt.dead >> g & 1) vis &= ~(0xffffull << (16 * g));
+      }
+      // the row's largest exponent
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c0 = 0; c0 < kN; c0 += CH) {
+        load_s(c0);
+        if (plain) {
+#pragma unroll
+          for (int g = 0; g < CH / 16; ++g) {
+            const float* x = s + 16 * g;
+            float u = max3(x[0], x[1], x[2]), w = max3(x[3], x[4], x[5]);
+#pragma unroll
+            for (int e = 6; e < 14; e += 4) u = max3(u, x[e], x[e + 1]), w = max3(w, x[e + 2], x[e + 3]);
+            u = max3(u, x[14], x[15]);
+            mx = fmaxf(mx, fmaf(fmaxf(u, w), mt.ks[c0 / 16 + g] * rs, mt.lv[c0 / 16 + g]));
+          }
+        } else {
+          const uint64_t v = vis >> c0;
+#pragma unroll
+          for (int e = 0; e < CH; ++e) {
+            const int g = (c0 + e) >> 4;
+            if (v >> e & 1) mx = fmaxf(mx, fmaf(s[e], mt.ks[g] * rs, mt.lv[g]));
+          }
+        }
+      }
+      // the next scores, into the buffer of the previous P once its product is formed
+      if (issuer && elect_one() && j + 1 < j1 &&
+          (n == 0 || wait_for(&B->pv_full[rt], (uint32_t)(n - 1) & 1u, abort, L.status, W_PV, j)))
+        issue_s(j + 1);
+      __syncwarp();
+      const float mn = SPLIT ? fmaxf(m, mx) : mx > m + kLag || m == -INFINITY ? fmaxf(m, mx) : m;
+      const bool moved = __any_sync(0xffffffffu, mn != m);
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      const float al = ex2f(m - ref);
+      m = mn;
+      // P into the columns of the scores that it comes from, and its sum
+      float sum = 0.f;
+#pragma unroll
+      for (int c0 = 0; c0 < kN; c0 += CH) {
+        if (CH < kN) load_s(c0);
+        auto form = [&](auto masked) {
+#pragma unroll
+          for (int h = 0; h < CH / 32; ++h) {
+            uint32_t ph[16], pl[SPLIT ? 16 : 1];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const int grp = c0 / 16 + 2 * h + g;
+              const float k = mt.ks[grp] * rs, sh = mt.lv[grp] - ref + kPShift<SPLIT>;
+              float2 part = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) {
+                const int i = 32 * h + 16 * g + e;
+                float2 x = __ffma2_rn(make_float2(s[i], s[i + 1]), make_float2(k, k), make_float2(sh, sh));
+                if constexpr (decltype(masked)::value) {
+                  if (!(vis >> (c0 + i) & 1)) x.x = -INFINITY;
+                  if (!(vis >> (c0 + i + 1) & 1)) x.y = -INFINITY;
+                }
+                x.x = ex2f(x.x);
+                x.y = ex2f(x.y);
+                part = __fadd2_rn(part, x);
+                if constexpr (decltype(masked)::value) {
+                  if (mt.neg >> grp & 1) x.x = -x.x, x.y = -x.y;
+                }
+                const int w = 8 * g + (e >> 1);
+                ph[w] = pack2<__half>(x.x, x.y);
+                if constexpr (SPLIT) {
+                  const float2 y = unpack2<__half>(ph[w]);
+                  const float2 d = __ffma2_rn(y, make_float2(-1.f, -1.f), x);
+                  pl[w] = pack2<__half>(d.x, d.y);
+                }
+              }
+              const float p = part.x + part.y;
+              if constexpr (decltype(masked)::value) sum += p == 0.f ? 0.f : p * mt.iv[grp];  // (an unseen block's may be NaN)
+              else sum = fmaf(p, mt.iv[grp], sum);
+            }
+            tmem_st16(ts + c0 + 32 * h, ph);
+            if constexpr (SPLIT) tmem_st16(ts + c0 + 32 * h + 16, pl);
+          }
+        };
+        if (plain) form(std::false_type{});
+        else form(std::true_type{});
+      }
+      l = fmaf(l, al, sum);
+      if (n > 0 && (SPLIT || moved)) {
+        // fp32 rows: the previous product joins O. Either: O follows m.
+        ok = product_done(n - 1);
+        if (SPLIT && ok) add_product();
+        if (moved && ok) {
+          if constexpr (SPLIT) {
+#pragma unroll
+            for (int e = 0; e < OR; ++e) o[e] = __fmul2_rn(o[e], make_float2(al, al));
+          } else {
+            tc::fence_after_sync();
+#pragma unroll 1
+            for (int e = 0; e < DT; e += 32) {
+              float a[32];
+              tc::tmem_ld32(tl + Y::COL_ACC + e, a);
+              tc::tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) a[i] *= al;
+              tc::tmem_st32(tl + Y::COL_ACC + e, a);
+            }
+          }
+        }
+      }
+      tc::tmem_wait_st();
+      tc::fence_before_sync();
+      if (!(ok = bar_and(2 + rt, 128, ok))) break;
+      if (issuer && elect_one()) issue_pv(j);
+      __syncwarp();
     }
-    if (!ok && tr == 0 && *abort) {
+    if (ok && j0 < j1) {
+      ok = product_done(j1 - j0 - 1);
+      tc::fence_after_sync();
+      if (SPLIT && ok) add_product();
+    }
+    if (!ok && *abort && issuer && elect_one()) {
       // MMAs in flight end before TMEM is freed: an arrival of their own, waited for within limits
       tc::commit(&B->drain[rt]);
-      mbar_wait_bounded(&B->drain[rt], 0);
+      mbar_wait_clocked(&B->drain[rt], 0, nullptr);
     }
+    __syncwarp();
 
     // ---- epilogue: the row through shared memory (its own Q rows), stored in whole 16-byte pieces ----
-    if (L.ws_o) {
-      if (live) {
-        const int64_t at = (int64_t)blockIdx.x * (kM * RT) + r;
+    // 32 channels of the row's O
+    auto channels = [&](int e, float (&x)[32]) {
+      if constexpr (SPLIT) {
 #pragma unroll
-        for (int e = 0; e < DT; e += 4)
-          if (e < c.D) *reinterpret_cast<float4*>(L.ws_o + at * c.D + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-        L.ws_ml[at] = make_float2(m, l);
+        for (int i = 0; i < 16; ++i) x[2 * i] = o[e / 2 + i].x, x[2 * i + 1] = o[e / 2 + i].y;
+      } else if (j0 < j1 && ok) {
+        tc::tmem_ld32(tl + Y::COL_ACC + e, x);
+        tc::tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = 0.f;
       }
+    };
+    if (L.ws_o) {
+      const int64_t at = (int64_t)blockIdx.x * (kM * RT) + r;
+#pragma unroll
+      for (int e = 0; e < DT; e += 32) {
+        float x[32];
+        channels(e, x);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          if (live && e + i < c.D) *reinterpret_cast<float4*>(L.ws_o + at * c.D + e + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+      }
+      if (live) L.ws_ml[at] = make_float2(m, l);
     } else {
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      constexpr int PER = DT * (int)sizeof(T) / 16;  // pieces of a row
-      constexpr int V8 = 16 / (int)sizeof(T);
       uint8_t* mine = Qs + tr * (PER * 16);
 #pragma unroll
-      for (int p = 0; p < PER; ++p) {
-        float x[V8];
+      for (int e = 0; e < DT; e += 32) {
+        float x[32];
+        channels(e, x);
 #pragma unroll
-        for (int i = 0; i < V8; ++i) x[i] = l == 0.f ? 0.f : o[p * V8 + i] * inv;
-        store_row<T, V8, true>(reinterpret_cast<T*>(mine + ((p ^ (tr & 7)) << 4)), x);
+        for (int i = 0; i < 32; i += V8) {
+          float y[V8];
+#pragma unroll
+          for (int k = 0; k < V8; ++k) y[k] = l == 0.f ? 0.f : x[i + k] * inv;
+          const int p = (e + i) / V8;
+          store_row<T, V8, true>(reinterpret_cast<T*>(mine + ((p ^ (tr & 7)) << 4)), y);
+        }
       }
       __syncwarp();
       const int per = c.D / V8;  // pieces that exist
       // each row's address is known to its own thread
       T* mine_out = live ? static_cast<T*>(L.o) + (q.row0 + qi) * L.ldo + head : nullptr;
-      constexpr int RPI = 32 / PER;  // rows of an iteration
 #pragma unroll 4
-      for (int i = 0; i < 32; i += (RPI > 0 ? RPI : 1)) {
-        const int rl = i + (RPI > 0 ? lane / PER : 0), p = lane % PER;
+      for (int i = 0; i < 32; i += RPI) {
+        const int rl = i + lane / PER, p = lane % PER;
         T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine_out), rl));
         const T* from = reinterpret_cast<const T*>(Qs + ((tr & ~31) + rl) * (PER * 16) + ((p ^ (rl & 7)) << 4));
         if (!to || p >= per) continue;

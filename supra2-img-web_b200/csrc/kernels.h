@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 namespace supra {
 
 // Device status codes written to the context's status word (status[0]).
@@ -371,12 +373,12 @@ struct CacheAttnArgs {
 };
 // Boxes of the K and V pools, seen as [blocks * H * block_tokens, D] bytes: cache_attn_box_cols(D)
 // columns (zeros past D) and rows inside one block: for the rows kernel up to 32 with the swizzle of the
-// box's width, for the tensor-core kernel whole blocks without one.
+// box's width, for the tensor-core kernel up to 64 without one.
 struct CacheAttnLaunch : CacheAttnArgs {
   CUtensorMap mk, mv;
 };
 inline int cache_attn_box_cols(int D) { return D <= 64 ? 64 : 128; }
-inline int cache_attn_box_rows(int log2t, bool tc) { return tc ? 1 << log2t : log2t >= 5 ? 32 : 16; }
+inline int cache_attn_box_rows(int log2t, bool tc) { return std::min(1 << log2t, tc ? 64 : 32); }
 // How a call is split, from its sizes alone.
 struct CacheAttnPlan {
   bool tc;           // the tensor-core kernel (cache_attn_tc.cu)

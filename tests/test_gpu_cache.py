@@ -206,8 +206,8 @@ def test_write_of_values_that_are_not_finite(gpu):
 #     it (or its second part) is below 2^-14, where fp16 numbers are 2^-24 apart, by up to 2^-25: 2^-37 of
 #     the largest p, which is 1 and at most the sum of all, for each token: 2^-37 sum |v| of the quotient,
 #     however small p is (it shows where the tokens with large p have v = 0). Where many rows share a tile
-#     it is 2^15 p times its block's V scale over the tile's largest, no less than 2^-3 for fp32 (2^-37
-#     again) and 2^-8 for the others: 2^-32;
+#     it is p times its block's V scale, relative to the row's largest such product, times 2^15 (fp32) or at
+#     least 2^7: 2^-40 or 2^-32 of that product for each token, sum |code| of it;
 #   sums over tokens: a rounding for each 16 tokens, (tokens / 16 + 40) u of sum p|v|;
 #   the quotient: the error of sum p relative to itself is the same, so both count: twice;
 #   the result's own rounding: eps / 2 of its type (fp16 numbers below 2^-14 are 2^-24 apart: 2^-25).
@@ -218,7 +218,7 @@ def attention_bound(dtype, D, tokens, out, pv, av, st, sm):
         ds = ds + 2.0 ** -22 * st
     p = (2.0 ** -22 if dtype == "fp32" else 2.0 ** -12) + 2.0 ** -21
     rel = 2 * (np.expm1(ds) + p + (tokens / 16 + 40) * u)
-    err = rel[..., None] * pv + 2.0 ** (-37 if dtype == "fp32" else -32) * av
+    err = rel[..., None] * pv + 2.0 ** -37 * av[0] + 2.0 ** (-40 if dtype == "fp32" else -32) * av[1]
     return err + torch.finfo(TYPES[dtype]).eps / 2 * (np.abs(out) + err) + (2.0 ** -25 if dtype == "fp16" else 1e-37)
 
 
