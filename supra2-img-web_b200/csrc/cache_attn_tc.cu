@@ -8,7 +8,7 @@
 //                    token's block, m the row's largest exponent so far
 //   O += P C_v       tcgen05.mma kind::f16, P from TMEM x V codes (smem, MN-major)
 //   o = O / sum(P / v)
-// Codes are exact in fp16, so 8-bit K and V cost the tensor cores nothing but their conversion: four
+// Codes are exact in fp16, so 8-bit K and V cost the tensor cores nothing but their conversion: three
 // converter warps turn the raw bytes, which the TMA unit brings in block by block, into the swizzled
 // operand tiles, once for all rows of the CTA. P carries the V scale as an exponent, which costs nothing
 // per score, and m follows the product of both, so each row's P is as large as fp16 allows whatever the
@@ -49,11 +49,16 @@ template <int DT, bool SPLIT>
 struct Cfg {
   static constexpr int RT = DT == 64 ? 1 : 2;  // row tiles
   static constexpr int SOFT = 128 * RT;        // softmax threads
+  static constexpr int CONV = 96;  // converter threads, followed by one warp that issues the MMAs
   static constexpr int THREADS = SOFT + 128;
   static constexpr int PER_SM = DT == 64 ? 2 : 1;
   static constexpr int PARTS = SPLIT ? 2 : 1;
   static constexpr int CHUNK = SPLIT && DT == 128 ? 32 : 64;  // scores that a thread holds at once
-  static constexpr int REGS_SOFT = DT == 64 ? 168 : 208, REGS_CONV = 88;  // (SPLIT) 128 or 168 at launch
+  // fp32 rows: registers of a thread at launch, and after the softmax threads have taken some from the
+  // others; together no more than the CTA was launched with (the launcher checks what that was).
+  static constexpr int REGS = DT == 64 ? 128 : 168;
+  static constexpr int REGS_SOFT = DT == 64 ? 168 : 208, REGS_REST = 88;
+  static_assert(SOFT * REGS_SOFT + 128 * REGS_REST <= THREADS * REGS, "registers");
   static constexpr int SLABS = DT / 64;                       // 64-channel slabs of an operand tile
   static constexpr uint32_t QSLAB = kM * 128;                 // 128 rows of 128 bytes
   static constexpr uint32_t QPART = SLABS * QSLAB;            // one part of one row tile
@@ -86,14 +91,14 @@ struct TileMeta {  // of a tile's four 16-token groups
 static_assert(sizeof(TileMeta) == 64, "META");
 
 struct Bars {
-  uint64_t raw[2], k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2][2], pv_full[2], drain[2];
+  uint64_t raw[2], k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2][2], p_full[2], pv_full[2], drain;
   uint32_t tmem;
   int32_t abort;
 };
 static_assert(sizeof(Bars) <= 192, "BAR");
 
 // status[2] of a wait that ran out
-enum TcWait : int32_t { W_RAW = 80, W_K_FULL = 81, W_V_FULL = 82, W_K_EMPTY = 83, W_V_EMPTY = 84, W_S = 85, W_PV = 86 };
+enum TcWait : int32_t { W_RAW = 80, W_K_FULL = 81, W_V_FULL = 82, W_K_EMPTY = 83, W_V_EMPTY = 84, W_S = 85, W_PV = 86, W_P = 87 };
 
 __device__ __forceinline__ float ex2f(float x) {
   float y;
@@ -228,15 +233,16 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&B->raw[i], 1);
-      mbar_init(&B->k_full[i], 128);
-      mbar_init(&B->v_full[i], 128);
+      mbar_init(&B->k_full[i], Y::CONV);
+      mbar_init(&B->v_full[i], Y::CONV);
       mbar_init(&B->k_empty[i], RT);
       mbar_init(&B->v_empty[i], RT);
       mbar_init(&B->s_full[i][0], 1);
       mbar_init(&B->s_full[i][1], 1);
+      mbar_init(&B->p_full[i], 128);
       mbar_init(&B->pv_full[i], 1);
-      mbar_init(&B->drain[i], 1);
     }
+    mbar_init(&B->drain, 1);
     B->abort = 0;
     mbar_fence_init();
   }
@@ -252,9 +258,9 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
   tc::fence_after_sync();
   const uint32_t tmem = B->tmem;
 
-  if (warp >= 4 * RT) {
+  if (warp >= 4 * RT && warp < 4 * RT + 3) {
     // ---------------- converters ----------------
-    if constexpr (SPLIT) reg_dec<Y::REGS_CONV>();
+    if constexpr (SPLIT) reg_dec<Y::REGS_REST>();
     const int ct = threadIdx.x - Y::SOFT;
     const int log2t = c.log2t;
     // The first warp knows the blocks of 8 tiles at a time, a 16-token group per lane, and loads the next
@@ -332,9 +338,8 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
     if (ct < 32) {
       for (; loaded < j0 + 2; ++loaded) load(loaded);
     }
-    constexpr int CPR = DT / 16;              // 16-byte pieces per row
-    constexpr int NP = kN * CPR / 128;        // pieces of a thread, 128 / CPR rows apart
-    const int pc = ct % CPR, pr = ct / CPR;
+    constexpr int CPR = DT / 16;                                       // 16-byte pieces per row
+    constexpr int PIECES = kN * CPR, NP = (PIECES + Y::CONV - 1) / Y::CONV;  // of a tile, of a thread
     bool ok = true;
     for (int j = j0; j < j1; ++j) {
       const int n = j - j0, st = n & 1;
@@ -347,24 +352,29 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       const bool cut = FMT == kCacheE4m3 && (tok0 + nrows > seen || dead);
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        const uint8_t* src = base + Y::RAWS + (st * 2 + kv) * Y::RAWB + pr * DT + 16 * pc;
+        const uint8_t* src = base + Y::RAWS + (st * 2 + kv) * Y::RAWB;
         uint4 w[NP];
 #pragma unroll
-        for (int i = 0; i < NP; ++i) w[i] = *reinterpret_cast<const uint4*>(src + i * (128 / CPR) * DT);
+        for (int i = 0; i < NP; ++i) {
+          const int p = ct + i * Y::CONV;
+          if (p < PIECES) w[i] = *reinterpret_cast<const uint4*>(src + 16 * p);
+        }
         if (cut) {
 #pragma unroll
           for (int i = 0; i < NP; ++i) {
-            const int r = pr + i * (128 / CPR);
+            const int r = (ct + i * Y::CONV) / CPR;
             if (tok0 + r >= seen || (dead >> (r >> 4) & 1)) w[i] = make_uint4(0, 0, 0, 0);
           }
         }
         if (ok && n >= 2)
           ok = wait_for(kv ? &B->v_empty[st] : &B->k_empty[st], ph ^ 1u, abort, L.status, kv ? W_V_EMPTY : W_K_EMPTY, j);
         if (!ok) break;
-        uint8_t* dst = base + (kv ? Y::V : Y::K) + st * Y::TILE + (pc >> 2) * Y::SLAB;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          const int r = pr + i * (128 / CPR), k = 2 * (pc & 3);
+          const int p = ct + i * Y::CONV;
+          if (p >= PIECES) break;
+          const int r = p / CPR, pc = p % CPR, k = 2 * (pc & 3);
+          uint8_t* dst = base + (kv ? Y::V : Y::K) + st * Y::TILE + (pc >> 2) * Y::SLAB;
           uint4 x, y;
           codes_in_order<FMT>(w[i].x, x.x, x.y);
           codes_in_order<FMT>(w[i].y, x.z, x.w);
@@ -376,14 +386,94 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         fence_proxy_async_smem();
         mbar_arrive(kv ? &B->v_full[st] : &B->k_full[st]);
       }
-      if (!(ok = bar_and(1, 128, ok))) break;  // every converter has left the raw stage
+      if (!(ok = bar_and(1, Y::CONV, ok))) break;  // every converter has left the raw stage
       if (ct < 32 && loaded < j1) load(loaded++);
     }
     if (!ok && ct == 0) {  // copies in flight land before the CTA may leave
       for (int j = j0; j < min(loaded, j1); ++j) mbar_wait_clocked(&B->raw[(j - j0) & 1], (uint32_t)((j - j0) >> 1) & 1u, nullptr);
     }
+  } else if (warp == 4 * RT + 3) {
+    // ---------------- MMA issue ----------------
+    if constexpr (SPLIT) reg_dec<Y::REGS_REST>();
+    const uint64_t dq0 = tc::smem_desc(base + Y::Q, 16, 1024, tc::kLayoutSW128);
+    const uint64_t dk = tc::smem_desc(base + Y::K, 16, 1024, tc::kLayoutSW128);
+    // V is MN-major: 64-channel slabs SLAB apart (LBO), 8-token groups 1024 B apart (SBO)
+    const uint64_t dv = tc::smem_desc(base + Y::V, Y::SLAB, 1024, tc::kLayoutSW128);
+    auto all_wait = [&](uint64_t* bar, uint32_t parity, int32_t id, int32_t detail) {
+      const bool ok = __all_sync(0xffffffffu, wait_for(bar, parity, abort, L.status, id, detail));
+      tc::fence_after_sync();
+      return ok;
+    };
+    // The scores of tile j into the S buffer of its parity, and P's product with V; each releases its
+    // operand's stage.
+    auto issue_s = [&](int rt, int j) {
+      const int n = j - j0, st = n & 1;
+      const uint64_t dq = dq0 + (uint64_t)(rt * ((Y::PARTS * Y::QPART) >> 4));
+      if (!all_wait(&B->k_full[st], (uint32_t)(n >> 1) & 1u, W_K_FULL, j)) return false;
+      if (elect_one()) {
+        const uint32_t id = idesc_f16(min(kN, (seen - j * kN + 31) & ~31), false);
+        const uint32_t d = tmem + (uint32_t)(rt * Y::COL_RT + st * kN);
+        const uint64_t dks = dk + (uint64_t)(st * (Y::TILE >> 4));
+#pragma unroll
+        for (int p = 0; p < Y::PARTS; ++p)
+#pragma unroll
+          for (int k = 0; k < DT / 16; ++k)
+            mma_ss(d, dq + ((p * Y::QPART + (k >> 2) * Y::QSLAB + (k & 3) * 32) >> 4), dks + (((k >> 2) * Y::SLAB + (k & 3) * 32) >> 4),
+                   id, p + k > 0);
+        tc::commit(&B->s_full[rt][st]);
+        tc::commit(&B->k_empty[st]);
+      }
+      __syncwarp();
+      return true;
+    };
+    auto issue_pv = [&](int rt, int j) {
+      const int n = j - j0, st = n & 1;
+      if (!all_wait(&B->v_full[st], (uint32_t)(n >> 1) & 1u, W_V_FULL, j)) return false;
+      if (!all_wait(&B->p_full[rt], (uint32_t)n & 1u, W_P, j)) return false;
+      if (elect_one()) {
+        const int steps = (min(kN, seen - j * kN) + 15) >> 4;
+        constexpr uint32_t id = idesc_f16(DT, true);
+        const uint32_t s0 = tmem + (uint32_t)(rt * Y::COL_RT + st * kN), d = tmem + (uint32_t)rt * Y::COL_RT + Y::COL_ACC;
+        const uint64_t dvs = dv + (uint64_t)(st * (Y::TILE >> 4));
+#pragma unroll
+        for (int k = 0; k < kN / 16; ++k) {
+          if (k >= steps) break;
+          const uint32_t a = s0 + 32 * (k >> 1) + 8 * (k & 1);  // P of 32 tokens: 16 columns, then its low part
+          mma_ts(d, a, dvs + ((k * 2048) >> 4), id, k > 0 || (!SPLIT && n > 0));
+          if constexpr (SPLIT) mma_ts(d, a + 16, dvs + ((k * 2048) >> 4), id, 1);
+        }
+        tc::commit(&B->pv_full[rt]);
+        tc::commit(&B->v_empty[st]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = true;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      bar_sync(2 + rt, 160);  // Q is in shared memory
+      tc::fence_after_sync();
+      if (j0 < j1 && ok) ok = issue_s(rt, j0);
+    }
+    for (int j = j0; j < j1 && ok; ++j) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        // the next scores go where the previous P was, once its product is formed
+        if (j + 1 < j1 && ok)
+          ok = (j == j0 || all_wait(&B->pv_full[rt], (uint32_t)(j - j0 - 1) & 1u, W_PV, j)) && issue_s(rt, j + 1);
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        if (ok) ok = issue_pv(rt, j);
+    }
+    if (!ok && elect_one()) {
+      // MMAs in flight end before TMEM is freed: an arrival of their own, waited for within limits
+      tc::commit(&B->drain);
+      mbar_wait_clocked(&B->drain, 0, nullptr);
+    }
+    __syncwarp();
   } else {
-    // ---------------- softmax, MMA issue, epilogue: one row per thread ----------------
+    // ---------------- softmax, epilogue: one row per thread ----------------
     if constexpr (SPLIT) reg_inc<Y::REGS_SOFT>();
     const int rt = warp >> 2, tr = threadIdx.x & 127;
     const int r = rt * kM + tr;  // row of the CTA
@@ -405,26 +495,34 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
     {
       const T* mine = live ? static_cast<const T*>(L.q) + (q.row0 + qi) * L.ldq + head : nullptr;
       const int p = lane % PER, e = p * V8;
-      constexpr int UN = 4;  // loads under way
+      constexpr int UN = 32 / RPI < 16 ? 32 / RPI : 16;  // loads under way
+#pragma unroll 1
       for (int i0 = 0; i0 < 32; i0 += UN * RPI) {
-        float x[UN][V8];
+        uint4 raw[UN];
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
           const int rl = i0 + u * RPI + lane / PER;
-          const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), rl & 31));
-#pragma unroll
-          for (int i = 0; i < V8; ++i) x[u][i] = 0.f;
+          const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), rl));
+          raw[u] = make_uint4(0, 0, 0, 0);
           if (src && e < c.D) {
-            if (L.vec) load_row<T, V8, true>(src + e, x[u]);
-            else load_row<T, V8, false>(src + e, x[u]);
+            if (L.vec) {
+              raw[u] = *reinterpret_cast<const uint4*>(src + e);
+            } else {
+              T y[V8];
+#pragma unroll
+              for (int i = 0; i < V8; ++i) y[i] = src[e + i];
+              memcpy(&raw[u], y, 16);
+            }
           }
         }
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
           const int row = (tr & ~31) + i0 + u * RPI + lane / PER;
+          float x[V8];
+          load_row<T, V8, true>(reinterpret_cast<const T*>(&raw[u]), x);
           float top = 0.f;
 #pragma unroll
-          for (int i = 0; i < V8; ++i) top = fmaxf(top, fabsf(x[u][i]));
+          for (int i = 0; i < V8; ++i) top = fmaxf(top, fabsf(x[i]));
 #pragma unroll
           for (int o = PER / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           const int ex = min(max((int)(__float_as_uint(top) >> 23), 27), 254) - 127;
@@ -433,7 +531,7 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
           uint32_t h[V8 / 2], lo[V8 / 2];
 #pragma unroll
           for (int i = 0; i < V8 / 2; ++i) {
-            const float y0 = x[u][2 * i] * up, y1 = x[u][2 * i + 1] * up;
+            const float y0 = x[2 * i] * up, y1 = x[2 * i + 1] * up;
             h[i] = pack2<__half>(y0, y1);
             const float2 f = unpack2<__half>(h[i]);
             lo[i] = SPLIT ? pack2<__half>(y0 - f.x, y1 - f.y) : 0u;
@@ -449,53 +547,10 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       }
       fence_proxy_async_smem();
     }
-    bar_sync(2 + rt, 128);
+    bar_sync(2 + rt, 160);  // (with the issuing warp)
     const float rs = rsm[tr];
 
     bool ok = true;
-    // By one lane of the row tile's first warp: the scores of tile j into the S buffer of its parity, and P's
-    // product with V. Each releases its operand's stage.
-    const bool issuer = (warp & 3) == 0;
-    const uint64_t dq = tc::smem_desc(base + Y::Q + rt * Y::PARTS * Y::QPART, 16, 1024, tc::kLayoutSW128);
-    const uint64_t dk = tc::smem_desc(base + Y::K, 16, 1024, tc::kLayoutSW128);
-    // V is MN-major: 64-channel slabs SLAB apart (LBO), 8-token groups 1024 B apart (SBO)
-    const uint64_t dv = tc::smem_desc(base + Y::V, Y::SLAB, 1024, tc::kLayoutSW128);
-    const uint32_t trt = tmem + (uint32_t)rt * Y::COL_RT;
-    auto issue_s = [&](int j) {
-      const int n = j - j0, st = n & 1;
-      if (!wait_for(&B->k_full[st], (uint32_t)(n >> 1) & 1u, abort, L.status, W_K_FULL, j)) return;
-      tc::fence_after_sync();
-      const uint32_t id = idesc_f16(min(kN, (seen - j * kN + 31) & ~31), false);
-      const uint32_t d = trt + (uint32_t)(st * kN);
-      const uint64_t dks = dk + (uint64_t)(st * (Y::TILE >> 4));
-#pragma unroll
-      for (int p = 0; p < Y::PARTS; ++p)
-#pragma unroll
-        for (int k = 0; k < DT / 16; ++k)
-          mma_ss(d, dq + ((p * Y::QPART + (k >> 2) * Y::QSLAB + (k & 3) * 32) >> 4), dks + (((k >> 2) * Y::SLAB + (k & 3) * 32) >> 4), id,
-                 p + k > 0);
-      tc::commit(&B->s_full[rt][st]);
-      tc::commit(&B->k_empty[st]);
-    };
-    auto issue_pv = [&](int j) {
-      const int n = j - j0, st = n & 1;
-      if (!wait_for(&B->v_full[st], (uint32_t)(n >> 1) & 1u, abort, L.status, W_V_FULL, j)) return;
-      tc::fence_after_sync();
-      const int steps = (min(kN, seen - j * kN) + 15) >> 4;
-      constexpr uint32_t id = idesc_f16(DT, true);
-      const uint32_t s0 = trt + (uint32_t)(st * kN), d = trt + Y::COL_ACC;
-      const uint64_t dvs = dv + (uint64_t)(st * (Y::TILE >> 4));
-#pragma unroll
-      for (int k = 0; k < kN / 16; ++k) {
-        if (k >= steps) break;
-        const uint32_t a = s0 + 32 * (k >> 1) + 8 * (k & 1);  // P of 32 tokens: 16 columns, then its low part
-        mma_ts(d, a, dvs + ((k * 2048) >> 4), id, k > 0 || (!SPLIT && n > 0));
-        if constexpr (SPLIT) mma_ts(d, a + 16, dvs + ((k * 2048) >> 4), id, 1);
-      }
-      tc::commit(&B->pv_full[rt]);
-      tc::commit(&B->v_empty[st]);
-    };
-
     constexpr int OR = SPLIT ? DT / 2 : 1;
     float2 o[OR];  // fp32 rows: O
 #pragma unroll
@@ -518,17 +573,11 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         }
       }
     };
-    if (j0 < j1 && issuer && elect_one()) issue_s(j0);
-    __syncwarp();
     for (int j = j0; j < j1; ++j) {
       const int n = j - j0;
       const TileMeta& mt = meta[n % kMeta];
       const int tok0 = j * kN;
-      // (a warp that gives up a wait goes on to the barrier, where all leave together)
-      if (!__all_sync(0xffffffffu, wait_for(&B->s_full[rt][n & 1], (uint32_t)(n >> 1) & 1u, abort, L.status, W_S, j))) {
-        ok = bar_and(2 + rt, 128, false);
-        break;
-      }
+      if (!(ok = __all_sync(0xffffffffu, wait_for(&B->s_full[rt][n & 1], (uint32_t)(n >> 1) & 1u, abort, L.status, W_S, j)))) break;
       tc::fence_after_sync();
       const uint32_t ts = tl + (uint32_t)((n & 1) * kN);
       constexpr int CH = Y::CHUNK;
@@ -572,11 +621,6 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
           }
         }
       }
-      // the next scores, into the buffer of the previous P once its product is formed
-      if (issuer && elect_one() && j + 1 < j1 &&
-          (n == 0 || wait_for(&B->pv_full[rt], (uint32_t)(n - 1) & 1u, abort, L.status, W_PV, j)))
-        issue_s(j + 1);
-      __syncwarp();
       const float mn = SPLIT ? fmaxf(m, mx) : mx > m + kLag || m == -INFINITY ? fmaxf(m, mx) : m;
       const bool moved = __any_sync(0xffffffffu, mn != m);
       const float ref = mn == -INFINITY ? 0.f : mn;
@@ -630,9 +674,11 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         else form(std::true_type{});
       }
       l = fmaf(l, al, sum);
+      // Every product is waited for in its turn, needed or not: a wait by parity tells a phase only from its
+      // neighbours. (This one could not start before the last one's end.)
+      if (n > 0) ok = product_done(n - 1);
       if (n > 0 && (SPLIT || moved)) {
         // fp32 rows: the previous product joins O. Either: O follows m.
-        ok = product_done(n - 1);
         if (SPLIT && ok) add_product();
         if (moved && ok) {
           if constexpr (SPLIT) {
@@ -654,22 +700,14 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       }
       tc::tmem_wait_st();
       tc::fence_before_sync();
-      if (!(ok = bar_and(2 + rt, 128, ok))) break;
-      if (issuer && elect_one()) issue_pv(j);
-      __syncwarp();
+      if (!ok) break;
+      mbar_arrive(&B->p_full[rt]);
     }
     if (ok && j0 < j1) {
       ok = product_done(j1 - j0 - 1);
       tc::fence_after_sync();
       if (SPLIT && ok) add_product();
     }
-    if (!ok && *abort && issuer && elect_one()) {
-      // MMAs in flight end before TMEM is freed: an arrival of their own, waited for within limits
-      tc::commit(&B->drain[rt]);
-      mbar_wait_clocked(&B->drain[rt], 0, nullptr);
-    }
-    __syncwarp();
-
     // ---- epilogue: the row through shared memory (its own Q rows), stored in whole 16-byte pieces ----
     // 32 channels of the row's O
     auto channels = [&](int e, float (&x)[32]) {
@@ -745,6 +783,12 @@ cudaError_t tc_as(const CacheAttnLaunch& L, const CacheAttnPlan& P, cudaStream_t
   auto kernel = cache_attn_tc_kernel<T, FMT, DT>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Y::SMEM);
   if (e != cudaSuccess) return e;
+  if constexpr (sizeof(T) == 4) {
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, kernel);
+    if (e != cudaSuccess) return e;
+    if (fa.numRegs != Y::REGS) return cudaErrorInvalidConfiguration;  // the exchange of registers would not add up
+  }
   kernel<<<(unsigned)(P.units * P.splits), Y::THREADS, Y::SMEM, s>>>(L, L.mk, L.mv, P.tiles);
   return cudaGetLastError();
 }
