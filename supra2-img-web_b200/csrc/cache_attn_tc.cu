@@ -85,7 +85,7 @@ struct TileMeta {  // of a tile's four 16-token groups
   float iv[4];   // 1 / |v_scale|
   int32_t dead;  // groups whose block does not exist (bits), tokens past the end not among them
   int32_t neg;   // groups with a negative V scale (bits), which no write makes
-  int32_t odd;   // the tile has dead or negative groups: taken score by score
+  int32_t odd;   // some group is dead, or a scale of it negative, not finite, or its K scale 0
   int32_t pad;
 };
 static_assert(sizeof(TileMeta) == 64, "META");
@@ -258,6 +258,74 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
   tc::fence_after_sync();
   const uint32_t tmem = B->tmem;
 
+  constexpr int V8 = 16 / (int)sizeof(T);  // channels of a 16-byte piece
+  constexpr int PER = DT / V8;             // pieces of a row: 8, 16 or 32
+  constexpr int RPI = 32 / PER;            // rows of a warp's load
+  // 32 rows of a row tile by one warp, PER lanes a row: q times a power of two that brings the row's largest
+  // channel into [2^13, 2^14) (and the sign of the scale), as fp16.
+  auto load_q = [&](int rt, int row0) {
+    uint8_t* Qs = base + Y::Q + rt * Y::PARTS * Y::QPART;
+    float* rsm = reinterpret_cast<float*>(base + Y::RS) + rt * kM;
+    const int my = rt * kM + row0 + lane;  // the row whose address this lane works out
+    const T* mine = nullptr;
+    if (my < nrow) {
+      const int pk = r0 + my;
+      mine = static_cast<const T*>(L.q) + (q.row0 + pk / L.G) * L.ldq + (int64_t)(hk * L.G + pk % L.G) * c.D;
+    }
+    const int p = lane % PER, e = p * V8;
+    constexpr int N = 32 / RPI, UN = N < 16 ? N : 16;  // loads, and those under way
+#pragma unroll 1
+    for (int i0 = 0; i0 < N; i0 += UN) {
+      uint4 raw[UN];
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const int rl = (i0 + u) * RPI + lane / PER;
+        const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), rl));
+        raw[u] = make_uint4(0, 0, 0, 0);
+        if (src && e < c.D) {
+          if (L.vec) {
+            raw[u] = *reinterpret_cast<const uint4*>(src + e);
+          } else {
+            T y[V8];
+#pragma unroll
+            for (int i = 0; i < V8; ++i) y[i] = src[e + i];
+            memcpy(&raw[u], y, 16);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const int row = row0 + (i0 + u) * RPI + lane / PER;
+        float x[V8];
+        load_row<T, V8, true>(reinterpret_cast<const T*>(&raw[u]), x);
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < V8; ++i) top = fmaxf(top, fabsf(x[i]));
+#pragma unroll
+        for (int o = PER / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int ex = min(max((int)(__float_as_uint(top) >> 23), 27), 254) - 127;
+        const float up = __uint_as_float(((uint32_t)(13 - ex + 127) << 23) | (L.scale_log2 < 0.f ? 0x80000000u : 0u));
+        if (p == 0) rsm[row] = fabsf(L.scale_log2) * __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
+        uint32_t h[V8 / 2], lo[V8 / 2];
+#pragma unroll
+        for (int i = 0; i < V8 / 2; ++i) {
+          const float y0 = x[2 * i] * up, y1 = x[2 * i + 1] * up;
+          h[i] = pack2<__half>(y0, y1);
+          const float2 f = unpack2<__half>(h[i]);
+          lo[i] = SPLIT ? pack2<__half>(y0 - f.x, y1 - f.y) : 0u;
+        }
+        uint8_t* at = Qs + (e >> 6) * Y::QSLAB + row * 128 + ((((e >> 3) & 7) ^ (row & 7)) << 4) + (e & 7) * 2;
+        if constexpr (V8 == 8) {
+          *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+        } else {
+          *reinterpret_cast<uint2*>(at) = make_uint2(h[0], h[1]);
+          *reinterpret_cast<uint2*>(at + Y::QPART) = make_uint2(lo[0], lo[1]);
+        }
+      }
+    }
+    fence_proxy_async_smem();
+  };
+
   if (warp >= 4 * RT && warp < 4 * RT + 3) {
     // ---------------- converters ----------------
     if constexpr (SPLIT) reg_dec<Y::REGS_REST>();
@@ -288,27 +356,24 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       page = page_at(g0 + lane);
       page_n = page_at(g0 + 32 + lane);
     }
-    // Tile j's blocks into its raw stage and its scales into meta[j % kMeta].
-    auto load = [&](int j) {
+    // Tile j's blocks into its raw stage, and its scales into meta[j % kMeta]: lanes w .. w + 3 know its groups.
+    auto copy = [&](int j) {
       if (j >= j1) return;
-      const int n = j - j0, st = n & 1, w = 4 * (n & 7);
+      const int n = j - j0, st = n & 1, a = lane - 4 * (n & 7);
       if ((n & 7) == 0 && n > 0) {
         page = page_n, ks = ks_n, vs = vs_n;
         page_n = page_at(g0 + 4 * n + 32 + lane);
         logs();
       }
       if ((n & 7) == 4) scales_at(page_n, ks_n, vs_n);
-      TileMeta& mt = meta[n % kMeta];
-      const int a = lane - w;  // lanes w .. w + 3: the tile's groups
-      const bool mine = a >= 0 && a < 4;
-      const bool live = mine && page >= 0 && page < c.blocks;
+      const bool mine = a >= 0 && a < 4, live = mine && page >= 0 && page < c.blocks;
       if (mine && !live && page != -2) report_error(L.status, DEV_BAD_BLOCK, 2, page);
       const bool first = log2t >= 6 ? a == 0 : ((16 * a) & ((1 << log2t) - 1)) == 0;  // one box per block of the tile
       const uint32_t boxes = __ballot_sync(0xffffffffu, live && first);
-      const uint32_t dead = __ballot_sync(0xffffffffu, mine && !live && page != -2) >> w;
+      const uint32_t dead = __ballot_sync(0xffffffffu, mine && !live && page != -2) >> (4 * (n & 7));
       const int box_rows = min(kN, 1 << log2t);
       if (lane == 0) {
-        mt.dead = (int32_t)(dead & 15u);  // (before the arrival: the converters read it)
+        meta[n % kMeta].dead = (int32_t)(dead & 15u);  // (before the arrival: the converters read it)
         mbar_arrive_expect_tx(&B->raw[st], (uint32_t)(__popc(boxes) * 2 * box_rows * DT));
       }
       __syncwarp();
@@ -318,25 +383,33 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         tc::tma_load_2d(to, &mk, 0, y, &B->raw[st]);
         tc::tma_load_2d(to + Y::RAWB, &mv, 0, y, &B->raw[st]);
       }
-      if (n == 0) {  // (the first scales are fetched behind the first copies)
-        scales_at(page, ks, vs);
-        logs();
-      }
+    };
+    auto describe = [&](int j) {
+      if (j >= j1) return;
+      const int n = j - j0, w = 4 * (n & 7), a = lane - w;
+      TileMeta& mt = meta[n % kMeta];
+      const bool mine = a >= 0 && a < 4, live = mine && page >= 0 && page < c.blocks;
+      const uint32_t dead = __ballot_sync(0xffffffffu, mine && !live && page != -2) >> w;
       const uint32_t neg = __ballot_sync(0xffffffffu, live && vs < 0.f) >> w;
-      const uint32_t kneg = __ballot_sync(0xffffffffu, live && ks < 0.f) >> w;
+      const uint32_t kodd = __ballot_sync(0xffffffffu, live && !(ks > 0.f && ks <= 3.4028234e38f && fabsf(vs) <= 3.4028234e38f)) >> w;
       if (mine) {
-        mt.ks[a] = ks;
+        mt.ks[a] = live ? ks : 1.f;  // (past the end: -inf times it stays -inf)
         mt.lv[a] = lv;
         mt.iv[a] = iv;
       }
       if (lane == 0) {
         mt.neg = (int32_t)(neg & 15u);
-        mt.odd = ((dead | neg | kneg) & 15u) != 0;
+        mt.odd = ((dead | neg | kodd) & 15u) != 0;
       }
     };
-    int loaded = j0;
+    int loaded = min(j0 + 2, j1);
     if (ct < 32) {
-      for (; loaded < j0 + 2; ++loaded) load(loaded);
+      copy(j0);
+      copy(j0 + 1);
+      scales_at(page, ks, vs);
+      logs();
+      describe(j0);
+      describe(j0 + 1);
     }
     constexpr int CPR = DT / 16;                                       // 16-byte pieces per row
     constexpr int PIECES = kN * CPR, NP = (PIECES + Y::CONV - 1) / Y::CONV;  // of a tile, of a thread
@@ -387,10 +460,16 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         mbar_arrive(kv ? &B->v_full[st] : &B->k_full[st]);
       }
       if (!(ok = bar_and(1, Y::CONV, ok))) break;  // every converter has left the raw stage
-      if (ct < 32 && loaded < j1) load(loaded++);
+      if (loaded < j1) {
+        if (ct < 32) {
+          copy(loaded);
+          describe(loaded);
+        }
+        ++loaded;
+      }
     }
     if (!ok && ct == 0) {  // copies in flight land before the CTA may leave
-      for (int j = j0; j < min(loaded, j1); ++j) mbar_wait_clocked(&B->raw[(j - j0) & 1], (uint32_t)((j - j0) >> 1) & 1u, nullptr);
+      for (int j = j0; j < loaded; ++j) mbar_wait_clocked(&B->raw[(j - j0) & 1], (uint32_t)((j - j0) >> 1) & 1u, nullptr);
     }
   } else if (warp == 4 * RT + 3) {
     // ---------------- MMA issue ----------------
@@ -486,69 +565,9 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
     const uint32_t tl = tmem + (uint32_t)rt * Y::COL_RT + ((uint32_t)((warp & 3) * 32) << 16);  // this warp's lanes
     uint8_t* Qs = base + Y::Q + rt * Y::PARTS * Y::QPART;
 
-    // q, times a power of two that brings its row's largest channel into [2^13, 2^14) (and the sign of the
-    // scale): PER lanes load a row together, 16 bytes each
-    constexpr int V8 = 16 / (int)sizeof(T);         // channels of a piece
-    constexpr int PER = DT / V8;                    // pieces of a row: 8, 16 or 32
-    constexpr int RPI = 32 / PER;                   // rows of a warp's load
-    float* rsm = reinterpret_cast<float*>(base + Y::RS) + rt * kM;
-    {
-      const T* mine = live ? static_cast<const T*>(L.q) + (q.row0 + qi) * L.ldq + head : nullptr;
-      const int p = lane % PER, e = p * V8;
-      constexpr int UN = 32 / RPI < 16 ? 32 / RPI : 16;  // loads under way
-#pragma unroll 1
-      for (int i0 = 0; i0 < 32; i0 += UN * RPI) {
-        uint4 raw[UN];
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-          const int rl = i0 + u * RPI + lane / PER;
-          const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), rl));
-          raw[u] = make_uint4(0, 0, 0, 0);
-          if (src && e < c.D) {
-            if (L.vec) {
-              raw[u] = *reinterpret_cast<const uint4*>(src + e);
-            } else {
-              T y[V8];
-#pragma unroll
-              for (int i = 0; i < V8; ++i) y[i] = src[e + i];
-              memcpy(&raw[u], y, 16);
-            }
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-          const int row = (tr & ~31) + i0 + u * RPI + lane / PER;
-          float x[V8];
-          load_row<T, V8, true>(reinterpret_cast<const T*>(&raw[u]), x);
-          float top = 0.f;
-#pragma unroll
-          for (int i = 0; i < V8; ++i) top = fmaxf(top, fabsf(x[i]));
-#pragma unroll
-          for (int o = PER / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const int ex = min(max((int)(__float_as_uint(top) >> 23), 27), 254) - 127;
-          const float up = __uint_as_float(((uint32_t)(13 - ex + 127) << 23) | (L.scale_log2 < 0.f ? 0x80000000u : 0u));
-          if (p == 0) rsm[row] = fabsf(L.scale_log2) * __uint_as_float((uint32_t)(ex - 13 + 127) << 23);
-          uint32_t h[V8 / 2], lo[V8 / 2];
-#pragma unroll
-          for (int i = 0; i < V8 / 2; ++i) {
-            const float y0 = x[2 * i] * up, y1 = x[2 * i + 1] * up;
-            h[i] = pack2<__half>(y0, y1);
-            const float2 f = unpack2<__half>(h[i]);
-            lo[i] = SPLIT ? pack2<__half>(y0 - f.x, y1 - f.y) : 0u;
-          }
-          uint8_t* at = Qs + (e >> 6) * Y::QSLAB + row * 128 + ((((e >> 3) & 7) ^ (row & 7)) << 4) + (e & 7) * 2;
-          if constexpr (V8 == 8) {
-            *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
-          } else {
-            *reinterpret_cast<uint2*>(at) = make_uint2(h[0], h[1]);
-            *reinterpret_cast<uint2*>(at + Y::QPART) = make_uint2(lo[0], lo[1]);
-          }
-        }
-      }
-      fence_proxy_async_smem();
-    }
+    load_q(rt, (warp & 3) * 32);
     bar_sync(2 + rt, 160);  // (with the issuing warp)
-    const float rs = rsm[tr];
+    const float rs = reinterpret_cast<const float*>(base + Y::RS)[r];
 
     bool ok = true;
     constexpr int OR = SPLIT ? DT / 2 : 1;
@@ -587,10 +606,12 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         else tc::tmem_ld32(ts + c0, s);
         tc::tmem_wait_ld();
       };
-      // The common tile, all of it seen by every row of the warp, and any other, score by score.
-      const bool plain = !mt.odd && __all_sync(0xffffffffu, lim >= tok0 + kN - 1);
+      // The common tile, all of it seen by every row of the warp; one that ends for some row, whose scores
+      // past the end become -inf; and an odd one, taken score by score.
+      const bool odd = mt.odd || L.scale_log2 == 0.f;
+      const bool edge = !odd && !__all_sync(0xffffffffu, lim >= tok0 + kN - 1);
       uint64_t vis = ~0ull;  // the columns that the row sees
-      if (!plain) {
+      if (odd) {
         const int hi = min(max(lim - tok0 + 1, 0), kN);
         vis = hi == kN ? ~0ull : (1ull << hi) - 1ull;
 #pragma unroll
@@ -602,7 +623,13 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
 #pragma unroll
       for (int c0 = 0; c0 < kN; c0 += CH) {
         load_s(c0);
-        if (plain) {
+        if (edge) {
+          const int hi = lim - tok0 - c0;
+#pragma unroll
+          for (int e = 0; e < CH; ++e)
+            if (e > hi) s[e] = -INFINITY;
+        }
+        if (!odd) {
 #pragma unroll
           for (int g = 0; g < CH / 16; ++g) {
             const float* x = s + 16 * g;
@@ -630,7 +657,15 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       float sum = 0.f;
 #pragma unroll
       for (int c0 = 0; c0 < kN; c0 += CH) {
-        if (CH < kN) load_s(c0);
+        if (CH < kN) {
+          load_s(c0);
+          if (edge) {
+            const int hi = lim - tok0 - c0;
+#pragma unroll
+            for (int e = 0; e < CH; ++e)
+              if (e > hi) s[e] = -INFINITY;
+          }
+        }
         auto form = [&](auto masked) {
 #pragma unroll
           for (int h = 0; h < CH / 32; ++h) {
@@ -670,8 +705,8 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
             if constexpr (SPLIT) tmem_st16(ts + c0 + 32 * h + 16, pl);
           }
         };
-        if (plain) form(std::false_type{});
-        else form(std::true_type{});
+        if (odd) form(std::true_type{});
+        else form(std::false_type{});
       }
       l = fmaf(l, al, sum);
       // Every product is waited for in its turn, needed or not: a wait by parity tells a phase only from its
