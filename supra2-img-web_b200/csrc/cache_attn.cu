@@ -587,8 +587,11 @@ cudaError_t attn_as(const CacheAttnLaunch& L, const CacheAttnPlan& P, cudaStream
   constexpr size_t smem = smem_of<NT, kW>(DT);
   static_assert(smem <= 227 * 1024, "shared memory");
   const int cluster = P.ws_bytes ? 1 : P.splits;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e == cudaSuccess && cluster > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = once_per_device(done, L.device, [&] {
+    const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    return r != cudaSuccess ? r : cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  });
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(P.units * P.splits));

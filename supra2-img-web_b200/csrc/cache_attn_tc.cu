@@ -816,14 +816,17 @@ template <typename T, int FMT, int DT>
 cudaError_t tc_as(const CacheAttnLaunch& L, const CacheAttnPlan& P, cudaStream_t s) {
   using Y = Cfg<DT, sizeof(T) == 4>;
   auto kernel = cache_attn_tc_kernel<T, FMT, DT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Y::SMEM);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = once_per_device(done, L.device, [&] {
+    if constexpr (sizeof(T) == 4) {
+      cudaFuncAttributes fa;
+      const cudaError_t r = cudaFuncGetAttributes(&fa, kernel);
+      if (r != cudaSuccess) return r;
+      if (fa.numRegs != Y::REGS) return cudaErrorInvalidConfiguration;  // the exchange of registers would not add up
+    }
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Y::SMEM);
+  });
   if (e != cudaSuccess) return e;
-  if constexpr (sizeof(T) == 4) {
-    cudaFuncAttributes fa;
-    e = cudaFuncGetAttributes(&fa, kernel);
-    if (e != cudaSuccess) return e;
-    if (fa.numRegs != Y::REGS) return cudaErrorInvalidConfiguration;  // the exchange of registers would not add up
-  }
   kernel<<<(unsigned)(P.units * P.splits), Y::THREADS, Y::SMEM, s>>>(L, L.mk, L.mv, P.tiles);
   return cudaGetLastError();
 }

@@ -431,16 +431,15 @@ int check_cache_attn(supra_attn_ctx* c, const supra_attn_cache_attn_desc* d, Che
   return SUPRA_ATTN_OK;
 }
 
-int flush_cache(supra_attn_ctx* c, std::vector<const Queued*>& g) {
-  for (const Queued* q : g) {
-    CacheCall& call = c->cache_calls[q->call];
+int flush_cache(supra_attn_ctx* c) {
+  for (CacheCall& call : c->cache_calls) {
     cudaError_t e = cudaSuccess;
     const char* name = "";
     switch (call.kind) {
       case CacheCall::QK_NORM: {
         name = "qk_norm";
         call.norm.status = c->d_status;
-        ProfScope ps(c, name, q->flops, q->bytes);
+        ProfScope ps(c, name, call.flops, call.bytes);
         e = launch_qk_norm(call.norm, call.type, call.vec, c->stream);
         break;
       }
@@ -449,7 +448,7 @@ int flush_cache(supra_attn_ctx* c, std::vector<const Queued*>& g) {
         const bool w = call.kind == CacheCall::WRITE;
         name = w ? "cache_write" : "cache_read";
         call.rows.status = c->d_status;
-        ProfScope ps(c, name, q->flops, q->bytes);
+        ProfScope ps(c, name, call.flops, call.bytes);
         e = (w ? launch_cache_write : launch_cache_read)(call.rows, call.type, call.format, call.vec, c->stream);
         break;
       }
@@ -465,6 +464,7 @@ int flush_cache(supra_attn_ctx* c, std::vector<const Queued*>& g) {
             !encode_byte_map(&L.mv, L.c.v, tokens, L.c.D, cols, rows, !plan.tc))
           return set_err(c, SUPRA_ATTN_ECUDA, "cuTensorMapEncodeTiled failed");
         L.splits = plan.splits;
+        L.device = c->device;
         void* ws = nullptr;
         if (plan.ws_bytes) {
           int rc = scratch_alloc(c, plan.ws_bytes, &ws);
@@ -474,7 +474,7 @@ int flush_cache(supra_attn_ctx* c, std::vector<const Queued*>& g) {
           c->launches += 1;  // the join
         }
         {
-          ProfScope ps(c, name, q->flops, q->bytes);
+          ProfScope ps(c, name, call.flops, call.bytes);
           e = launch_cache_attn(L, plan, call.type, call.format, c->stream);
         }
         if (ws) {

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 namespace supra {
 
@@ -376,7 +377,17 @@ struct CacheAttnArgs {
 // box's width, for the tensor-core kernel up to 64 without one.
 struct CacheAttnLaunch : CacheAttnArgs {
   CUtensorMap mk, mv;
+  int device;
 };
+// Runs `set` (a kernel's attributes) once for each device; a failure is tried again by the next launch.
+template <typename Set>
+cudaError_t once_per_device(std::atomic<uint64_t>& done, int device, Set set) {
+  const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  const cudaError_t e = set();
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 inline int cache_attn_box_cols(int D) { return D <= 64 ? 64 : 128; }
 inline int cache_attn_box_rows(int log2t, bool tc) { return std::min(1 << log2t, tc ? 64 : 32); }
 // How a call is split, from its sizes alone.

@@ -107,7 +107,7 @@ enum Path : int {
   PATH_TF32 = 2,
   PATH_FP32_TMA = 3,
   PATH_LINEAR = 4,
-  PATH_CACHE = 5,  // the calls of cache_ops.cpp, one launch each
+  PATH_CACHE = 5,  // the calls of cache_ops.cpp, one launch each (the context's cache_calls)
 };
 
 // A recorded qk_norm, cache_write, cache_read or cache_attention call: its launch descriptor.
@@ -115,6 +115,7 @@ struct CacheCall {
   enum Kind : int32_t { QK_NORM = 0, WRITE = 1, READ = 2, ATTENTION = 3 } kind;
   int32_t type, format;
   bool vec;
+  double flops, bytes;
   union {
     supra::QkNormLaunch norm;
     supra::CacheRowsLaunch rows;
@@ -126,7 +127,6 @@ struct Queued {
   union {
     AttnProb p;          // attention problems
     supra::LinProb lin;  // PATH_LINEAR: the linear problem
-    size_t call;         // PATH_CACHE: index in the context's cache_calls
   };
   int path;
   int cfg;
@@ -229,7 +229,7 @@ struct supra_attn_ctx {
   bool ring_ev_used[2] = {false, false};
 
   std::vector<supra::rt::Queued> queue;
-  std::vector<supra::rt::CacheCall> cache_calls;  // the recorded PATH_CACHE calls (Queued::call)
+  std::vector<supra::rt::CacheCall> cache_calls;  // the recorded PATH_CACHE calls, in order
   supra::rt::IntervalSet qreads, qwrites;
   // enqueue_batch's working storage, kept across calls
   std::vector<supra::rt::Checked> batch_checked;
@@ -361,7 +361,7 @@ struct TcJob {
 int check_qk_norm(supra_attn_ctx* c, const supra_attn_qk_norm_desc* d, Checked* out, CacheCall* call);
 int check_cache_rows(supra_attn_ctx* c, const supra_attn_cache_rows_desc* d, bool write, Checked* out, CacheCall* call);
 int check_cache_attn(supra_attn_ctx* c, const supra_attn_cache_attn_desc* d, Checked* out, CacheCall* call);
-int flush_cache(supra_attn_ctx* c, std::vector<const Queued*>& g);
+int flush_cache(supra_attn_ctx* c);
 
 int flush_fused(supra_attn_ctx* c, std::vector<const Queued*>& g);
 int flush_gemm(supra_attn_ctx* c, std::vector<const Queued*>& g);

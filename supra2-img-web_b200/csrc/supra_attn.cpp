@@ -24,10 +24,23 @@ using namespace supra::rt;
 
 namespace {
 
+void clear_queue(supra_attn_ctx* c) {
+  c->queue.clear();
+  c->cache_calls.clear();
+  c->qreads.clear();
+  c->qwrites.clear();
+}
+
 int do_flush(supra_attn_ctx* c) {
   if (c->queue.empty()) return SUPRA_ATTN_OK;
+  if (c->cache_calls.size() == c->queue.size()) {  // only calls of cache_ops.cpp: nothing to group
+    const int rc = flush_cache(c);
+    clear_queue(c);
+    return rc;
+  }
   std::map<int, std::vector<const Queued*>> groups;
   for (const Queued& q : c->queue) {
+    if (q.path == PATH_CACHE) continue;
     // (a T5 table and an expanded bias run as different kernel forms)
     const int key = q.path * 1024 + q.cfg * 8 + (q.t5_buckets ? 4 : 0) + (q.bias ? 2 : 0) + (q.aligned ? 1 : 0);
     groups[key].push_back(&q);
@@ -38,15 +51,12 @@ int do_flush(supra_attn_ctx* c) {
     rc = path == PATH_FUSED ? flush_fused(c, kv.second)
          : path == PATH_TF32 ? flush_tma(c, kv.second, true)
          : path == PATH_FP32_TMA ? flush_tma(c, kv.second, false)
-         : path == PATH_CACHE ? flush_cache(c, kv.second)
          : path == PATH_LINEAR ? (kv.second[0]->cfg ? flush_linear_tc(c, kv.second) : flush_linear(c, kv.second))
                              : flush_gemm(c, kv.second);
     if (rc) break;
   }
-  c->queue.clear();
-  c->cache_calls.clear();
-  c->qreads.clear();
-  c->qwrites.clear();
+  if (rc == SUPRA_ATTN_OK) rc = flush_cache(c);
+  clear_queue(c);
   return rc;
 }
 
@@ -109,7 +119,8 @@ int record_call(supra_attn_ctx* c, Check check) {
     DeviceGuard g(c->device);
     rc = record(c, ck);  // (may flush: the call's index is known only after it)
     if (rc) return rc;
-    c->queue.back().call = c->cache_calls.size();
+    call.flops = ck.q.flops;
+    call.bytes = ck.q.bytes;
     try {
       c->cache_calls.push_back(call);
     } catch (const std::bad_alloc&) {

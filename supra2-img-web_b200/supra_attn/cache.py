@@ -31,36 +31,43 @@ from .ops import GPU, Tensor
 
 FORMATS = {"int8": _lib.CACHE_INT8, "e4m3": _lib.CACHE_E4M3}
 _TYPES = {"fp32": _lib.T_F32, "fp16": _lib.T_F16, "bf16": _lib.T_BF16}
-_TORCH = {"torch.float32": "fp32", "torch.float16": "fp16", "torch.bfloat16": "bf16", "torch.int32": "int32",
-          "torch.uint8": "uint8", "torch.int8": "uint8", "torch.float8_e4m3fn": "uint8"}
+_kinds = {}  # torch dtype -> name, filled when the first torch tensor is seen
+
+
+def _fill_kinds():
+    import torch
+
+    _kinds.update({torch.float32: "fp32", torch.float16: "fp16", torch.bfloat16: "bf16", torch.int32: "int32",
+                   torch.uint8: "uint8", torch.int8: "uint8", torch.float8_e4m3fn: "uint8"})
 
 
 def _operand(gpu: GPU, x, name: str, dtypes):
     """(address, elements, dtype) of a Tensor or a contiguous CUDA torch tensor on the GPU's device."""
-    if isinstance(x, Tensor):
+    if x.__class__ is Tensor:
         if not x.buf:
             raise ValueError(f"{name}: tensor was released")
-        addr, n, dtype = x.buf, x.capacity, x.dtype
         if x.gpu.device != gpu.device:
             raise ValueError(f"{name}: tensor of another device")
-    elif hasattr(x, "data_ptr") and hasattr(x, "is_cuda"):
-        if not x.is_cuda or x.get_device() != gpu.device:
+        kind = x.dtype
+        if kind in dtypes:
+            return x.buf, x.capacity, kind
+    else:
+        if not hasattr(x, "data_ptr"):
+            raise TypeError(f"{name}: unsupported operand type {type(x).__name__}")
+        if not _kinds:
+            _fill_kinds()
+        if x.get_device() != gpu.device:  # (-1: not on a GPU)
             raise ValueError(f"{name}: torch tensors must live on cuda:{gpu.device}")
         if not x.is_contiguous():
             raise ValueError(f"{name}: torch tensors must be contiguous")
-        addr, n, dtype = x.data_ptr(), x.numel(), _TORCH.get(str(x.dtype))
-    else:
-        raise TypeError(f"{name}: unsupported operand type {type(x).__name__}")
-    if dtype not in dtypes:
-        raise ValueError(f"{name}: must be {' or '.join(dtypes)}, not {getattr(x, 'dtype', dtype)}")
-    return addr, n, dtype
+        kind = _kinds.get(x.dtype)
+        if kind in dtypes:
+            return x.data_ptr(), x.numel(), kind
+    raise ValueError(f"{name}: must be {' or '.join(dtypes)}, not {x.dtype}")
 
 
 _FLOATS = ("fp32", "fp16", "bf16")
-
-
-def _shape(x):
-    return [int(s) for s in x.shape]
+_INTS, _CODES, _F32 = ("int32",), ("uint8",), ("fp32",)
 
 
 class KVCache:
@@ -75,13 +82,13 @@ class KVCache:
                  v=None, k_scale=None, v_scale=None):
         if format not in FORMATS:
             raise ValueError(f"format must be one of {sorted(FORMATS)}")
-        own = [x is None for x in (k, v, k_scale, v_scale)]
-        if any(own) and not all(own):
+        given = (k is not None) + (v is not None) + (k_scale is not None) + (v_scale is not None)
+        if given not in (0, 4):
             raise ValueError("pass all of k, v, k_scale and v_scale, or none")
         self.gpu, self.format = gpu, format
         self.blocks, self.block_tokens, self.H, self.D = int(blocks), int(block_tokens), int(H), int(D)
         self._owned = []
-        if own[0]:
+        if not given:
             if min(self.blocks, self.block_tokens, self.H, self.D) < 1:
                 raise ValueError("blocks, block_tokens, H and D must be positive")
             shape = [self.blocks, self.H, self.block_tokens, self.D]
@@ -94,10 +101,10 @@ class KVCache:
             k, v, k_scale, v_scale = self._owned
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         d = Cache()
-        d.k, d.k_size, _ = _operand(gpu, k, "k", ("uint8",))
-        d.v, d.v_size, _ = _operand(gpu, v, "v", ("uint8",))
-        d.k_scale, d.k_scale_size, _ = _operand(gpu, k_scale, "k_scale", ("fp32",))
-        d.v_scale, d.v_scale_size, _ = _operand(gpu, v_scale, "v_scale", ("fp32",))
+        d.k, d.k_size, _ = _operand(gpu, k, "k", _CODES)
+        d.v, d.v_size, _ = _operand(gpu, v, "v", _CODES)
+        d.k_scale, d.k_scale_size, _ = _operand(gpu, k_scale, "k_scale", _F32)
+        d.v_scale, d.v_scale_size, _ = _operand(gpu, v_scale, "v_scale", _F32)
         d.blocks, d.block_tokens, d.H, d.D, d.format = self.blocks, self.block_tokens, self.H, self.D, FORMATS[format]
         self._desc = d
 
@@ -130,13 +137,14 @@ class CacheBatch:
     def __init__(self, gpu: GPU, lengths, table, *, max_rows: int = 1, row_start=None, rows: int | None = None,
                  max_len: int | None = None):
         s = CacheSeqs()
-        s.lengths, s.lengths_size, _ = _operand(gpu, lengths, "lengths", ("int32",))
-        s.table, s.table_size, _ = _operand(gpu, table, "table", ("int32",))
-        if len(lengths.shape) != 1 or len(table.shape) != 2 or _shape(table)[0] != _shape(lengths)[0]:
+        s.lengths, s.lengths_size, _ = _operand(gpu, lengths, "lengths", _INTS)
+        s.table, s.table_size, _ = _operand(gpu, table, "table", _INTS)
+        shape = tuple(table.shape)
+        if len(shape) != 2 or tuple(lengths.shape) != shape[:1]:
             raise ValueError("lengths must be [B] and table [B, blocks]")
-        s.B, s.ld_table = _shape(table)
+        s.B, s.ld_table = shape
         if row_start is not None:
-            s.row_start, s.row_start_size, _ = _operand(gpu, row_start, "row_start", ("int32",))
+            s.row_start, s.row_start_size, _ = _operand(gpu, row_start, "row_start", _INTS)
             if rows is None:
                 raise ValueError("row_start needs rows, an upper bound of its last entry")
             s.rows = int(rows)
@@ -152,18 +160,19 @@ class CacheBatch:
         self.gpu, self._seqs, self._keep = gpu, s, (lengths, table, row_start)
         self.rows = s.rows
 
-    def _fill(self, gpu: GPU, cache: KVCache, to: CacheSeqs):
+    def _fill(self, gpu: GPU, cache: KVCache, to):
+        """Copies the cache and the sequences into a descriptor."""
         if gpu.device != self.gpu.device:
             raise ValueError("batch of another device")
-        C.memmove(C.byref(to), C.byref(self._seqs), C.sizeof(CacheSeqs))
-        if to.max_len < 0:
-            to.max_len = min(to.ld_table * cache.block_tokens, 1 << 30)
+        to.cache = cache._struct(gpu)
+        to.seqs = self._seqs
+        if self._seqs.max_len < 0:
+            to.seqs.max_len = min(self._seqs.ld_table * cache.block_tokens, 1 << 30)
 
 
 def _rows_desc(gpu: GPU, cache: KVCache, seqs: CacheBatch, k, v, ldk, ldv, kOff, vOff) -> CacheRowsDesc:
     d = CacheRowsDesc()
-    C.memmove(C.byref(d.cache), C.byref(cache._struct(gpu)), C.sizeof(Cache))
-    seqs._fill(gpu, cache, d.seqs)
+    seqs._fill(gpu, cache, d)
     d.k, d.k_size, kt = _operand(gpu, k, "k", _FLOATS)
     d.v, d.v_size, vt = _operand(gpu, v, "v", _FLOATS)
     if kt != vt:
@@ -176,13 +185,6 @@ def _rows_desc(gpu: GPU, cache: KVCache, seqs: CacheBatch, k, v, ldk, ldv, kOff,
     return d
 
 
-def _hold(gpu: GPU, *operands):
-    if gpu.pending():
-        gpu._held.append(operands)
-    else:  # (nothing was recorded: an empty call)
-        gpu._held.clear()
-
-
 def cache_write(gpu: GPU, cache: KVCache, seqs: CacheBatch, *, k, v, ldk=None, ldv=None, kOff=0, vOff=0):
     """Quantises K/V rows into the cache: the rows of `seqs` are the last tokens of their sequences.
 
@@ -193,7 +195,7 @@ def cache_write(gpu: GPU, cache: KVCache, seqs: CacheBatch, *, k, v, ldk=None, l
     """
     d = _rows_desc(gpu, cache, seqs, k, v, ldk, ldv, kOff, vOff)
     check(lib.supra_attn_enqueue_cache_write(gpu.ctx, C.byref(d)), gpu.ctx)
-    _hold(gpu, cache, seqs, k, v)
+    gpu._held.append((cache, seqs, k, v))
 
 
 def cache_read(gpu: GPU, cache: KVCache, seqs: CacheBatch, *, k, v, ldk=None, ldv=None, kOff=0, vOff=0):
@@ -201,7 +203,7 @@ def cache_read(gpu: GPU, cache: KVCache, seqs: CacheBatch, *, k, v, ldk=None, ld
     of `seqs` are the last tokens of their sequences. Rows after the last sequence's stay as they are."""
     d = _rows_desc(gpu, cache, seqs, k, v, ldk, ldv, kOff, vOff)
     check(lib.supra_attn_enqueue_cache_read(gpu.ctx, C.byref(d)), gpu.ctx)
-    _hold(gpu, cache, seqs, k, v)
+    gpu._held.append((cache, seqs, k, v))
 
 
 def cache_attention(gpu: GPU, cache: KVCache, seqs: CacheBatch, *, q, H: int, out=None, scale=None, causal: bool = False,
@@ -220,8 +222,7 @@ def cache_attention(gpu: GPU, cache: KVCache, seqs: CacheBatch, *, q, H: int, ou
         out = gpu.empty([seqs.rows, int(H) * cache.D], qt)
     try:
         d = CacheAttnDesc()
-        C.memmove(C.byref(d.cache), C.byref(cache._struct(gpu)), C.sizeof(Cache))
-        seqs._fill(gpu, cache, d.seqs)
+        seqs._fill(gpu, cache, d)
         d.q, d.q_size = qa, qn
         d.out, d.out_size, ot = _operand(gpu, out, "out", _FLOATS)
         if ot != qt:
@@ -241,7 +242,7 @@ def cache_attention(gpu: GPU, cache: KVCache, seqs: CacheBatch, *, q, H: int, ou
         if own:
             out.release()
         raise
-    _hold(gpu, cache, seqs, q, out)
+    gpu._held.append((cache, seqs, q, out))
     return out
 
 
@@ -282,20 +283,20 @@ def qk_norm(gpu: GPU, *, q, M: int, Hq: int, D: int, k=None, Hk: int = 0, qOut=N
             o.ldy = o.H * int(D) if ldo is None else int(ldo)
             o.y_off = int(oo)
         if w is not None:
-            o.w, o.w_size, _ = _operand(gpu, w, "w" + name, ("fp32",))
+            o.w, o.w_size, _ = _operand(gpu, w, "w" + name, _F32)
         hold += [x, out, w]
     if len(kinds) != 1:
         raise ValueError("q, k and their outputs must have the same type")
     d.type = _TYPES[kinds.pop()]
     d.M, d.D, d.rot, d.eps = int(M), int(D), int(rot), float(eps)
     if turns is not None:
-        d.turns, d.turns_size, _ = _operand(gpu, turns, "turns", ("fp32",))
+        d.turns, d.turns_size, _ = _operand(gpu, turns, "turns", _F32)
         d.n_turns = min(d.turns_size // max(1, d.rot), (1 << 31) - 1)
     if positions is not None:
-        d.positions, d.positions_size, _ = _operand(gpu, positions, "positions", ("int32",))
+        d.positions, d.positions_size, _ = _operand(gpu, positions, "positions", _INTS)
     d.flags = (0 if norm else _lib.QK_NO_NORM) | (_lib.QK_INTERLEAVED if interleaved else 0)
     check(lib.supra_attn_enqueue_qk_norm(gpu.ctx, C.byref(d)), gpu.ctx)
-    _hold(gpu, hold, turns, positions)
+    gpu._held.append((hold, turns, positions))
 
 
 def rotation_turns(gpu: GPU, positions, rot: int, base: float = 10000.0) -> Tensor:
