@@ -162,6 +162,69 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
   mbar_fence_init();
   __syncwarp();
 
+  // ---- this warp's tiles ----
+  const int nt = (seen + kTile - 1) / kTile;
+  const int parts = csize * W, part = crank * W + warp;
+  const int share = nt / parts, extra = nt % parts;
+  const int t0 = part * share + min(part, extra);
+  const int cnt = share + (part < extra ? 1 : 0);
+
+  // Blocks of the next 16-token groups, one group per lane: the set in use, and the next one, whose
+  // loads are under way while the first is used up.
+  const int log2t = c.log2t;
+  auto page_at = [&](int grp) {  // grp: 16-token group of the sequence
+    return grp * 16 < seen ? L.s.table[(int64_t)b * L.s.ld_table + ((grp * 16) >> log2t)] : -2;
+  };
+  auto scales_at = [&](int p, float& ks, float& vs) {
+    ks = vs = 0.f;
+    if (p >= 0 && p < c.blocks) {
+      const int64_t u = (int64_t)p * c.H + hk;
+      ks = c.ks[u];
+      vs = c.vs[u];
+    }
+  };
+  int page = page_at(2 * t0 + lane), page_n = page_at(2 * t0 + 32 + lane);
+  float ks, vs, ks_n = 0.f, vs_n = 0.f;
+  // The warp's tile i into its stage: the lanes that know its groups load them (both by one, when they are
+  // in one block), and describe them; a block outside the cache is not loaded.
+  auto copy = [&](int i) {
+    if (i >= cnt) return;
+    const int w = i & 15, st = i % kStages;
+    if (w == 0 && i > 0) {
+      page = page_n, ks = ks_n, vs = vs_n;
+      page_n = page_at(2 * (t0 + i) + 32 + lane);
+    }
+    if (w == 8) scales_at(page_n, ks_n, vs_n);
+    const int a = lane - 2 * w;
+    const bool mine = a == 0 || a == 1;
+    const bool dead = page < 0 || page >= c.blocks;
+    const uint32_t live = __ballot_sync(0xffffffffu, (ONE ? a == 0 : mine) && !dead);
+    constexpr int box = ONE ? kTile : 16;
+    if (lane == 0) mbar_arrive_expect_tx(full + st, (uint32_t)(__popc(live) * 2 * box * DT));
+    __syncwarp();
+    if (live >> lane & 1) {
+      const int tok = (t0 + i) * kTile + 16 * a;
+      const int y = ((page * c.H + hk) << log2t) + (tok & ((1 << log2t) - 1));
+      uint8_t* to = ring + st * sbytes + 16 * a * DT;
+      tc::tma_load_2d(to, &mk, 0, y, full + st);
+      tc::tma_load_2d(to + tile_bytes, &mv, 0, y, full + st);
+    }
+  };
+  auto describe = [&](int i) {
+    if (i >= cnt) return;
+    const int a = lane - 2 * (i & 15);
+    if (a == 0 || a == 1) {
+      const bool dead = page < 0 || page >= c.blocks;
+      Group* gr = groups + (i % kStages) * 2 + a;
+      gr->ks = ks, gr->vs = vs, gr->dead = dead;
+      if (dead && page != -2) report_error(L.status, DEV_BAD_BLOCK, 1, page);
+    }
+  };
+  // the first copies go out before q and the scales are fetched
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) copy(i);
+  scales_at(page, ks, vs);
+
   // ---- q fragments: lane (g, t) holds channels 16 k + 4 t .. + 3 of row g of each row group, paired
   // as codes4_any pairs K's ----
   constexpr int P1 = FMT == kCacheInt8 ? 2 : 1;  // the channel beside the first
@@ -209,6 +272,9 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
     }
   }
 
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) describe(i);
+
   float o[CH][NT][4];
   float m[NT][2], l[NT][2];
 #pragma unroll
@@ -222,66 +288,6 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[k][n][e] = 0.f;
 
-  // ---- this warp's tiles ----
-  const int nt = (seen + kTile - 1) / kTile;
-  const int parts = csize * W, part = crank * W + warp;
-  const int share = nt / parts, extra = nt % parts;
-  const int t0 = part * share + min(part, extra);
-  const int cnt = share + (part < extra ? 1 : 0);
-
-  // Blocks of the next 16-token groups, one group per lane: the set in use, and the next one, whose
-  // loads are under way while the first is used up.
-  const int log2t = c.log2t;
-  auto page_at = [&](int grp) {  // grp: 16-token group of the sequence
-    const int j = (grp * 16) >> log2t;
-    if (grp * 16 >= seen) return -2;
-    const int32_t p = L.s.table[(int64_t)b * L.s.ld_table + j];
-    return p;
-  };
-  auto scales_at = [&](int p, float& ks, float& vs) {
-    ks = vs = 0.f;
-    if (p >= 0 && p < c.blocks) {
-      const int64_t u = (int64_t)p * c.H + hk;
-      ks = c.ks[u];
-      vs = c.vs[u];
-    }
-  };
-  int page = page_at(2 * t0 + lane), page_n = page_at(2 * t0 + 32 + lane);
-  float ks, vs, ks_n = 0.f, vs_n = 0.f;
-  scales_at(page, ks, vs);
-  auto issue = [&](int i) {  // loads the warp's tile i into its stage
-    if (i >= cnt) return;
-    const int w = i & 15, st = i % kStages;
-    if (w == 0 && i > 0) {
-      page = page_n, ks = ks_n, vs = vs_n;
-      page_n = page_at(2 * (t0 + i) + 32 + lane);
-    }
-    if (w == 8) scales_at(page_n, ks_n, vs_n);
-    // the lanes that know the tile's groups describe them and load them (both by one, when they are
-    // in one block); a block outside the cache is not loaded
-    const int a = lane - 2 * w;
-    const bool mine = a == 0 || a == 1;
-    const bool dead = page < 0 || page >= c.blocks;
-    if (mine) {
-      Group* gr = groups + st * 2 + a;
-      gr->ks = ks, gr->vs = vs, gr->dead = dead;
-      if (dead && page != -2) report_error(L.status, DEV_BAD_BLOCK, 1, page);
-    }
-    const uint32_t live = __ballot_sync(0xffffffffu, (ONE ? a == 0 : mine) && !dead);
-    constexpr int box = ONE ? kTile : 16;
-    if (lane == 0) mbar_arrive_expect_tx(full + st, (uint32_t)(__popc(live) * 2 * box * DT));
-    __syncwarp();
-    if (live >> lane & 1) {
-      const int tok = (t0 + i) * kTile + 16 * a;
-      const int y = ((page * c.H + hk) << log2t) + (tok & ((1 << log2t) - 1));
-      uint8_t* to = ring + st * sbytes + 16 * a * DT;
-      tc::tma_load_2d(to, &mk, 0, y, full + st);
-      tc::tma_load_2d(to + tile_bytes, &mv, 0, y, full + st);
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) issue(i);
-
   bool lost = false;
   int lost_at = 0;
   for (int i = 0; i < cnt; ++i) {
@@ -292,7 +298,8 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
       break;
     }
     __syncwarp();
-    issue(i + kStages - 1);  // into the stage that the previous tile has left
+    copy(i + kStages - 1);  // into the stage that the previous tile has left
+    describe(i + kStages - 1);
     const Group* gr = groups + stg * 2;
     const uint32_t kb = smem_u32(ring + stg * sbytes) + chunk0_at<DT>(lane), vb = kb + (uint32_t)tile_bytes;
     const int tok0 = (t0 + i) * kTile;
@@ -639,9 +646,14 @@ CacheAttnPlan plan_cache_attn(const CacheAttnArgs& L) {
     // fewer units than run at once, each with many tiles of tokens: split them
     if (wide >= 2) P.splits = (int)wide;
   } else {
-    // CTAs of a cluster that split one unit: enough to fill the SMs several times over, each left with
-    // at least 256 tokens of the longest sequence
-    while (P.splits < 16 && P.units * P.splits < 148 * 8 && L.s.max_len >= P.splits * 2 * 256) P.splits *= 2;
+    // CTAs of a cluster that split one unit: about a wave of four CTAs per SM, as long as each is left with
+    // 128 tokens of the longest sequence, and up to two waves, for sequences of unlike length to even
+    // out, while each is left with 1024
+    while (P.splits < 16) {
+      const int64_t ctas = P.units * P.splits * 2, tokens = L.s.max_len / (P.splits * 2);
+      if (!(ctas <= 148 * 4 && tokens >= 128) && !(ctas <= 148 * 16 && tokens >= 1024)) break;
+      P.splits *= 2;
+    }
     // Without clusters: one wave of three CTAs per SM, each left with 512 tokens. Worth the second
     // launch where it is well over 16 CTAs a unit.
     if (wide >= 20) P.splits = (int)wide;
