@@ -3,12 +3,14 @@
 // Write: per block and head, with x over the block's written tokens,
 //   s = max(amax|x|, 2^-100) * (1/qmax), at least the old scale when the block holds earlier tokens
 //   code = nearest(x * (1/s)); the held codes become nearest(code * (old / s)) when the scale grew.
-// One CTA per (block, head, K or V): the block's rows are read once into registers, the maximum is
-// reduced over the CTA, and the codes leave as 16-byte stores into the block's contiguous
-// block_tokens * D bytes. Nothing is read twice and one launch does it all, so the kernel is bound by
-// the rows' bytes in and the codes out; a block is the unit because its scale is.
+// One CTA per (block, head, K or V): the block's rows are read once into registers, 16 bytes a load and
+// neighbouring lanes on neighbouring pieces, the maximum is reduced over the CTA, and the codes leave
+// into the block's contiguous block_tokens * D bytes. Nothing is read twice and one launch does it all,
+// so the kernel is bound by the rows' bytes in and the codes out; a block is the unit because its scale is.
 // Read: value = code * scale in fp32, rounded once to the output type; one CTA per block of tokens
-// and K or V, its threads in the order of the output rows.
+// and K or V, a row per warp at a time, each lane storing 16 bytes.
+#include <algorithm>
+
 #include "cache.cuh"
 
 namespace supra {
@@ -16,10 +18,38 @@ namespace {
 
 __device__ __forceinline__ uint32_t warp_max(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
 
-// NV 16-element pieces per thread, T * D / 16 <= NV * blockDim.x.
+// The codes of V channels (4 or 8), as one or two words.
+template <int FMT, int V>
+__device__ __forceinline__ void encode_row(const float (&x)[V], uint32_t (&u)[V / 4]) {
+#pragma unroll
+  for (int k = 0; k < V / 4; ++k) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = x[4 * k + e];
+    u[k] = encode4<FMT>(y);
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_codes(const uint8_t* p, uint32_t (&u)[N]) {
+  if constexpr (N == 1) {
+    u[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    u[0] = w.x, u[1] = w.y;
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t (&u)[N]) {
+  if constexpr (N == 1) *reinterpret_cast<uint32_t*>(p) = u[0];
+  else *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+}
+
+// Threads take pieces of 16 bytes of a row (V channels): thread t < rows * per_row has piece t % per_row of slots
+// t / per_row + i * rows, i < NV.
 template <typename T, int FMT, int NV, bool VEC>
-__global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant__ CacheRowsLaunch L, int nblk) {
-  __shared__ uint32_t part[8];
+__global__ void __launch_bounds__(512) cache_write_kernel(const __grid_constant__ CacheRowsLaunch L, int nblk, int rows) {
+  constexpr int V = 16 / (int)sizeof(T);
+  __shared__ uint32_t part[16];
   const CachePool& c = L.c;
   const int b = blockIdx.x / nblk, h = blockIdx.y;
   SeqView q;
@@ -34,25 +64,28 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant_
   if (page < 0) return;
   const bool is_v = blockIdx.z != 0;
   const int64_t unit = (int64_t)page * c.H + h;
-  uint8_t* codes = (is_v ? c.v : c.k) + (unit << c.log2t) * c.D;
+  const int per_row = c.D / V;
+  const int slot0 = threadIdx.x / per_row, e = (threadIdx.x - slot0 * per_row) * V;
+  const int end = slot0 < rows ? hi : 0;  // threads past the last whole row of pieces have nothing
+  uint8_t* codes = (is_v ? c.v : c.k) + (unit << c.log2t) * c.D + e;
   float* scale = (is_v ? c.vs : c.ks) + unit;
   const int64_t ld = is_v ? L.ldv : L.ldk;
-  const T* rows = static_cast<const T*>(is_v ? L.v : L.k) + (q.row0 + t0 - first) * ld + (int64_t)h * c.D;
-  const int per_row = c.D >> 4;
+  const T* src = static_cast<const T*>(is_v ? L.v : L.k) + (q.row0 + t0 - first) * ld + (int64_t)h * c.D + e;
   const float old = lo > 0 ? *scale : 0.f;
 
-  float x[NV][16];
+  float x[NV][V];
   uint32_t top = 0;  // |x| as its bits: NaN above infinity above every number
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
-    const int slot = v / per_row;
-    if (slot >= lo && slot < hi) {
-      load_row<T, 16, VEC>(rows + slot * ld + (v - slot * per_row) * 16, x[i]);
+    const int slot = slot0 + i * rows;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) top = max(top, __float_as_uint(x[i][k]) & 0x7fffffffu);
-    }
+    for (int k = 0; k < V; ++k) x[i][k] = 0.f;
+    if (slot >= lo && slot < end) load_row<T, V, VEC>(src + slot * ld, x[i]);
   }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < V; ++k) top = max(top, __float_as_uint(x[i][k]) & 0x7fffffffu);
   top = warp_max(top);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
   __syncthreads();  // (also: every thread has read the old scale)
@@ -67,31 +100,24 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant_
   const float ratio = again ? old / s : 1.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
-    const int slot = v / per_row;
-    uint4* at = reinterpret_cast<uint4*>(codes) + v;
-    if (slot >= lo && slot < hi) {
-      uint32_t u[4];
+    const int slot = slot0 + i * rows;
+    if (slot >= end) break;
+    uint8_t* at = codes + slot * c.D;
+    uint32_t u[V / 4];
+    if (slot >= lo) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float y[4];
+      for (int k = 0; k < V; ++k) x[i][k] = bad ? 0.f : mul_odd(x[i][k], inv);
+      encode_row<FMT, V>(x[i], u);
+      store_codes(at, u);
+    } else if (again) {
+      load_codes(at, u);
+      float y[V];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = bad ? 0.f : mul_odd(x[i][4 * k + e], inv);
-        u[k] = encode4<FMT>(y);
-      }
-      *at = make_uint4(u[0], u[1], u[2], u[3]);
-    } else if (again && slot < lo) {
-      const uint4 w = *at;
-      uint32_t u[4] = {w.x, w.y, w.z, w.w};
+      for (int k = 0; k < V / 4; ++k) decode4<FMT>(u[k], y + 4 * k);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float y[4];
-        decode4<FMT>(u[k], y);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = mul_odd(y[e], ratio);
-        u[k] = encode4<FMT>(y);
-      }
-      *at = make_uint4(u[0], u[1], u[2], u[3]);
+      for (int k = 0; k < V; ++k) y[k] = mul_odd(y[k], ratio);
+      encode_row<FMT, V>(y, u);
+      store_codes(at, u);
     }
   }
   if (threadIdx.x == 0) *scale = s;
@@ -99,6 +125,8 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant_
 
 template <typename T, int FMT, bool VEC>
 __global__ void __launch_bounds__(256) cache_read_kernel(const __grid_constant__ CacheRowsLaunch L, int nblk) {
+  constexpr int V = 16 / (int)sizeof(T);
+  constexpr int UN = 4;  // pieces of a row that a lane has under way
   const CachePool& c = L.c;
   const int b = blockIdx.x / nblk;
   SeqView q;
@@ -116,21 +144,35 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const __grid_constant__
   const uint8_t* codes = (is_v ? c.v : c.k) + (unit << c.log2t) * c.D;
   const float* scale = (is_v ? c.vs : c.ks) + unit;
   const int64_t ld = is_v ? L.ldv : L.ldk;
-  T* rows = static_cast<T*>(is_v ? L.v : L.k) + (q.row0 + t0 - first) * ld;
-  const int per_head = c.D >> 4, per_row = c.H * per_head;
-  const int total = (hi - lo) * per_row;
-  for (int i = threadIdx.x; i < total; i += blockDim.x) {
-    const int slot = lo + i / per_row, p = i % per_row;
-    const int h = p / per_head, e = (p - h * per_head) * 16;
-    const uint4 w = *reinterpret_cast<const uint4*>(codes + (((int64_t)h << c.log2t) + slot) * c.D + e);
-    const float s = scale[h];
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    float x[16];
+  T* dst = static_cast<T*>(is_v ? L.v : L.k) + (q.row0 + t0 - first) * ld;
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_head = c.D / V, per_row = c.H * per_head;
+  const int head_bytes = c.D << c.log2t;
+  // a lane's pieces are the same in every row: their heads are worked out once per UN of them
+  for (int p0 = lane; p0 < per_row; p0 += 32 * UN) {
+    const uint8_t* from[UN];
+    float s[UN];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) decode4<FMT>(u[k], x + 4 * k);
+    for (int i = 0; i < UN; ++i) {
+      const int p = min(p0 + 32 * i, per_row - 1), h = p / per_head;
+      from[i] = codes + (int64_t)h * head_bytes + (p - h * per_head) * V;
+      s[i] = scale[h];
+    }
+    for (int slot = lo + warp; slot < hi; slot += warps) {
+      uint32_t u[UN][V / 4];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) x[k] *= s;
-    store_row<T, 16, VEC>(rows + slot * ld + (int64_t)p * 16, x);
+      for (int i = 0; i < UN; ++i) load_codes(from[i] + slot * c.D, u[i]);
+#pragma unroll
+      for (int i = 0; i < UN; ++i) {
+        if (p0 + 32 * i >= per_row) break;
+        float x[V];
+#pragma unroll
+        for (int k = 0; k < V / 4; ++k) decode4<FMT>(u[i][k], x + 4 * k);
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[k] *= s[i];
+        store_row<T, V, VEC>(dst + slot * ld + (int64_t)(p0 + 32 * i) * V, x);
+      }
+    }
   }
 }
 
@@ -140,15 +182,19 @@ int touched(const CacheSeqs& s, int log2t) { return (int)((s.max_rows + 2ll * (1
 template <typename T, int FMT, bool VEC>
 cudaError_t write_as(const CacheRowsLaunch& L, cudaStream_t s) {
   const int nblk = touched(L.s, L.c.log2t);
-  const int pieces = (L.c.D >> 4) << L.c.log2t;
+  // As many threads as there are pieces, up to 256 (512 where a thread would hold more than 32 channels):
+  // whole rows of pieces, the last warp filled up.
+  constexpr int V = 16 / (int)sizeof(T), MOST = 32 / V;
+  const int per_row = L.c.D / V, tokens = 1 << L.c.log2t;
+  int rows = std::min(tokens, 256 / per_row);
+  if ((tokens + rows - 1) / rows > MOST) rows = std::min(tokens, 512 / per_row);
+  const int nv = (tokens + rows - 1) / rows;
+  const int threads = (rows * per_row + 31) / 32 * 32;
   const dim3 grid((unsigned)(L.s.B * nblk), (unsigned)L.c.H, 2);
-  if (pieces <= 256) {
-    cache_write_kernel<T, FMT, 1, VEC><<<grid, (pieces + 31) / 32 * 32, 0, s>>>(L, nblk);
-  } else if (pieces <= 512) {
-    cache_write_kernel<T, FMT, 2, VEC><<<grid, 256, 0, s>>>(L, nblk);
-  } else {
-    cache_write_kernel<T, FMT, 4, VEC><<<grid, 256, 0, s>>>(L, nblk);
-  }
+  if (nv <= 1) cache_write_kernel<T, FMT, 1, VEC><<<grid, threads, 0, s>>>(L, nblk, rows);
+  else if (nv <= 2) cache_write_kernel<T, FMT, 2, VEC><<<grid, threads, 0, s>>>(L, nblk, rows);
+  else if (nv <= 4) cache_write_kernel<T, FMT, 4, VEC><<<grid, threads, 0, s>>>(L, nblk, rows);
+  else cache_write_kernel<T, FMT, 8, VEC><<<grid, threads, 0, s>>>(L, nblk, rows);  // (fp32; 8 is the most)
   return cudaGetLastError();
 }
 template <typename T, int FMT, bool VEC>

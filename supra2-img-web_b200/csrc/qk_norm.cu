@@ -3,29 +3,13 @@
 // Bound by the rows' bytes in and out. The vector form gives a head to a group of lanes, each with
 // one 16-byte piece: the sum of squares and the partner channels of the rotation go by shuffles, so
 // every element is read once, and a warp walks over the heads of one row with the row's turns and the
-// weights held in registers. Every lane stores only pieces that it loaded itself, so in-place calls
+// weights held in registers (1 / sqrt is rsqrtf, 2 ulp; a correctly rounded root and division a head
+// made the kernel issue-bound). Every lane stores only pieces that it loaded itself, so in-place calls
 // need no ordering. The scalar form (odd sizes and alignments) gives a head to a warp.
 #include "cache.cuh"
 
 namespace supra {
 namespace {
-
-template <typename T>
-struct Head {
-  const T* x;
-  T* y;
-  bool key;
-};
-template <typename T>
-__device__ __forceinline__ Head<T> head_of(const QkNormLaunch& L, int64_t row, int h) {
-  Head<T> r;
-  r.key = h >= L.q.H;
-  const QkOperand& o = r.key ? L.k : L.q;
-  const int64_t at = (int64_t)(r.key ? h - L.q.H : h) * L.D;
-  r.x = static_cast<const T*>(o.x) + row * o.ldx + at;
-  r.y = static_cast<T*>(o.y) + row * o.ldy + at;
-  return r;
-}
 
 // The row of the turns table for `row`, or null (reported) when its position is outside.
 __device__ __forceinline__ const float* turns_of(const QkNormLaunch& L, int64_t row, int lane, bool* ok) {
@@ -40,14 +24,15 @@ __device__ __forceinline__ const float* turns_of(const QkNormLaunch& L, int64_t 
   return L.turns + p * L.rot;
 }
 
-// LPH lanes per head (a power of two), V elements per lane; `wpr` warps share a row's heads.
-template <typename T, int LPH>
+// LPH lanes per head (a power of two), V elements per lane; `wpr` warps share a row's heads. ROT: 0 no
+// rotation, 1 pairs half a rotation apart, 2 neighbours.
+template <typename T, int LPH, int ROT>
 __global__ void __launch_bounds__(256) qk_norm_vec(const __grid_constant__ QkNormLaunch L, int wpr) {
   constexpr int V = 16 / (int)sizeof(T);
   constexpr int UNROLL = 4;
   const int lane = threadIdx.x & 31, g = lane / LPH, l = lane % LPH;
-  const int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int64_t row = w / wpr;
+  const uint32_t w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int row = (int)(w / (uint32_t)wpr), part = (int)(w - (uint32_t)row * wpr);
   if (row >= L.M) return;
   bool ok;
   const float* turns = turns_of(L, row, lane, &ok);
@@ -55,59 +40,83 @@ __global__ void __launch_bounds__(256) qk_norm_vec(const __grid_constant__ QkNor
   const int e0 = l * V;                 // the lane's first channel
   const bool on = e0 < L.D;             // lanes past the head only take part in the shuffles
   const int half = L.rot >> 1;
-  const bool turn = on && e0 < L.rot;
-  // Interleaved: the lane's own pairs. Else the partner piece is half a rotation away, in the
-  // lane `away` from this one, and this lane's results are n cos -+ partner sin.
-  const bool second = !L.interleaved && e0 >= half;
-  const int peer = L.interleaved ? lane : g * LPH + (turn ? (second ? e0 - half : e0 + half) / V : l);
-  float co[V], si[V], wq[V], wk[V];
+  const bool turn = ROT != 0 && on && e0 < L.rot;
+  // Pairs half a rotation apart: the partner piece is in the lane `peer`, and this lane's results are
+  // n cos -+ partner sin.
+  const bool second = ROT == 1 && e0 >= half;
+  const int peer = ROT == 1 && turn ? g * LPH + (second ? e0 - half : e0 + half) / V : lane;
+  constexpr int NC = ROT == 2 ? V / 2 : V;  // cosines of a lane
+  float co[NC], si[NC], wq[V], wk[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    co[i] = 1.f, si[i] = 0.f, wq[i] = 1.f, wk[i] = 1.f;
+  for (int i = 0; i < NC; ++i) {
+    co[i] = 1.f, si[i] = 0.f;
     if (turn) {
-      const int p = L.interleaved ? (e0 + i) >> 1 : second ? e0 + i - half : e0 + i;
+      const int p = ROT == 2 ? (e0 >> 1) + i : (second ? e0 - half : e0) + i;
       co[i] = turns[p];
       si[i] = turns[half + p];
-      if (L.interleaved ? !(i & 1) : !second) si[i] = -si[i];
+      if (ROT == 1 && !second) si[i] = -si[i];
     }
-    if (on && L.q.w) wq[i] = L.q.w[e0 + i];
-    if (on && L.k.w) wk[i] = L.k.w[e0 + i];
   }
-  const int heads = L.q.H + L.k.H;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    wq[i] = on && L.q.w ? L.q.w[e0 + i] : 1.f;
+    wk[i] = on && L.k.w ? L.k.w[e0 + i] : 1.f;
+  }
+  const int Hq = L.q.H, heads = Hq + L.k.H;
   const int step = wpr * (32 / LPH);
   const float inv_d = 1.f / (float)L.D;
+  // the row's heads, the keys' addressed as if they followed the queries
+  const T* xq = static_cast<const T*>(L.q.x) + (int64_t)row * L.q.ldx + e0;
+  const T* xk = static_cast<const T*>(L.k.x) + (int64_t)row * L.k.ldx + e0 - Hq * L.D;
+  T* yq = static_cast<T*>(L.q.y) + (int64_t)row * L.q.ldy + e0;
+  T* yk = static_cast<T*>(L.k.y) + (int64_t)row * L.k.ldy + e0 - Hq * L.D;
   // (whole warps stay in the loop: the shuffles need every lane)
-  for (int base = (int)(w - row * wpr) * (32 / LPH); base < heads; base += step * UNROLL) {
+  for (int base = part * (32 / LPH); base < heads; base += step * UNROLL) {
     float x[UNROLL][V];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const int h = base + u * step + g;
 #pragma unroll
       for (int i = 0; i < V; ++i) x[u][i] = 0.f;
-      if (on && h < heads) load_row<T, V, true>(head_of<T>(L, row, h).x + e0, x[u]);
+      if (on && h < heads) load_row<T, V, true>((h < Hq ? xq : xk) + h * L.D, x[u]);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       if (base + u * step >= heads) break;  // uniform over the warp
       const int h = base + u * step + g;
-      const Head<T> hd = head_of<T>(L, row, min(h, heads - 1));
+      const bool key = h >= Hq;
       if (L.norm) {
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) ss = fmaf(x[u][i], x[u][i], ss);
 #pragma unroll
         for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float r = 1.f / sqrtf(ss * inv_d + L.eps);
+        const float r = rsqrtf(fmaf(ss, inv_d, L.eps));
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[u][i] = x[u][i] * r * (hd.key ? wk[i] : wq[i]);
+        for (int i = 0; i < V; ++i) x[u][i] = x[u][i] * r * (key ? wk[i] : wq[i]);
       }
       float y[V];
+      if constexpr (ROT == 1) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float other = L.interleaved ? x[u][i ^ 1] : __shfl_sync(0xffffffffu, x[u][i], peer);
-        y[i] = turn ? fmaf(x[u][i], co[i], other * si[i]) : x[u][i];
+        for (int i = 0; i < V; ++i) {
+          const float other = __shfl_sync(0xffffffffu, x[u][i], peer);
+          y[i] = turn ? fmaf(x[u][i], co[i], other * si[i]) : x[u][i];
+        }
+      } else if constexpr (ROT == 2) {  // (lanes that do not turn have cosine 1 and sine 0)
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+          y[i] = fmaf(x[u][i], co[i / 2], -(x[u][i + 1] * si[i / 2]));
+          y[i + 1] = fmaf(x[u][i + 1], co[i / 2], x[u][i] * si[i / 2]);
+        }
+        if (!turn) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) y[i] = x[u][i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) y[i] = x[u][i];
       }
-      if (on && h < heads) store_row<T, V, true>(hd.y + e0, y);
+      if (on && h < heads) store_row<T, V, true>((key ? yk : yq) + h * L.D, y);
     }
   }
 }
@@ -122,8 +131,13 @@ __global__ void __launch_bounds__(256) qk_norm_scalar(const __grid_constant__ Qk
   bool ok;
   const float* turns = turns_of(L, row, lane, &ok);
   if (!ok) return;
-  const Head<T> hd = head_of<T>(L, row, (int)(w - row * heads));
-  const float* wt = hd.key ? L.k.w : L.q.w;
+  const int h = (int)(w - row * heads);
+  const bool key = h >= L.q.H;
+  const QkOperand& op = key ? L.k : L.q;
+  const int64_t at0 = (int64_t)(key ? h - L.q.H : h) * L.D;
+  const T* src = static_cast<const T*>(op.x) + row * op.ldx + at0;
+  T* dst = static_cast<T*>(op.y) + row * op.ldy + at0;
+  const float* wt = op.w;
   const int half = L.rot >> 1;
   float x[8], other[8];  // D <= 256
   float ss = 0.f;
@@ -132,16 +146,16 @@ __global__ void __launch_bounds__(256) qk_norm_scalar(const __grid_constant__ Qk
     const int e = lane + 32 * i;
     x[i] = other[i] = 0.f;
     if (e < L.D) {
-      x[i] = to_f32<T>(hd.x[e]);
+      x[i] = to_f32<T>(src[e]);
       ss = fmaf(x[i], x[i], ss);
-      if (e < L.rot) other[i] = to_f32<T>(hd.x[L.interleaved ? e ^ 1 : e < half ? e + half : e - half]);
+      if (e < L.rot) other[i] = to_f32<T>(src[L.interleaved ? e ^ 1 : e < half ? e + half : e - half]);
     }
   }
   float r = 1.f;
   if (L.norm) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    r = 1.f / sqrtf(ss * (1.f / (float)L.D) + L.eps);
+    r = rsqrtf(fmaf(ss, 1.f / (float)L.D, L.eps));
   }
   __syncwarp();  // in place: every lane has read its partners before any lane stores
 #pragma unroll
@@ -157,7 +171,7 @@ __global__ void __launch_bounds__(256) qk_norm_scalar(const __grid_constant__ Qk
       const bool first = L.interleaved ? !(e & 1) : e < half;
       y = fmaf(n, turns[p], m * (first ? -turns[half + p] : turns[half + p]));
     }
-    hd.y[e] = from_f32<T>(y);
+    dst[e] = from_f32<T>(y);
   }
 }
 
@@ -174,8 +188,12 @@ cudaError_t norm_as(const QkNormLaunch& L, bool vec, cudaStream_t s) {
     wpr = wpr < groups ? wpr : groups;
     const int64_t grid = (L.M * wpr + 7) / 8;
     if (grid > INT32_MAX) return cudaErrorInvalidValue;
-#define SUPRA_QK(N) \
-  case N: qk_norm_vec<T, N><<<(unsigned)grid, 256, 0, s>>>(L, (int)wpr); break;
+#define SUPRA_QK(N)                                                                               \
+  case N:                                                                                         \
+    if (L.rot == 0) qk_norm_vec<T, N, 0><<<(unsigned)grid, 256, 0, s>>>(L, (int)wpr);             \
+    else if (!L.interleaved) qk_norm_vec<T, N, 1><<<(unsigned)grid, 256, 0, s>>>(L, (int)wpr);    \
+    else qk_norm_vec<T, N, 2><<<(unsigned)grid, 256, 0, s>>>(L, (int)wpr);                        \
+    break;
     switch (lph) {
       SUPRA_QK(1)
       SUPRA_QK(2)
