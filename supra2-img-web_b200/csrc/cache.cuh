@@ -119,12 +119,15 @@ __device__ __forceinline__ void decode4(uint32_t u, float* x) {
   }
 }
 
-// x * y rounded to odd: truncated, with the last bit set when anything was cut off. Rounding such
-// a value to fewer bits gives what rounding the exact product would, so the code below is the
+// x * f and y * f rounded to odd: truncated, with the last bit set when anything was cut off. Rounding
+// such a value to fewer bits gives what rounding the exact product would, so a code made from it is the
 // nearest to the product itself and does not depend on how fp32 would round it first.
-__device__ __forceinline__ float mul_odd(float x, float y) {
-  const float p = __fmul_rz(x, y);
-  return fmaf(x, y, -p) != 0.f ? __uint_as_float(__float_as_uint(p) | 1u) : p;
+__device__ __forceinline__ void mul_odd2(float x, float y, float f, float& px, float& py) {
+  const float2 a = make_float2(x, y), b = make_float2(f, f);
+  const float2 p = __fmul2_rz(a, b);
+  const float2 r = __ffma2_rn(a, b, make_float2(-p.x, -p.y));  // what was cut off, exact
+  px = __uint_as_float(__float_as_uint(p.x) | min(__float_as_uint(r.x), 1u));
+  py = __uint_as_float(__float_as_uint(p.y) | min(__float_as_uint(r.y), 1u));
 }
 
 // The codes nearest to four values, ties to even, as one 32-bit word; |x| <= kQmax (up to one fp32

@@ -18,15 +18,44 @@ namespace {
 
 __device__ __forceinline__ uint32_t warp_max(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
 
-// The codes of V channels (4 or 8), as one or two words.
+// The codes nearest to V channels (4 or 8) times f, as one or two words.
 template <int FMT, int V>
-__device__ __forceinline__ void encode_row(const float (&x)[V], uint32_t (&u)[V / 4]) {
+__device__ __forceinline__ void encode_row(const float (&x)[V], float f, uint32_t (&u)[V / 4]) {
 #pragma unroll
   for (int k = 0; k < V / 4; ++k) {
     float y[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = x[4 * k + e];
+    mul_odd2(x[4 * k], x[4 * k + 1], f, y[0], y[1]);
+    mul_odd2(x[4 * k + 2], x[4 * k + 3], f, y[2], y[3]);
     u[k] = encode4<FMT>(y);
+  }
+}
+// The largest magnitude among the pieces, as fp32 bits: NaN above infinity above every number.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+template <typename T, int NV>
+__device__ __forceinline__ uint32_t largest_bits(const uint4 (&raw)[NV]) {
+  if constexpr (sizeof(T) == 4) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      m = max3_nan(m, fabsf(__uint_as_float(raw[i].x)), fabsf(__uint_as_float(raw[i].y)));
+      m = max3_nan(m, fabsf(__uint_as_float(raw[i].z)), fabsf(__uint_as_float(raw[i].w)));
+    }
+    return __float_as_uint(m);
+  } else {  // two at a time: magnitudes of 16-bit floats are in the order of their bits
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      m = __vmaxu2(m, raw[i].x & 0x7fff7fffu);
+      m = __vmaxu2(m, raw[i].y & 0x7fff7fffu);
+      m = __vmaxu2(m, raw[i].z & 0x7fff7fffu);
+      m = __vmaxu2(m, raw[i].w & 0x7fff7fffu);
+    }
+    const float2 f = unpack2<T>(__vmaxu2(m, m >> 16));
+    return __float_as_uint(f.x);
   }
 }
 template <int N>
@@ -73,20 +102,23 @@ __global__ void __launch_bounds__(512) cache_write_kernel(const __grid_constant_
   const T* src = static_cast<const T*>(is_v ? L.v : L.k) + (q.row0 + t0 - first) * ld + (int64_t)h * c.D + e;
   const float old = lo > 0 ? *scale : 0.f;
 
-  float x[NV][V];
-  uint32_t top = 0;  // |x| as its bits: NaN above infinity above every number
+  uint4 raw[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int slot = slot0 + i * rows;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (slot >= lo && slot < end) {
+      if constexpr (VEC) {
+        raw[i] = *reinterpret_cast<const uint4*>(src + slot * ld);
+      } else {
+        T y[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) x[i][k] = 0.f;
-    if (slot >= lo && slot < end) load_row<T, V, VEC>(src + slot * ld, x[i]);
+        for (int k = 0; k < V; ++k) y[k] = src[slot * ld + k];
+        memcpy(&raw[i], y, 16);
+      }
+    }
   }
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int k = 0; k < V; ++k) top = max(top, __float_as_uint(x[i][k]) & 0x7fffffffu);
-  top = warp_max(top);
+  uint32_t top = warp_max(largest_bits<T, NV>(raw));
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
   __syncthreads();  // (also: every thread has read the old scale)
   for (int w = 0; w < (int)(blockDim.x >> 5); ++w) top = max(top, part[w]);
@@ -103,20 +135,17 @@ __global__ void __launch_bounds__(512) cache_write_kernel(const __grid_constant_
     const int slot = slot0 + i * rows;
     if (slot >= end) break;
     uint8_t* at = codes + slot * c.D;
-    uint32_t u[V / 4];
+    uint32_t u[V / 4] = {};
+    float x[V];
     if (slot >= lo) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) x[i][k] = bad ? 0.f : mul_odd(x[i][k], inv);
-      encode_row<FMT, V>(x[i], u);
+      load_row<T, V, true>(reinterpret_cast<const T*>(&raw[i]), x);
+      if (!bad) encode_row<FMT, V>(x, inv, u);
       store_codes(at, u);
     } else if (again) {
       load_codes(at, u);
-      float y[V];
 #pragma unroll
-      for (int k = 0; k < V / 4; ++k) decode4<FMT>(u[k], y + 4 * k);
-#pragma unroll
-      for (int k = 0; k < V; ++k) y[k] = mul_odd(y[k], ratio);
-      encode_row<FMT, V>(y, u);
+      for (int k = 0; k < V / 4; ++k) decode4<FMT>(u[k], x + 4 * k);
+      encode_row<FMT, V>(x, ratio, u);
       store_codes(at, u);
     }
   }
@@ -158,19 +187,25 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const __grid_constant__
       from[i] = codes + (int64_t)h * head_bytes + (p - h * per_head) * V;
       s[i] = scale[h];
     }
-    for (int slot = lo + warp; slot < hi; slot += warps) {
-      uint32_t u[UN][V / 4];
+    for (int slot = lo + warp; slot < hi; slot += 2 * warps) {  // two rows at a time
+      uint32_t u[2][UN][V / 4];
 #pragma unroll
-      for (int i = 0; i < UN; ++i) load_codes(from[i] + slot * c.D, u[i]);
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int i = 0; i < UN; ++i) {
-        if (p0 + 32 * i >= per_row) break;
-        float x[V];
+        for (int i = 0; i < UN; ++i) load_codes(from[i] + min(slot + r * warps, hi - 1) * c.D, u[r][i]);
 #pragma unroll
-        for (int k = 0; k < V / 4; ++k) decode4<FMT>(u[i][k], x + 4 * k);
+      for (int r = 0; r < 2; ++r) {
+        if (slot + r * warps >= hi) break;
 #pragma unroll
-        for (int k = 0; k < V; ++k) x[k] *= s[i];
-        store_row<T, V, VEC>(dst + slot * ld + (int64_t)(p0 + 32 * i) * V, x);
+        for (int i = 0; i < UN; ++i) {
+          if (p0 + 32 * i >= per_row) break;
+          float x[V];
+#pragma unroll
+          for (int k = 0; k < V / 4; ++k) decode4<FMT>(u[r][i][k], x + 4 * k);
+#pragma unroll
+          for (int k = 0; k < V; ++k) x[k] *= s[i];
+          store_row<T, V, VEC>(dst + (slot + r * warps) * ld + (int64_t)(p0 + 32 * i) * V, x);
+        }
       }
     }
   }

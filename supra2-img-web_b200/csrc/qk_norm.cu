@@ -27,7 +27,7 @@ __device__ __forceinline__ const float* turns_of(const QkNormLaunch& L, int64_t 
 // LPH lanes per head (a power of two), V elements per lane; `wpr` warps share a row's heads. ROT: 0 no
 // rotation, 1 pairs half a rotation apart, 2 neighbours.
 template <typename T, int LPH, int ROT>
-__global__ void __launch_bounds__(256) qk_norm_vec(const __grid_constant__ QkNormLaunch L, int wpr) {
+__global__ void __launch_bounds__(128) qk_norm_vec(const __grid_constant__ QkNormLaunch L, int wpr) {
   constexpr int V = 16 / (int)sizeof(T);
   constexpr int UNROLL = 4;
   const int lane = threadIdx.x & 31, g = lane / LPH, l = lane % LPH;
@@ -186,13 +186,13 @@ cudaError_t norm_as(const QkNormLaunch& L, bool vec, cudaStream_t s) {
     const int groups = (heads + 32 / lph - 1) / (32 / lph);
     int64_t wpr = (148 * 16 + L.M - 1) / L.M;
     wpr = wpr < groups ? wpr : groups;
-    const int64_t grid = (L.M * wpr + 7) / 8;
+    const int64_t grid = (L.M * wpr + 3) / 4;
     if (grid > INT32_MAX) return cudaErrorInvalidValue;
 #define SUPRA_QK(N)                                                                               \
   case N:                                                                                         \
-    if (L.rot == 0) qk_norm_vec<T, N, 0><<<(unsigned)grid, 256, 0, s>>>(L, (int)wpr);             \
-    else if (!L.interleaved) qk_norm_vec<T, N, 1><<<(unsigned)grid, 256, 0, s>>>(L, (int)wpr);    \
-    else qk_norm_vec<T, N, 2><<<(unsigned)grid, 256, 0, s>>>(L, (int)wpr);                        \
+    if (L.rot == 0) qk_norm_vec<T, N, 0><<<(unsigned)grid, 128, 0, s>>>(L, (int)wpr);             \
+    else if (!L.interleaved) qk_norm_vec<T, N, 1><<<(unsigned)grid, 128, 0, s>>>(L, (int)wpr);    \
+    else qk_norm_vec<T, N, 2><<<(unsigned)grid, 128, 0, s>>>(L, (int)wpr);                        \
     break;
     switch (lph) {
       SUPRA_QK(1)
