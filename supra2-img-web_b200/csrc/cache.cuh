@@ -120,29 +120,41 @@ __device__ __forceinline__ void decode4(uint32_t u, float* x) {
 }
 
 // x * f and y * f rounded to odd: truncated, with the last bit set when anything was cut off. Rounding
-// such a value to fewer bits gives what rounding the exact product would, so a code made from it is the
-// nearest to the product itself and does not depend on how fp32 would round it first.
-__device__ __forceinline__ void mul_odd2(float x, float y, float f, float& px, float& py) {
+// such a value to fewer bits gives what rounding the exact product would.
+__device__ __forceinline__ float2 mul_odd2(float x, float y, float f) {
   const float2 a = make_float2(x, y), b = make_float2(f, f);
-  const float2 p = __fmul2_rz(a, b);
+  float2 p = __fmul2_rz(a, b);
   const float2 r = __ffma2_rn(a, b, make_float2(-p.x, -p.y));  // what was cut off, exact
-  px = __uint_as_float(__float_as_uint(p.x) | min(__float_as_uint(r.x), 1u));
-  py = __uint_as_float(__float_as_uint(p.y) | min(__float_as_uint(r.y), 1u));
+  p.x = __uint_as_float(__float_as_uint(p.x) | (__float_as_uint(r.x) != 0u));
+  p.y = __uint_as_float(__float_as_uint(p.y) | (__float_as_uint(r.y) != 0u));
+  return p;
 }
 
-// The codes nearest to four values, ties to even, as one 32-bit word; |x| <= kQmax (up to one fp32
-// rounding above it).
+// The codes nearest to the products of four values with f, ties to even, as one 32-bit word; the
+// products are at most kQmax (up to one fp32 rounding above it). The exact product is rounded once, to
+// the code.
 template <int FMT>
-__device__ __forceinline__ uint32_t encode4(const float (&x)[4]) {
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float f) {
   if constexpr (FMT == kCacheInt8) {
-    // adding 1.5 * 2^23 rounds to a whole number whose two's complement is in the low bits
-    uint32_t u[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(x[i] + 12582912.f);
-    return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+    // the fused sum with 1.5 * 2^23 rounds to a whole number whose two's complement is in the low bits
+    const float2 m = make_float2(12582912.f, 12582912.f), g = make_float2(f, f);
+    const float2 x = __ffma2_rn(make_float2(a, b), g, m), y = __ffma2_rn(make_float2(c, d), g, m);
+    return __byte_perm(__byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x0040),
+                       __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040), 0x5410);
   } else {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+    // A truncated product rounds like the exact one unless it lies on the border between two codes, and then
+    // its 19 low bits are 0: only those few are formed with what was cut off.
+    const float2 g = make_float2(f, f);
+    float2 x = __fmul2_rz(make_float2(a, b), g), y = __fmul2_rz(make_float2(c, d), g);
+    const uint32_t m = 0x7ffffu;
+    const uint32_t low = min(min(__float_as_uint(x.x) & m, __float_as_uint(x.y) & m),
+                             min(__float_as_uint(y.x) & m, __float_as_uint(y.y) & m));
+    if (low == 0u) {
+      x = mul_odd2(a, b, f);
+      y = mul_odd2(c, d, f);
+    }
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
     return lo | (hi << 16);
   }
 }

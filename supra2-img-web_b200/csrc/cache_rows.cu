@@ -7,8 +7,8 @@
 // neighbouring lanes on neighbouring pieces, the maximum is reduced over the CTA, and the codes leave
 // into the block's contiguous block_tokens * D bytes. Nothing is read twice and one launch does it all,
 // so the kernel is bound by the rows' bytes in and the codes out; a block is the unit because its scale is.
-// Read: value = code * scale in fp32, rounded once to the output type; one CTA per block of tokens
-// and K or V, a row per warp at a time, each lane storing 16 bytes.
+// Read: value = code * scale in fp32, rounded once to the output type; one CTA per 16 slots of a
+// block and K or V, a few rows per warp at a time, each lane storing 16 bytes.
 #include <algorithm>
 
 #include "cache.cuh"
@@ -22,12 +22,7 @@ __device__ __forceinline__ uint32_t warp_max(uint32_t x) { return __reduce_max_s
 template <int FMT, int V>
 __device__ __forceinline__ void encode_row(const float (&x)[V], float f, uint32_t (&u)[V / 4]) {
 #pragma unroll
-  for (int k = 0; k < V / 4; ++k) {
-    float y[4];
-    mul_odd2(x[4 * k], x[4 * k + 1], f, y[0], y[1]);
-    mul_odd2(x[4 * k + 2], x[4 * k + 3], f, y[2], y[3]);
-    u[k] = encode4<FMT>(y);
-  }
+  for (int k = 0; k < V / 4; ++k) u[k] = encode4<FMT>(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3], f);
 }
 // The largest magnitude among the pieces, as fp32 bits: NaN above infinity above every number.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
@@ -76,9 +71,9 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t (&u)[N]) 
 // Threads take pieces of 16 bytes of a row (V channels): thread t < rows * per_row has piece t % per_row of slots
 // t / per_row + i * rows, i < NV.
 template <typename T, int FMT, int NV, bool VEC>
-__global__ void __launch_bounds__(512) cache_write_kernel(const __grid_constant__ CacheRowsLaunch L, int nblk, int rows) {
+__global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant__ CacheRowsLaunch L, int nblk, int rows) {
   constexpr int V = 16 / (int)sizeof(T);
-  __shared__ uint32_t part[16];
+  __shared__ uint32_t part[8];
   const CachePool& c = L.c;
   const int b = blockIdx.x / nblk, h = blockIdx.y;
   SeqView q;
@@ -152,10 +147,11 @@ __global__ void __launch_bounds__(512) cache_write_kernel(const __grid_constant_
   if (threadIdx.x == 0) *scale = s;
 }
 
+constexpr int kReadRows = 16;  // slots of a CTA: small ones, so that the last wave is short
 template <typename T, int FMT, bool VEC>
-__global__ void __launch_bounds__(256) cache_read_kernel(const __grid_constant__ CacheRowsLaunch L, int nblk) {
+__global__ void __launch_bounds__(128) cache_read_kernel(const __grid_constant__ CacheRowsLaunch L, int nblk) {
   constexpr int V = 16 / (int)sizeof(T);
-  constexpr int UN = 4;  // pieces of a row that a lane has under way
+  constexpr int UN = 4, RN = V == 4 ? 4 : 2;  // pieces of a row, and rows, that a lane has under way
   const CachePool& c = L.c;
   const int b = blockIdx.x / nblk;
   SeqView q;
@@ -165,7 +161,9 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const __grid_constant__
   const int blk = (first >> c.log2t) + blockIdx.x % nblk;
   const int t0 = blk << c.log2t;
   if (t0 >= q.len) return;
-  const int lo = max(first - t0, 0), hi = min(q.len - t0, tokens);
+  const int part = blockIdx.z * kReadRows;
+  const int lo = max(first - t0, part), hi = min(min(q.len - t0, tokens), part + kReadRows);
+  if (lo >= hi) return;
   const int32_t page = block_of(L.s, c, b, blk, L.status);
   if (page < 0) return;
   const bool is_v = blockIdx.y != 0;
@@ -187,14 +185,14 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const __grid_constant__
       from[i] = codes + (int64_t)h * head_bytes + (p - h * per_head) * V;
       s[i] = scale[h];
     }
-    for (int slot = lo + warp; slot < hi; slot += 2 * warps) {  // two rows at a time
-      uint32_t u[2][UN][V / 4];
+    for (int slot = lo + warp; slot < hi; slot += RN * warps) {
+      uint32_t u[RN][UN][V / 4];
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < RN; ++r)
 #pragma unroll
         for (int i = 0; i < UN; ++i) load_codes(from[i] + min(slot + r * warps, hi - 1) * c.D, u[r][i]);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
+      for (int r = 0; r < RN; ++r) {
         if (slot + r * warps >= hi) break;
 #pragma unroll
         for (int i = 0; i < UN; ++i) {
@@ -217,25 +215,26 @@ int touched(const CacheSeqs& s, int log2t) { return (int)((s.max_rows + 2ll * (1
 template <typename T, int FMT, bool VEC>
 cudaError_t write_as(const CacheRowsLaunch& L, cudaStream_t s) {
   const int nblk = touched(L.s, L.c.log2t);
-  // As many threads as there are pieces, up to 256 (512 where a thread would hold more than 32 channels):
-  // whole rows of pieces, the last warp filled up.
-  constexpr int V = 16 / (int)sizeof(T), MOST = 32 / V;
+  // As many threads as there are pieces, up to 128 (256 where a thread would hold more than 8 pieces): whole
+  // rows of pieces, the last warp filled up. What a warp does besides its pieces is worth four of them.
+  constexpr int V = 16 / (int)sizeof(T);
   const int per_row = L.c.D / V, tokens = 1 << L.c.log2t;
-  int rows = std::min(tokens, 256 / per_row);
-  if ((tokens + rows - 1) / rows > MOST) rows = std::min(tokens, 512 / per_row);
+  int rows = std::min(tokens, 128 / per_row);
+  if ((tokens + rows - 1) / rows > 8) rows = std::min(tokens, 256 / per_row);
   const int nv = (tokens + rows - 1) / rows;
   const int threads = (rows * per_row + 31) / 32 * 32;
   const dim3 grid((unsigned)(L.s.B * nblk), (unsigned)L.c.H, 2);
   if (nv <= 1) cache_write_kernel<T, FMT, 1, VEC><<<grid, threads, 0, s>>>(L, nblk, rows);
   else if (nv <= 2) cache_write_kernel<T, FMT, 2, VEC><<<grid, threads, 0, s>>>(L, nblk, rows);
   else if (nv <= 4) cache_write_kernel<T, FMT, 4, VEC><<<grid, threads, 0, s>>>(L, nblk, rows);
-  else cache_write_kernel<T, FMT, 8, VEC><<<grid, threads, 0, s>>>(L, nblk, rows);  // (fp32; 8 is the most)
+  else if (nv <= 8) cache_write_kernel<T, FMT, 8, VEC><<<grid, threads, 0, s>>>(L, nblk, rows);
+  else cache_write_kernel<T, FMT, 18, VEC><<<grid, threads, 0, s>>>(L, nblk, rows);  // (fp32: up to 18)
   return cudaGetLastError();
 }
 template <typename T, int FMT, bool VEC>
 cudaError_t read_as(const CacheRowsLaunch& L, cudaStream_t s) {
   const int nblk = touched(L.s, L.c.log2t);
-  cache_read_kernel<T, FMT, VEC><<<dim3((unsigned)(L.s.B * nblk), 2), 256, 0, s>>>(L, nblk);
+  cache_read_kernel<T, FMT, VEC><<<dim3((unsigned)(L.s.B * nblk), 2, (1u << L.c.log2t) / kReadRows), 128, 0, s>>>(L, nblk);
   return cudaGetLastError();
 }
 
