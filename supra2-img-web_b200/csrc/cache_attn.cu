@@ -84,7 +84,9 @@ template <int FMT>
 __device__ __forceinline__ void codes4(uint32_t u, uint32_t& even, uint32_t& odd) {
   if constexpr (FMT == kCacheInt8) {
     // 0x64 above a byte b is the fp16 number 1024 + b; with b = code + 128, 1152 off gives the code
-    const uint32_t a = (u & 0x00ff00ffu) ^ 0x64806480u, b = ((u >> 8) & 0x00ff00ffu) ^ 0x64806480u;
+    // (masking and shifting, which takes both constants apart, came to five operations a word, this to three)
+    const uint32_t x = u ^ 0x80808080u;
+    const uint32_t a = __byte_perm(x, 0x64646464u, 0x4240), b = __byte_perm(x, 0x64646464u, 0x4341);
     const uint32_t off = 0x64806480u;
     const __half2 ha = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&off));
     const __half2 hb = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&off));
@@ -526,16 +528,20 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
   }
 }
 
-// Joins the workspace's parts of one row of one unit, always in the same order: warp w takes splits w, w + 8,
-// .. (lane: 4 channels), then the warps are added up.
+constexpr int kMaxSplits = 444;  // (one wave of three CTAs per SM)
+
+// Joins the workspace's parts of one row of one unit, always in the same order: the weights of all parts
+// first, then 256 / (D / 4) groups of threads (4 channels each) add up every so many-th part, and the
+// groups are added up.
 template <typename T>
 __global__ void __launch_bounds__(256) cache_attn_join(const __grid_constant__ CacheAttnArgs L, int tiles, int NR, bool last_first) {
-  __shared__ float4 po[8][32];
-  __shared__ float2 pml[8];
+  __shared__ float wt[kMaxSplits];
+  __shared__ float red[16];
+  __shared__ float4 po[256];
   const CachePool& c = L.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int unit = blockIdx.x;
-  const int64_t part0 = (int64_t)unit * L.splits;
+  const int64_t part0 = (int64_t)unit * L.splits * NR + blockIdx.y;
   // (the tensor-core kernel orders its units by row tile, the last ones first)
   const int heads = L.s.B * c.H;
   const int rt = last_first ? tiles - 1 - unit / heads : unit % tiles;
@@ -545,36 +551,52 @@ __global__ void __launch_bounds__(256) cache_attn_join(const __grid_constant__ C
   if (!seq_view(L.s, b, false, L.status, q)) return;
   const int pr = rt * NR + blockIdx.y;
   if (pr >= q.n * L.G) return;
-  float mx = -INFINITY, sum = 0.f;
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = warp; s < L.splits; s += 8) {
-    const int64_t at = (part0 + s) * NR + blockIdx.y;
-    const float2 ml = L.ws_ml[at];
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (4 * lane < c.D) v = *reinterpret_cast<const float4*>(L.ws_o + at * c.D + 4 * lane);
-    const float mn = fmaxf(mx, ml.x), ref = mn == -INFINITY ? 0.f : mn;
-    const float f = ex2f(mx - ref), g = ex2f(ml.x - ref);
-    mx = mn;
-    sum = sum * f + ml.y * g;
-    x.x = x.x * f + v.x * g, x.y = x.y * f + v.y * g, x.z = x.z * f + v.z * g, x.w = x.w * f + v.w * g;
+  float mx = -INFINITY, m[2], l[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int s = threadIdx.x + 256 * i;
+    const float2 ml = s < L.splits ? L.ws_ml[part0 + (int64_t)s * NR] : make_float2(-INFINITY, 0.f);
+    m[i] = ml.x, l[i] = ml.y;
+    mx = fmaxf(mx, ml.x);
   }
-  po[warp][lane] = x;
-  if (lane == 0) pml[warp] = make_float2(mx, sum);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) red[warp] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) mx = fmaxf(mx, red[w]);
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float f = ex2f(m[i] - ref);
+    if (threadIdx.x + 256 * i < L.splits) wt[threadIdx.x + 256 * i] = f;
+    sum = fmaf(l[i], f, sum);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) red[8 + warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) sum += red[8 + w];
+  const int per = c.D / 4, groups = 256 / per;
+  const int g = threadIdx.x / per, e = (threadIdx.x - g * per) * 4;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (g < groups) {
+#pragma unroll 8
+    for (int s = g; s < L.splits; s += groups) {
+      const float4 v = *reinterpret_cast<const float4*>(L.ws_o + (part0 + (int64_t)s * NR) * c.D + e);
+      const float f = wt[s];
+      x.x = fmaf(v.x, f, x.x), x.y = fmaf(v.y, f, x.y), x.z = fmaf(v.z, f, x.z), x.w = fmaf(v.w, f, x.w);
+    }
+  }
+  po[threadIdx.x] = x;
   __syncthreads();
   if (threadIdx.x >= c.D) return;
   const int d = threadIdx.x;
-  mx = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) mx = fmaxf(mx, pml[w].x);
-  const float ref = mx == -INFINITY ? 0.f : mx;
   float y = 0.f;
-  sum = 0.f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const float f = ex2f(pml[w].x - ref);
-    sum = fmaf(pml[w].y, f, sum);
-    y = fmaf(reinterpret_cast<const float*>(po[w])[d], f, y);
-  }
+  for (int k = 0; k < groups; ++k) y += reinterpret_cast<const float*>(po + k * per)[d];
   static_cast<T*>(L.o)[(q.row0 + pr / L.G) * L.ldo + (int64_t)(hk * L.G + pr % L.G) * c.D + d] =
       from_f32<T>(sum == 0.f ? 0.f : y / sum);
 }
@@ -640,7 +662,7 @@ CacheAttnPlan plan_cache_attn(const CacheAttnArgs& L) {
   P.tiles = (int)((rows + P.nr - 1) / P.nr);
   P.units = (int64_t)L.s.B * L.c.H * P.tiles;
   P.splits = 1;
-  const int wave = P.tc ? (L.c.D <= 64 ? 148 * 2 : 148) : 148 * 3;  // CTAs that run at once
+  const int wave = P.tc ? (L.c.D <= 64 ? 148 * 2 : 148) : kMaxSplits;  // CTAs that run at once
   const int64_t wide = std::min<int64_t>(wave / std::max<int64_t>(P.units, 1), L.s.max_len / 512);
   if (P.tc) {
     // fewer units than run at once, each with many tiles of tokens: split them
