@@ -163,6 +163,15 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, 
 // Waits for the phase with the given parity, for about two seconds at most; gives up at once when
 // *abort is set (abort may be null). The limit is counted in SM clocks and looked at only every 64
 // tries: a read of the global timer takes about 1500 cycles, more than most of these waits.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
 constexpr long long kWaitLimitClocks = 4000000000ll;
 __device__ __forceinline__ bool mbar_wait_clocked(uint64_t* bar, uint32_t parity, volatile int32_t* abort) {
   long long t0 = 0;

@@ -98,7 +98,7 @@ struct Bars {
 static_assert(sizeof(Bars) <= 192, "BAR");
 
 // status[2] of a wait that ran out
-enum TcWait : int32_t { W_RAW = 80, W_K_FULL = 81, W_V_FULL = 82, W_K_EMPTY = 83, W_V_EMPTY = 84, W_S = 85, W_PV = 86, W_P = 87 };
+enum TcWait : int32_t { W_RAW = 80, W_ISSUE = 81, W_K_EMPTY = 83, W_V_EMPTY = 84, W_S = 85, W_PV = 86 };
 
 __device__ __forceinline__ float ex2f(float x) {
   float y;
@@ -478,17 +478,13 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
     const uint64_t dk = tc::smem_desc(base + Y::K, 16, 1024, tc::kLayoutSW128);
     // V is MN-major: 64-channel slabs SLAB apart (LBO), 8-token groups 1024 B apart (SBO)
     const uint64_t dv = tc::smem_desc(base + Y::V, Y::SLAB, 1024, tc::kLayoutSW128);
-    auto all_wait = [&](uint64_t* bar, uint32_t parity, int32_t id, int32_t detail) {
-      const bool ok = __all_sync(0xffffffffu, wait_for(bar, parity, abort, L.status, id, detail));
-      tc::fence_after_sync();
-      return ok;
-    };
+    auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar, parity & 1u)); };
     // The scores of tile j into the S buffer of its parity, and P's product with V; each releases its
     // operand's stage.
     auto issue_s = [&](int rt, int j) {
       const int n = j - j0, st = n & 1;
       const uint64_t dq = dq0 + (uint64_t)(rt * ((Y::PARTS * Y::QPART) >> 4));
-      if (!all_wait(&B->k_full[st], (uint32_t)(n >> 1) & 1u, W_K_FULL, j)) return false;
+      tc::fence_after_sync();
       if (elect_one()) {
         const uint32_t id = idesc_f16(min(kN, (seen - j * kN + 31) & ~31), false);
         const uint32_t d = tmem + (uint32_t)(rt * Y::COL_RT + st * kN);
@@ -503,12 +499,10 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         tc::commit(&B->k_empty[st]);
       }
       __syncwarp();
-      return true;
     };
     auto issue_pv = [&](int rt, int j) {
       const int n = j - j0, st = n & 1;
-      if (!all_wait(&B->v_full[st], (uint32_t)(n >> 1) & 1u, W_V_FULL, j)) return false;
-      if (!all_wait(&B->p_full[rt], (uint32_t)n & 1u, W_P, j)) return false;
+      tc::fence_after_sync();
       if (elect_one()) {
         const int steps = (min(kN, seen - j * kN) + 15) >> 4;
         constexpr uint32_t id = idesc_f16(DT, true);
@@ -525,25 +519,44 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         tc::commit(&B->v_empty[st]);
       }
       __syncwarp();
-      return true;
     };
-    bool ok = true;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      bar_sync(2 + rt, 160);  // Q is in shared memory
-      tc::fence_after_sync();
-      if (j0 < j1 && ok) ok = issue_s(rt, j0);
-    }
-    for (int j = j0; j < j1 && ok; ++j) {
+    for (int rt = 0; rt < RT; ++rt) bar_sync(2 + rt, 160);  // Q is in shared memory
+    // Whatever is ready, for either row tile: they run at their own pace, so that one's softmax falls into the
+    // other's MMAs. Scores n need K and the S buffer that P n - 2 has left, product n needs P and V.
+    const int total = j1 - j0;
+    int ns[RT] = {}, np[RT] = {};
+    bool ok = true;
+    long long t0 = clock64();
+    for (int left = 2 * RT * total, idle = 0; left > 0 && ok;) {
+      bool moved = false;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        // the next scores go where the previous P was, once its product is formed
-        if (j + 1 < j1 && ok)
-          ok = (j == j0 || all_wait(&B->pv_full[rt], (uint32_t)(j - j0 - 1) & 1u, W_PV, j)) && issue_s(rt, j + 1);
+        int n = np[rt];
+        if (n < ns[rt] && ready(&B->p_full[rt], n) && ready(&B->v_full[n & 1], n >> 1)) {
+          issue_pv(rt, j0 + n);
+          ++np[rt], --left, moved = true;
+        }
+        n = ns[rt];
+        // (a parity tells a phase from its neighbours only: where product n - 1 is issued, P n - 1 was there,
+        // whose threads had waited for product n - 2)
+        if (n < total && n <= np[rt] + 1 && ready(&B->k_full[n & 1], n >> 1) && (n < 2 || np[rt] >= n || ready(&B->pv_full[rt], n - 2))) {
+          issue_s(rt, j0 + n);
+          ++ns[rt], --left, moved = true;
+        }
       }
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-        if (ok) ok = issue_pv(rt, j);
+      if (moved) {
+        idle = 0;
+        t0 = clock64();
+      } else if ((++idle & 63) == 0) {
+        if (*abort) ok = false;
+        else if (clock64() - t0 > kWaitLimitClocks) {
+          if (lane == 0) report_error(L.status, DEV_TIMEOUT, W_ISSUE, left);
+          *abort = 1;
+          ok = false;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+      }
     }
     if (!ok && elect_one()) {
       // MMAs in flight end before TMEM is freed: an arrival of their own, waited for within limits
