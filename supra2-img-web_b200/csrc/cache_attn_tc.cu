@@ -85,7 +85,7 @@ struct TileMeta {  // of a tile's four 16-token groups
   float iv[4];   // 1 / |v_scale|
   int32_t dead;  // groups whose block does not exist (bits), tokens past the end not among them
   int32_t neg;   // groups with a negative V scale (bits), which no write makes
-  int32_t odd;   // some group is dead, or a scale of it negative, not finite, or its K scale 0
+  int32_t odd;   // groups that are dead, or a scale of theirs is negative, not finite, or the K scale 0
   int32_t pad;
 };
 static_assert(sizeof(TileMeta) == 64, "META");
@@ -347,69 +347,74 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
     };
     int page = -2, page_n = -2;
     float ks = 0.f, vs = 0.f, ks_n = 0.f, vs_n = 0.f, lv = 0.f, iv = 1.f;
-    auto logs = [&] {
+    // Of the 8 tiles: the pool row of the lane's group, and over all groups (bits) those that a box starts at,
+    // whose block does not exist, with a negative V scale, and odd ones.
+    const uint32_t box_bytes = (uint32_t)min(kN, 1 << log2t) * 2 * DT;  // K and V
+    int y = 0;
+    uint32_t boxes = 0, dead = 0, neg = 0, odd = 0;
+    auto place = [&] {
+      const bool live = page >= 0 && page < c.blocks;
+      if (!live && page != -2) report_error(L.status, DEV_BAD_BLOCK, 2, page);
+      const int at = 16 * (lane & 3);  // of the group in its tile
+      const bool first = log2t >= 6 ? at == 0 : (at & ((1 << log2t) - 1)) == 0;  // one box per block of a tile
+      y = ((page * c.H + hk) << log2t) + ((16 * (g0 + lane)) & ((1 << log2t) - 1));  // (8 tiles on: the same slot)
+      boxes = __ballot_sync(0xffffffffu, live && first);
+      dead = __ballot_sync(0xffffffffu, !live && page != -2);
+    };
+    auto weigh = [&] {
+      const bool live = page >= 0 && page < c.blocks;
       const float av = fmaxf(fabsf(vs), kScaleFloor);
       lv = vs == vs ? log2f(av) : vs;
       iv = vs == vs ? 1.f / av : vs;
+      neg = __ballot_sync(0xffffffffu, live && vs < 0.f);
+      odd = dead | neg | __ballot_sync(0xffffffffu, live && !(ks > 0.f && ks <= 3.4028234e38f && fabsf(vs) <= 3.4028234e38f));
+      if (!live) ks = 1.f;  // (past the end: -inf times it stays -inf)
     };
-    if (ct < 32) {
-      page = page_at(g0 + lane);
-      page_n = page_at(g0 + 32 + lane);
-    }
-    // Tile j's blocks into its raw stage, and its scales into meta[j % kMeta]: lanes w .. w + 3 know its groups.
-    auto copy = [&](int j) {
-      if (j >= j1) return;
-      const int n = j - j0, st = n & 1, a = lane - 4 * (n & 7);
-      if ((n & 7) == 0 && n > 0) {
+    // The blocks of the CTA's n-th tile into its raw stage, and its scales into meta[n % kMeta]: lanes w .. w + 3
+    // know its groups.
+    auto copy = [&](int n) {
+      const int w = 4 * (n & 7), a = lane - w, st = n & 1;
+      if (w == 0 && n > 0) {
         page = page_n, ks = ks_n, vs = vs_n;
         page_n = page_at(g0 + 4 * n + 32 + lane);
-        logs();
+        place();
+        weigh();
       }
-      if ((n & 7) == 4) scales_at(page_n, ks_n, vs_n);
-      const bool mine = a >= 0 && a < 4, live = mine && page >= 0 && page < c.blocks;
-      if (mine && !live && page != -2) report_error(L.status, DEV_BAD_BLOCK, 2, page);
-      const bool first = log2t >= 6 ? a == 0 : ((16 * a) & ((1 << log2t) - 1)) == 0;  // one box per block of the tile
-      const uint32_t boxes = __ballot_sync(0xffffffffu, live && first);
-      const uint32_t dead = __ballot_sync(0xffffffffu, mine && !live && page != -2) >> (4 * (n & 7));
-      const int box_rows = min(kN, 1 << log2t);
+      const uint32_t b4 = boxes >> w & 15u;
       if (lane == 0) {
-        meta[n % kMeta].dead = (int32_t)(dead & 15u);  // (before the arrival: the converters read it)
-        mbar_arrive_expect_tx(&B->raw[st], (uint32_t)(__popc(boxes) * 2 * box_rows * DT));
+        meta[n % kMeta].dead = (int32_t)(dead >> w & 15u);  // (before the arrival: the converters read it)
+        mbar_arrive_expect_tx(&B->raw[st], (uint32_t)__popc(b4) * box_bytes);
       }
       __syncwarp();
-      if (boxes >> lane & 1) {
-        const int y = ((page * c.H + hk) << log2t) + ((j * kN + 16 * a) & ((1 << log2t) - 1));
+      if (a >= 0 && a < 4 && (b4 >> a & 1u)) {
         uint8_t* to = base + Y::RAWS + st * 2 * Y::RAWB + 16 * a * DT;
         tc::tma_load_2d(to, &mk, 0, y, &B->raw[st]);
         tc::tma_load_2d(to + Y::RAWB, &mv, 0, y, &B->raw[st]);
       }
+      if (w == 16) scales_at(page_n, ks_n, vs_n);
     };
-    auto describe = [&](int j) {
-      if (j >= j1) return;
-      const int n = j - j0, w = 4 * (n & 7), a = lane - w;
+    auto describe = [&](int n) {
+      const int w = 4 * (n & 7), a = lane - w;
       TileMeta& mt = meta[n % kMeta];
-      const bool mine = a >= 0 && a < 4, live = mine && page >= 0 && page < c.blocks;
-      const uint32_t dead = __ballot_sync(0xffffffffu, mine && !live && page != -2) >> w;
-      const uint32_t neg = __ballot_sync(0xffffffffu, live && vs < 0.f) >> w;
-      const uint32_t kodd = __ballot_sync(0xffffffffu, live && !(ks > 0.f && ks <= 3.4028234e38f && fabsf(vs) <= 3.4028234e38f)) >> w;
-      if (mine) {
-        mt.ks[a] = live ? ks : 1.f;  // (past the end: -inf times it stays -inf)
+      if (a >= 0 && a < 4) {
+        mt.ks[a] = ks;
         mt.lv[a] = lv;
         mt.iv[a] = iv;
       }
       if (lane == 0) {
-        mt.neg = (int32_t)(neg & 15u);
-        mt.odd = ((dead | neg | kodd) & 15u) != 0;
+        mt.neg = (int32_t)(neg >> w & 15u);
+        mt.odd = (int32_t)(odd >> w & 15u);
       }
     };
-    int loaded = min(j0 + 2, j1);
+    int loaded = min(2, j1 - j0);
     if (ct < 32) {
-      copy(j0);
-      copy(j0 + 1);
+      page = page_at(g0 + lane);
+      page_n = page_at(g0 + 32 + lane);
+      place();
+      for (int n = 0; n < loaded; ++n) copy(n);
       scales_at(page, ks, vs);
-      logs();
-      describe(j0);
-      describe(j0 + 1);
+      weigh();
+      for (int n = 0; n < loaded; ++n) describe(n);
     }
     constexpr int CPR = DT / 16;                                       // 16-byte pieces per row
     constexpr int PIECES = kN * CPR, NP = (PIECES + Y::CONV - 1) / Y::CONV;  // of a tile, of a thread
@@ -460,7 +465,7 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         mbar_arrive(kv ? &B->v_full[st] : &B->k_full[st]);
       }
       if (!(ok = bar_and(1, Y::CONV, ok))) break;  // every converter has left the raw stage
-      if (loaded < j1) {
+      if (loaded < j1 - j0) {
         if (ct < 32) {
           copy(loaded);
           describe(loaded);
@@ -469,7 +474,7 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       }
     }
     if (!ok && ct == 0) {  // copies in flight land before the CTA may leave
-      for (int j = j0; j < loaded; ++j) mbar_wait_clocked(&B->raw[(j - j0) & 1], (uint32_t)((j - j0) >> 1) & 1u, nullptr);
+      for (int n = 0; n < loaded; ++n) mbar_wait_clocked(&B->raw[n & 1], (uint32_t)(n >> 1) & 1u, nullptr);
     }
   } else if (warp == 4 * RT + 3) {
     // ---------------- MMA issue ----------------
