@@ -43,7 +43,7 @@ template <bool SPLIT>
 constexpr float kPShift = SPLIT ? 15.f : 7.f;
 constexpr float kLag = 8.f;
 constexpr float kScaleFloor = 7.7037197775489434e-34f;  // 2^-110, below any scale that a write makes
-constexpr int kMeta = 4;  // tiles whose scales are kept at once
+constexpr int kMeta = 8;  // tiles whose scales are kept at once
 
 template <int DT, bool SPLIT>
 struct Cfg {
@@ -418,52 +418,53 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
     }
     constexpr int CPR = DT / 16;                                       // 16-byte pieces per row
     constexpr int PIECES = kN * CPR, NP = (PIECES + Y::CONV - 1) / Y::CONV;  // of a tile, of a thread
-    bool ok = true;
-    for (int j = j0; j < j1; ++j) {
-      const int n = j - j0, st = n & 1;
-      const uint32_t ph = (uint32_t)(n >> 1) & 1u;
-      ok = wait_for(&B->raw[st], ph, abort, L.status, W_RAW, j);
-      const int tok0 = j * kN;
+    // K (kv 0) or V (kv 1) of the n-th tile into its operand stage, from the registers that hold its codes.
+    auto convert = [&](int n, int kv, uint4 (&w)[NP]) {
+      const int st = n & 1, tok0 = (j0 + n) * kN;
       const int nrows = min(kN, (seen - tok0 + 31) & ~31);
       const uint32_t dead = FMT == kCacheE4m3 ? (uint32_t)meta[n % kMeta].dead : 0u;
       // bytes past the last token (or of a block that does not exist) may be NaN codes: zeros instead
-      const bool cut = FMT == kCacheE4m3 && (tok0 + nrows > seen || dead);
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const uint8_t* src = base + Y::RAWS + (st * 2 + kv) * Y::RAWB;
-        uint4 w[NP];
+      if (FMT == kCacheE4m3 && (tok0 + nrows > seen || dead)) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          const int p = ct + i * Y::CONV;
-          if (p < PIECES) w[i] = *reinterpret_cast<const uint4*>(src + 16 * p);
+          const int r = (ct + i * Y::CONV) / CPR;
+          if (tok0 + r >= seen || (dead >> (r >> 4) & 1)) w[i] = make_uint4(0, 0, 0, 0);
         }
-        if (cut) {
-#pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            const int r = (ct + i * Y::CONV) / CPR;
-            if (tok0 + r >= seen || (dead >> (r >> 4) & 1)) w[i] = make_uint4(0, 0, 0, 0);
-          }
-        }
-        if (ok && n >= 2)
-          ok = wait_for(kv ? &B->v_empty[st] : &B->k_empty[st], ph ^ 1u, abort, L.status, kv ? W_V_EMPTY : W_K_EMPTY, j);
-        if (!ok) break;
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          const int p = ct + i * Y::CONV;
-          if (p >= PIECES) break;
-          const int r = p / CPR, pc = p % CPR, k = 2 * (pc & 3);
-          uint8_t* dst = base + (kv ? Y::V : Y::K) + st * Y::TILE + (pc >> 2) * Y::SLAB;
-          uint4 x, y;
-          codes_in_order<FMT>(w[i].x, x.x, x.y);
-          codes_in_order<FMT>(w[i].y, x.z, x.w);
-          codes_in_order<FMT>(w[i].z, y.x, y.y);
-          codes_in_order<FMT>(w[i].w, y.z, y.w);
-          *reinterpret_cast<uint4*>(dst + r * 128 + ((k ^ (r & 7)) << 4)) = x;
-          *reinterpret_cast<uint4*>(dst + r * 128 + (((k + 1) ^ (r & 7)) << 4)) = y;
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(kv ? &B->v_full[st] : &B->k_full[st]);
       }
+      if (n >= 2 && !wait_for(kv ? &B->v_empty[st] : &B->k_empty[st], ((uint32_t)(n >> 1) & 1u) ^ 1u, abort, L.status,
+                              kv ? W_V_EMPTY : W_K_EMPTY, j0 + n))
+        return false;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int p = ct + i * Y::CONV;
+        if (p >= PIECES) break;
+        const int r = p / CPR, pc = p % CPR, k = 2 * (pc & 3);
+        uint8_t* dst = base + (kv ? Y::V : Y::K) + st * Y::TILE + (pc >> 2) * Y::SLAB;
+        uint4 x, y;
+        codes_in_order<FMT>(w[i].x, x.x, x.y);
+        codes_in_order<FMT>(w[i].y, x.z, x.w);
+        codes_in_order<FMT>(w[i].z, y.x, y.y);
+        codes_in_order<FMT>(w[i].w, y.z, y.w);
+        *reinterpret_cast<uint4*>(dst + r * 128 + ((k ^ (r & 7)) << 4)) = x;
+        *reinterpret_cast<uint4*>(dst + r * 128 + (((k + 1) ^ (r & 7)) << 4)) = y;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(kv ? &B->v_full[st] : &B->k_full[st]);
+      return true;
+    };
+    bool ok = true;
+    for (int n = 0; n < j1 - j0; ++n) {
+      const int st = n & 1;
+      ok = ok && wait_for(&B->raw[st], (uint32_t)(n >> 1) & 1u, abort, L.status, W_RAW, j0 + n);
+      uint4 w[2][NP];
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int p = ct + i * Y::CONV;
+          if (p < PIECES) w[kv][i] = *reinterpret_cast<const uint4*>(base + Y::RAWS + (st * 2 + kv) * Y::RAWB + 16 * p);
+        }
+      ok = ok && convert(n, 0, w[0]);
       if (!(ok = bar_and(1, Y::CONV, ok))) break;  // every converter has left the raw stage
       if (loaded < j1 - j0) {
         if (ct < 32) {
@@ -472,6 +473,7 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         }
         ++loaded;
       }
+      ok = convert(n, 1, w[1]);
     }
     if (!ok && ct == 0) {  // copies in flight land before the CTA may leave
       for (int n = 0; n < loaded; ++n) mbar_wait_clocked(&B->raw[n & 1], (uint32_t)(n >> 1) & 1u, nullptr);
