@@ -31,7 +31,7 @@ int check_type(supra_attn_ctx* c, const char* what, int32_t type) {
 // rows of `width` elements of a strided operand: [off, off + (rows - 1) * ld + width) inside size
 int check_rows(supra_attn_ctx* c, const char* what, const char* name, const void* p, int64_t size, int64_t ld,
                int64_t off, int64_t rows, int64_t width, int es) {
-  if (!p) return set_err(c, SUPRA_ATTN_EINVAL, "%s: %s must be non-NULL", what, name);
+  if (!p && rows > 0) return set_err(c, SUPRA_ATTN_EINVAL, "%s: %s must be non-NULL", what, name);
   if (misaligned(p, es))
     return set_err(c, SUPRA_ATTN_EINVAL, "%s: %s must be aligned to its element type", what, name);
   if (ld < 0 || ld > kLim || off < 0 || off > kLim)

@@ -185,6 +185,18 @@ def test_norm_refusals(kw, needle):
     assert st == _lib.EINVAL and needle in msg, msg
 
 
+def test_calls_without_rows_take_null_operands():
+    none = dict(k=0, v=0, k_size=0, v_size=0, seqs__rows=0, seqs__max_rows=0)
+    for fn in (write_check, read_check):
+        assert run(fn, rows_desc(**none)) == (0, "")
+        assert run(fn, rows_desc(**none, seqs__B=0, seqs__lengths=0, seqs__table=0, seqs__row_start=0)) == (0, "")
+    assert run(attn_check, attn_desc(q=0, out=0, q_size=0, out_size=0, seqs__rows=0, seqs__max_rows=0)) == (0, "")
+    assert run(norm_check, norm_desc(M=0, q__x=0, q__y=0, k__x=0, k__y=0)) == (0, "")
+    for kw in (dict(seqs__rows=1, k=0), dict(seqs__rows=1, v=0)):
+        st, msg = run(read_check, rows_desc(**kw))
+        assert st == _lib.EINVAL and "non-NULL" in msg
+
+
 def test_null_descriptors():
     for fn in (write_check, read_check, attn_check, norm_check):
         msg = C.create_string_buffer(64)
