@@ -396,7 +396,8 @@ int check_cache_attn(supra_attn_ctx* c, const supra_attn_cache_attn_desc* d, Che
   if (d->H < 1 || d->H > 65535 || d->H % d->cache.H)
     return set_err(c, SUPRA_ATTN_EINVAL, "%s: H=%d must be a multiple of the cache's H=%d", what, d->H, d->cache.H);
   const float scale = d->flags & SUPRA_ATTN_CA_DEFAULT_SCALE ? (float)(1.0 / std::sqrt((double)d->cache.D)) : d->scale;
-  if (!std::isfinite(scale)) return set_err(c, SUPRA_ATTN_EINVAL, "%s: scale must be finite", what);
+  if (!std::isfinite(scale * kLog2e))  // (scores are formed in powers of two)
+    return set_err(c, SUPRA_ATTN_EINVAL, "%s: scale must be finite, and so its product with log2(e)", what);
   if (((int64_t)d->cache.blocks * d->cache.H << L.c.log2t) > INT32_MAX)
     return set_err(c, SUPRA_ATTN_EINVAL, "%s: blocks*H*block_tokens must be below 2^31", what);
   const int es = esize(d->type);

@@ -185,6 +185,12 @@ def test_norm_refusals(kw, needle):
     assert st == _lib.EINVAL and needle in msg, msg
 
 
+@pytest.mark.parametrize("scale,ok", [(2.3e38, True), (-2.3e38, True), (2.4e38, False), (-3.4e38, False), (float("nan"), False)])
+def test_attention_scale_in_powers_of_two_stays_finite(scale, ok):
+    st, msg = run(attn_check, attn_desc(flags=0, scale=scale))
+    assert st == (0 if ok else _lib.EINVAL) and ("scale" in msg) == (not ok)
+
+
 def test_calls_without_rows_take_null_operands():
     none = dict(k=0, v=0, k_size=0, v_size=0, seqs__rows=0, seqs__max_rows=0)
     for fn in (write_check, read_check):
