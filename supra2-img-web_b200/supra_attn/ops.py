@@ -164,6 +164,7 @@ class GPU:
             raise ValueError("read: count exceeds the tensor")
         out = np.empty(n, dtype=np.float32)
         check(lib.supra_attn_download(self.ctx, out.ctypes.data_as(C.c_void_p), C.c_void_p(buf), n), self.ctx)
+        self._held.clear()
         return out
 
     def _read_as(self, t: Tensor, count: int | None) -> np.ndarray:

@@ -663,6 +663,17 @@ def test_more_rows_than_tokens_is_reported(gpu, what):
     bad_call(gpu, p, seqs, what, 4, "sequence 0")
 
 
+def test_every_read_lets_go_of_the_operands(gpu):
+    p = Pool(gpu, np.random.default_rng(20), "int8", 16, 2, 32, [3])
+    _, seqs = p.batch([3])
+    out = gpu.empty([3, 64])
+    for t in (out, gpu.empty([4], "int32")):
+        supra_attn.cache_attention(gpu, p.cache, seqs, q=torch.zeros(3, 64, device="cuda"), H=2, out=out)
+        assert len(gpu._held) == 1
+        gpu.read(t)
+        assert not gpu._held
+
+
 def test_python_refusals(gpu):
     p = Pool(gpu, np.random.default_rng(19), "int8", 16, 2, 32, [3])
     _, seqs = p.batch([3])
