@@ -135,7 +135,7 @@ class GPU:
         if dtype not in DTYPES:
             raise ValueError(f"dtype must be one of {sorted(DTYPES)}")
         a = np.asarray(arr)
-        if a.size and not np.array_equal(a.astype(DTYPES[dtype]), a):
+        if a.size and not np.array_equal(a.astype(DTYPES[dtype]), a, equal_nan=True):
             raise ValueError(f"from_array: values that {dtype} does not hold")
         a = np.ascontiguousarray(a.astype(DTYPES[dtype])).reshape(-1)
         t = self.empty(list(shape) if shape is not None else [a.size], dtype)

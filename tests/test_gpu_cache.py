@@ -663,6 +663,17 @@ def test_more_rows_than_tokens_is_reported(gpu, what):
     bad_call(gpu, p, seqs, what, 4, "sequence 0")
 
 
+def test_arrays_of_other_types_keep_their_values(gpu):
+    for a, t in ((np.array([1.5, -np.inf, np.nan, 6e-8], np.float16), "fp16"), (np.array([-3, 7], np.int32), "int32"),
+                 (np.arange(5, dtype=np.uint8), "uint8"), (np.array([0x7fc0, 1], np.uint16), "bf16")):
+        x = gpu.from_array(a, dtype=t)
+        assert x.dtype == t and x.shape == [a.size]
+        assert gpu.read(x).tobytes() == a.tobytes()
+    for a, t in (([1.1], "fp16"), ([1 << 31], "int32"), ([-1], "uint8"), ([np.nan], "int32")):
+        with pytest.raises(ValueError, match="does not hold"), np.errstate(all="ignore"):
+            gpu.from_array(a, dtype=t)
+
+
 def test_every_read_lets_go_of_the_operands(gpu):
     p = Pool(gpu, np.random.default_rng(20), "int8", 16, 2, 32, [3])
     _, seqs = p.batch([3])
