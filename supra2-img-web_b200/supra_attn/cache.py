@@ -66,6 +66,13 @@ def _operand(gpu: GPU, x, name: str, dtypes):
     raise ValueError(f"{name}: must be {' or '.join(dtypes)}, not {x.dtype}")
 
 
+def _counts(**n):
+    """The library's counts are 32-bit numbers; ctypes would cut longer ones off without a word."""
+    for name, x in n.items():
+        if not -1 << 31 <= x < 1 << 31:
+            raise ValueError(f"{name}={x} out of range")
+
+
 _FLOATS = ("fp32", "fp16", "bf16")
 _INTS, _CODES, _F32 = ("int32",), ("uint8",), ("fp32",)
 
@@ -87,6 +94,7 @@ class KVCache:
             raise ValueError("pass all of k, v, k_scale and v_scale, or none")
         self.gpu, self.format = gpu, format
         self.blocks, self.block_tokens, self.H, self.D = int(blocks), int(block_tokens), int(H), int(D)
+        _counts(blocks=self.blocks, block_tokens=self.block_tokens, H=self.H, D=self.D)
         self._owned = []
         if not given:
             if min(self.blocks, self.block_tokens, self.H, self.D) < 1:
@@ -152,6 +160,7 @@ class CacheBatch:
             s.rows = s.B * int(max_rows)
             if rows is not None and int(rows) != s.rows:
                 raise ValueError("without row_start, rows is B*max_rows")
+        _counts(max_rows=int(max_rows), max_len=int(max_len or 0))
         s.max_rows = int(max_rows)
         # (-1: as many as the table's rows hold, which needs the cache's block size)
         s.max_len = -1 if max_len is None else int(max_len)
@@ -228,6 +237,8 @@ def cache_attention(gpu: GPU, cache: KVCache, seqs: CacheBatch, *, q, H: int, ou
         if ot != qt:
             raise ValueError("q and out must have the same type")
         d.type, d.H = _TYPES[qt], int(H)
+        if d.H != H:
+            raise ValueError(f"H={H} out of range")
         width = d.H * cache.D
         d.ldq = width if ldq is None else int(ldq)
         d.ldo = width if ldo is None else int(ldo)
@@ -288,6 +299,7 @@ def qk_norm(gpu: GPU, *, q, M: int, Hq: int, D: int, k=None, Hk: int = 0, qOut=N
     if len(kinds) != 1:
         raise ValueError("q, k and their outputs must have the same type")
     d.type = _TYPES[kinds.pop()]
+    _counts(M=int(M), D=int(D), rot=int(rot), Hq=int(Hq), Hk=int(Hk))
     d.M, d.D, d.rot, d.eps = int(M), int(D), int(rot), float(eps)
     if turns is not None:
         d.turns, d.turns_size, _ = _operand(gpu, turns, "turns", _F32)

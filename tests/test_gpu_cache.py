@@ -674,6 +674,26 @@ def test_arrays_of_other_types_keep_their_values(gpu):
             gpu.from_array(a, dtype=t)
 
 
+def test_counts_past_32_bits_are_refused(gpu):
+    p = Pool(gpu, np.random.default_rng(21), "int8", 16, 2, 32, [3])
+    start, seqs = p.batch([3])
+    x = torch.zeros(3, 64, device="cuda")
+    big = 1 << 32
+    with pytest.raises(ValueError, match="out of range"):
+        supra_attn.cache_attention(gpu, p.cache, seqs, q=x, H=big + 2, out=x.clone())
+    with pytest.raises(ValueError, match="out of range"):
+        supra_attn.CacheBatch(gpu, p.d_len, p.d_table, max_rows=big + 3, row_start=torch.tensor(start).int().cuda(), rows=3)
+    with pytest.raises(ValueError, match="out of range"):
+        supra_attn.CacheBatch(gpu, p.d_len, p.d_table, max_len=big + 3)
+    c = p.cache
+    with pytest.raises(ValueError, match="out of range"):
+        supra_attn.KVCache(gpu, big + 1, c.H, c.D, block_tokens=16, k=c.k, v=c.v, k_scale=c.k_scale, v_scale=c.v_scale)
+    for kw in (dict(M=big + 3), dict(Hq=big + 2), dict(D=big + 32)):
+        with pytest.raises(ValueError, match="out of range"):
+            supra_attn.qk_norm(gpu, q=x, **{**dict(M=3, Hq=2, D=32), **kw})
+    assert gpu.pending() == 0
+
+
 def test_every_read_lets_go_of_the_operands(gpu):
     p = Pool(gpu, np.random.default_rng(20), "int8", 16, 2, 32, [3])
     _, seqs = p.batch([3])
