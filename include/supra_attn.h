@@ -385,9 +385,11 @@ SUPRA_ATTN_API int supra_attn_enqueue_cache_attention(supra_attn_ctx* ctx, const
 SUPRA_ATTN_API int supra_attn_check_cache_attention_desc(const supra_attn_cache_attn_desc* desc, char* msg,
                                                          int32_t cap);
 /* The launches of these four calls take their descriptors as kernel arguments and use no memory of
- * the context but its status word, so a flush of them alone (profiling off) may be captured into a
- * CUDA graph on the context's stream, and graphs captured from one context may run at the same time
- * where their own operands allow it. */
+ * the context but its status word and, for cache_attention where few rows meet a long cache, a
+ * workspace ordered on the context's stream, which inside a stream capture belongs to the graph. So a
+ * flush of them alone (profiling off) may be captured into a CUDA graph on the context's stream, a
+ * context's first flush among them, and graphs captured from one context may run at the same time where
+ * their own operands allow it. Release such graphs before the context. */
 
 /* ---- profiling (the reference's Profiler, app/gpu/device.js:91-99,222-233,272-325) -------- */
 /* When on, every grouped launch is bracketed by CUDA events on the launching stream and

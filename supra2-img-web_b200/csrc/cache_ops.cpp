@@ -158,13 +158,18 @@ int scratch_alloc(supra_attn_ctx* c, size_t bytes, void** p) {
     props.allocType = cudaMemAllocationTypePinned;
     props.location.type = cudaMemLocationTypeDevice;
     props.location.id = c->device;
+    // (the stream may be capturing: making a pool is not work of the graph)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
     e = cudaMemPoolCreate(&c->async_pool, &props);
+    uint64_t keep = UINT64_MAX;
+    if (e == cudaSuccess) e = cudaMemPoolSetAttribute(c->async_pool, cudaMemPoolAttrReleaseThreshold, &keep);
+    cudaThreadExchangeStreamCaptureMode(&mode);
     if (e != cudaSuccess) {
+      if (c->async_pool) cudaMemPoolDestroy(c->async_pool);
       c->async_pool = nullptr;
       return cuda_err(c, e, "cache_attention: memory pool");
     }
-    uint64_t keep = UINT64_MAX;
-    cudaMemPoolSetAttribute(c->async_pool, cudaMemPoolAttrReleaseThreshold, &keep);
   }
   e = cudaMallocFromPoolAsync(p, bytes, c->async_pool, c->stream);
   if (e == cudaErrorMemoryAllocation) {

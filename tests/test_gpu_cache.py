@@ -376,6 +376,116 @@ def test_captured_split_over_many_ctas(gpu):
     ctx.close()
 
 
+def test_first_call_of_a_context_may_be_a_captured_one(gpu):
+    """Nothing of a context has been set up yet when its first call, one with a workspace, is captured."""
+    p = Pool(gpu, np.random.default_rng(23), "int8", 128, 1, 64, [12000])
+    _, seqs = p.batch([1])
+    q = torch.randn(1, 128, device="cuda")
+    want, got = torch.zeros(1, 128, device="cuda"), torch.zeros(1, 128, device="cuda")
+    supra_attn.cache_attention(gpu, p.cache, seqs, q=q, H=2, out=want)
+    gpu.sync()
+    side = torch.cuda.Stream()
+    ctx = supra_attn.GPU(0, stream=side)
+    cache = supra_attn.KVCache(ctx, p.blocks, 1, 64, block_tokens=128, format="int8", k=p.d[0], v=p.d[1], k_scale=p.d[2], v_scale=p.d[3])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        supra_attn.cache_attention(ctx, cache, seqs, q=q, H=2, out=got)
+        ctx.flush()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    supra_attn.cache_attention(ctx, cache, seqs, q=q, H=2, out=got.zero_())  # and an eager one after it
+    torch.cuda.synchronize()
+    ctx.sync()
+    assert torch.equal(got, want)
+    del graph
+    ctx.close()
+
+
+def test_two_contexts_at_once(gpu):
+    """Two contexts on two streams read one cache at the same time; each has its own workspace."""
+    p = Pool(gpu, np.random.default_rng(24), "e4m3", 64, 2, 64, [11000, 9000])
+    _, seqs = p.batch([1, 1])
+    q = [torch.randn(2, 4 * 64, device="cuda") for _ in range(2)]
+    want = [torch.zeros(2, 256, device="cuda") for _ in range(2)]
+    for a, o in zip(q, want):
+        supra_attn.cache_attention(gpu, p.cache, seqs, q=a, H=4, out=o)
+    gpu.sync()
+    ctxs = [supra_attn.GPU(0, stream=torch.cuda.Stream()) for _ in range(2)]
+    outs = [[torch.zeros(2, 256, device="cuda") for _ in range(8)] for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(8):
+        for c, a, o in zip(ctxs, q, outs):
+            supra_attn.cache_attention(c, p.cache, seqs, q=a, H=4, out=o[i])
+            c.flush()
+    for c in ctxs:
+        c.sync()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(x, w) for x in o)
+    for c in ctxs:
+        c.close()
+
+
+def test_queue_of_all_kinds_of_calls(gpu):
+    """Independent calls of every kind in one queue give what each gives alone, also while profiled."""
+    rng = np.random.default_rng(25)
+    p = Pool(gpu, rng, "int8", 16, 2, 64, [40, 9])
+    _, seqs = p.batch([3, 1])
+    f = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32)).cuda()  # noqa: E731
+    x, w, q, kv, n = f(64, 128), f(96, 128), f(4, 256), f(64, 3 * 128), f(32, 256)
+
+    def calls(flush):
+        o = [torch.zeros(64, 96, device="cuda"), torch.zeros(64, 128, device="cuda"), torch.zeros(4, 256, device="cuda"),
+             torch.zeros(4, 128, device="cuda"), torch.zeros(4, 128, device="cuda"), torch.zeros(32, 256, device="cuda")]
+        torch.cuda.synchronize()
+        for call in (lambda: supra_attn.linear(gpu, x, w, N=96, K=128, M=64, out=o[0]),
+                     lambda: supra_attn.cache_attention(gpu, p.cache, seqs, q=q, H=4, out=o[2], causal=True),
+                     lambda: supra_attn.attention(gpu, q=kv, k=kv, v=kv, Lq=64, Lk=64, H=2, D=64, ldq=384, ldk=384, ldv=384,
+                                                  kOff=128, vOff=256, out=o[1]),
+                     lambda: supra_attn.cache_read(gpu, p.cache, seqs, k=o[3], v=o[4]),
+                     lambda: supra_attn.qk_norm(gpu, q=n, qOut=o[5], M=32, Hq=4, D=64)):
+            call()
+            if flush:
+                gpu.flush()
+        pending = gpu.pending()
+        gpu.sync()
+        return o, pending
+
+    alone, _ = calls(True)
+    together, pending = calls(False)
+    assert pending == 5
+    gpu.profile(True)
+    try:
+        profiled, _ = calls(False)
+        names = {e["name"] if isinstance(e, dict) else e[0] for e in gpu.profile_report()}
+    finally:
+        gpu.profile(False)
+        gpu.profile_reset()
+    assert {"qk_norm", "cache_read", "cache_attention_rows_fp32"} <= names
+    for a, b, c in zip(alone, together, profiled):
+        assert torch.equal(a, b) and torch.equal(a, c)
+        assert a.abs().max() > 0
+
+
+def test_calls_without_sequences_or_rows(gpu):
+    """No sequences, or none with rows: nothing runs, and empty torch tensors (which have no address) will do."""
+    p = Pool(gpu, np.random.default_rng(26), "int8", 16, 2, 32, [3])
+    none = torch.empty(0, 64, device="cuda")
+    ints = torch.empty(0, dtype=torch.int32, device="cuda")
+    no_seqs = supra_attn.CacheBatch(gpu, ints, ints.view(0, 4))
+    no_rows = supra_attn.CacheBatch(gpu, p.d_len, p.d_table, max_rows=0)
+    launched = gpu.launch_count()
+    for seqs in (no_seqs, no_rows):
+        supra_attn.cache_write(gpu, p.cache, seqs, k=none, v=none)
+        supra_attn.cache_read(gpu, p.cache, seqs, k=none, v=none)
+        assert supra_attn.cache_attention(gpu, p.cache, seqs, q=none, H=2, out=none) is none
+        supra_attn.cache_attention(gpu, p.cache, seqs, q=none, H=2).release()
+    supra_attn.qk_norm(gpu, q=none, M=0, Hq=2, D=32)
+    gpu.sync()
+    assert gpu.launch_count() == launched
+    p.check_same()
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_attention_scale_and_sharp_scores(gpu, dtype):
     check_attention(gpu, "int8", dtype, 64, 2, 2, 64, [300, 40], [5, 33], True, scale=0.25, seed=5, sharp=4.0)
