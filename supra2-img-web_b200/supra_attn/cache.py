@@ -94,7 +94,8 @@ class KVCache:
             raise ValueError("pass all of k, v, k_scale and v_scale, or none")
         self.gpu, self.format = gpu, format
         self.blocks, self.block_tokens, self.H, self.D = int(blocks), int(block_tokens), int(H), int(D)
-        _counts(blocks=self.blocks, block_tokens=self.block_tokens, H=self.H, D=self.D)
+        if (self.blocks | self.block_tokens | self.H | self.D) >> 31:
+            _counts(blocks=self.blocks, block_tokens=self.block_tokens, H=self.H, D=self.D)
         self._owned = []
         if not given:
             if min(self.blocks, self.block_tokens, self.H, self.D) < 1:
@@ -160,8 +161,10 @@ class CacheBatch:
             s.rows = s.B * int(max_rows)
             if rows is not None and int(rows) != s.rows:
                 raise ValueError("without row_start, rows is B*max_rows")
-        _counts(max_rows=int(max_rows), max_len=int(max_len or 0))
-        s.max_rows = int(max_rows)
+        max_rows = int(max_rows)
+        if (max_rows | int(max_len or 0)) >> 31:
+            _counts(max_rows=max_rows, max_len=int(max_len or 0))
+        s.max_rows = max_rows
         # (-1: as many as the table's rows hold, which needs the cache's block size)
         s.max_len = -1 if max_len is None else int(max_len)
         if max_len is not None and int(max_len) < 0:
@@ -299,8 +302,10 @@ def qk_norm(gpu: GPU, *, q, M: int, Hq: int, D: int, k=None, Hk: int = 0, qOut=N
     if len(kinds) != 1:
         raise ValueError("q, k and their outputs must have the same type")
     d.type = _TYPES[kinds.pop()]
-    _counts(M=int(M), D=int(D), rot=int(rot), Hq=int(Hq), Hk=int(Hk))
-    d.M, d.D, d.rot, d.eps = int(M), int(D), int(rot), float(eps)
+    M, D, rot = int(M), int(D), int(rot)
+    if (M | D | rot | int(Hq) | int(Hk)) >> 31:
+        _counts(M=M, D=D, rot=rot, Hq=int(Hq), Hk=int(Hk))
+    d.M, d.D, d.rot, d.eps = M, D, rot, float(eps)
     if turns is not None:
         d.turns, d.turns_size, _ = _operand(gpu, turns, "turns", _F32)
         d.n_turns = min(d.turns_size // max(1, d.rot), (1 << 31) - 1)
