@@ -530,27 +530,40 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
 
 constexpr int kMaxSplits = 444;  // (one wave of three CTAs per SM)
 
-// Joins the workspace's parts of one row of one unit, always in the same order: the weights of all parts
-// first, then 256 / (D / 4) groups of threads (4 channels each) add up every so many-th part, and the
-// groups are added up.
-template <typename T>
-__global__ void __launch_bounds__(256) cache_attn_join(const __grid_constant__ CacheAttnArgs L, int tiles, int NR, bool last_first) {
-  __shared__ float wt[kMaxSplits];
-  __shared__ float red[16];
-  __shared__ float4 po[256];
+// The row of the workspace's unit and tile that a join works on: its first part, and where it belongs.
+struct JoinRow {
+  int64_t part0;
+  int64_t out;  // element of its first channel
+};
+__device__ __forceinline__ bool join_row(const CacheAttnArgs& L, int tiles, int NR, bool last_first, int unit, int r, JoinRow& j) {
   const CachePool& c = L.c;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int unit = blockIdx.x;
-  const int64_t part0 = (int64_t)unit * L.splits * NR + blockIdx.y;
+  j.part0 = (int64_t)unit * L.splits * NR + r;
   // (the tensor-core kernel orders its units by row tile, the last ones first)
   const int heads = L.s.B * c.H;
   const int rt = last_first ? tiles - 1 - unit / heads : unit % tiles;
   unit = last_first ? unit % heads : unit / tiles;
   const int hk = unit % c.H, b = unit / c.H;
   SeqView q;
-  if (!seq_view(L.s, b, false, L.status, q)) return;
-  const int pr = rt * NR + blockIdx.y;
-  if (pr >= q.n * L.G) return;
+  if (!seq_view(L.s, b, false, L.status, q)) return false;
+  const int pr = rt * NR + r;
+  if (pr >= q.n * L.G) return false;
+  j.out = (q.row0 + pr / L.G) * L.ldo + (int64_t)(hk * L.G + pr % L.G) * c.D;
+  return true;
+}
+
+// Joins the workspace's parts of one row of one unit, always in the same order, where there are few rows and
+// many parts: the weights of all parts first, then 256 / (D / 4) groups of threads (4 channels each) add up every
+// so many-th part, and the groups are added up.
+template <typename T>
+__global__ void __launch_bounds__(256) cache_attn_join(const __grid_constant__ CacheAttnArgs L, int tiles, int NR) {
+  __shared__ float wt[kMaxSplits];
+  __shared__ float red[16];
+  __shared__ float4 po[256];
+  const CachePool& c = L.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  JoinRow row;
+  if (!join_row(L, tiles, NR, false, blockIdx.x, blockIdx.y, row)) return;
+  const int64_t part0 = row.part0;
   float mx = -INFINITY, m[2], l[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -597,8 +610,46 @@ __global__ void __launch_bounds__(256) cache_attn_join(const __grid_constant__ C
   const int d = threadIdx.x;
   float y = 0.f;
   for (int k = 0; k < groups; ++k) y += reinterpret_cast<const float*>(po + k * per)[d];
-  static_cast<T*>(L.o)[(q.row0 + pr / L.G) * L.ldo + (int64_t)(hk * L.G + pr % L.G) * c.D + d] =
-      from_f32<T>(sum == 0.f ? 0.f : y / sum);
+  static_cast<T*>(L.o)[row.out + d] = from_f32<T>(sum == 0.f ? 0.f : y / sum);
+}
+
+// The same where there are many rows: one row a warp, its parts' statistics 32 at a time in its lanes.
+template <typename T>
+__global__ void __launch_bounds__(256) cache_attn_join_rows(const __grid_constant__ CacheAttnArgs L, int tiles, int NR) {
+  const CachePool& c = L.c;
+  const int lane = threadIdx.x & 31;
+  JoinRow row;
+  if (!join_row(L, tiles, NR, true, blockIdx.x, blockIdx.y * 8 + (threadIdx.x >> 5), row)) return;  // (whole warps)
+  auto part = [&](int s) { return s < L.splits ? L.ws_ml[row.part0 + (int64_t)s * NR] : make_float2(-INFINITY, 0.f); };
+  float mx = -INFINITY;
+  for (int s0 = 0; s0 < L.splits; s0 += 32) mx = fmaxf(mx, part(s0 + lane).x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  const bool on = 4 * lane < c.D;
+  for (int s0 = 0; s0 < L.splits; s0 += 32) {
+    const float2 ml = part(s0 + lane);
+    const float f = ex2f(ml.x - ref);
+    sum = fmaf(ml.y, f, sum);
+    const int n = min(32, L.splits - s0);
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) {
+      const float w = __shfl_sync(0xffffffffu, f, k);
+      if (on) {
+        const float4 v = *reinterpret_cast<const float4*>(L.ws_o + (row.part0 + (int64_t)(s0 + k) * NR) * c.D + 4 * lane);
+        x.x = fmaf(v.x, w, x.x), x.y = fmaf(v.y, w, x.y), x.z = fmaf(v.z, w, x.z), x.w = fmaf(v.w, w, x.w);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (!on) return;
+  const float y[4] = {x.x / sum, x.y / sum, x.z / sum, x.w / sum};
+  T* to = static_cast<T*>(L.o) + row.out + 4 * lane;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) to[e] = from_f32<T>(sum == 0.f ? 0.f : y[e]);
 }
 
 template <int NT, int W>
@@ -654,31 +705,54 @@ cudaError_t attn_type(const CacheAttnLaunch& L, const CacheAttnPlan& P, int form
 
 }  // namespace
 
-CacheAttnPlan plan_cache_attn(const CacheAttnArgs& L) {
+CacheAttnPlan plan_cache_attn(const CacheAttnArgs& L, int type) {
   CacheAttnPlan P = {};
   const int64_t rows = (int64_t)L.s.max_rows * L.G;
-  P.tc = rows > 64;
+  const int64_t row_tiles = (rows + 15) / 16, units16 = (int64_t)L.s.B * L.c.H * row_tiles;
+  // The tensor-core kernel pads a unit to 128 or 256 rows, this file's reads and converts the cache again for
+  // every 16 rows, which costs nothing as long as its CTAs all run at once. Rows kernel / tensor cores, us:
+  //                                              16 rows      32           48           64
+  //   128 sequences of 128, 9 heads of 64, bf16  34 / 39      57 / 39                   100 / 39
+  //   the same, fp32                             39 / 47      70 / 49      98 / 49      127 / 49
+  //   1 of 512, 4 heads of 64, fp32                           14 / 21      14 / 21      14 / 21
+  //   64 of 2048, 8 heads of 128, bf16           131 / 209    162 / 209    229 / 211    279 / 211
+  //   4 of 8192, 8 heads of 128, bf16                         49 / 68      86 / 68      88 / 70
+  //   64 of 2048, 8 heads of 128, fp32           132 / 460    234 / 467                 320 / 467 (96: 472 / 469)
+  P.tc = rows > (L.c.D > 64 ? (type == kTypeF32 ? 64 : 48) : units16 > 2 * 148 ? 16 : 64);
   P.nr = P.tc ? cache_attn_tc_rows(L.c.D) : rows > 8 ? 16 : 8;
   P.tiles = (int)((rows + P.nr - 1) / P.nr);
   P.units = (int64_t)L.s.B * L.c.H * P.tiles;
   P.splits = 1;
-  const int wave = P.tc ? (L.c.D <= 64 ? 148 * 2 : 148) : kMaxSplits;  // CTAs that run at once
-  const int64_t wide = std::min<int64_t>(wave / std::max<int64_t>(P.units, 1), L.s.max_len / 512);
+  const int wave = P.tc ? (L.c.D <= 64 ? 148 * 2 : 148) : P.nr == 16 ? 148 * 2 : kMaxSplits;  // CTAs that run at once
+  // CTAs for each unit in one wave, each left with some tokens of the longest sequence
+  const int64_t wide = std::min<int64_t>(wave / std::max<int64_t>(P.units, 1), L.s.max_len / (P.tc ? 256 : 512));
   if (P.tc) {
-    // fewer units than run at once, each with many tiles of tokens: split them
-    if (wide >= 2) P.splits = (int)wide;
+    // Split units of many tiles, joined by a second launch (us whole / split):
+    //   4 units of 2048 tokens, D 64: 41 / 23      18 of 1024, D 64: 31 / 25       18 of 512: 20 / 21
+    //   72 of 1024, D 64: 27 / 29                  64 of 4096, D 128: 102 / 74     16 of 8192, D 128: 180 / 49
+    if (wide >= 2 && L.s.max_len >= 1024) P.splits = (int)wide;
+  } else if (wide >= 20 && L.s.max_len > 16 * 2048) {
+    // Without clusters: one wave, each CTA left with 512 tokens. Worth the second launch where 16 CTAs a unit
+    // would have more than 2048 tokens each (8 units, 16 CTAs / one wave: 32768 tokens 35 / 35 us, 131072 97 / 74).
+    P.splits = (int)wide;
   } else {
-    // CTAs of a cluster that split one unit: about a wave of four CTAs per SM, as long as each is left with
-    // 128 tokens of the longest sequence, and up to two waves, for sequences of unlike length to even
-    // out, while each is left with 1024
+    // CTAs of a cluster that split one unit: as many as run at once while each is left with 128 tokens of the
+    // longest sequence; and up to 8 for two to three waves, for sequences of unlike length to even out, while
+    // each is left with 2048. us by cluster size:
+    //                                    1     2     4     8     16
+    //   4 units of 2048 tokens           27    21    16    14    12
+    //   66 of up to 1511                 23    20    16    23    35
+    //   32 of 8192                       78    47    33    27    36
+    //   128 of up to 8192                80    56    53    59    84
+    //   512 of up to 8192                152   135   135   170   279
+    //   2048 of up to 2048               128   162   223   381   780
+    // (Of the row tiles only those of `rows` rows exist, half a tile a sequence more for the ragged ends.)
+    const int64_t tiles = std::min<int64_t>((int64_t)L.s.B * P.tiles, (L.s.rows * L.G + (int64_t)L.s.B * P.nr / 2) / P.nr);
     while (P.splits < 16) {
-      const int64_t ctas = P.units * P.splits * 2, tokens = L.s.max_len / (P.splits * 2);
-      if (!(ctas <= 148 * 4 && tokens >= 128) && !(ctas <= 148 * 16 && tokens >= 1024)) break;
+      const int64_t ctas = tiles * L.c.H * P.splits * 2, tokens = L.s.max_len / (P.splits * 2);
+      if (!(ctas <= wave && tokens >= 128) && !(ctas <= 148 * 8 && tokens >= 2048 && P.splits < 8)) break;
       P.splits *= 2;
     }
-    // Without clusters: one wave of three CTAs per SM, each left with 512 tokens. Worth the second
-    // launch where it is well over 16 CTAs a unit.
-    if (wide >= 20) P.splits = (int)wide;
   }
   if (P.splits > (P.tc ? 1 : 16)) P.ws_bytes = (size_t)(P.units * P.splits * P.nr) * (L.c.D * sizeof(float) + sizeof(float2));
   return P;
@@ -691,11 +765,11 @@ cudaError_t launch_cache_attn(const CacheAttnLaunch& L, const CacheAttnPlan& P, 
                   : type == kTypeF16 ? attn_type<__half>(L, P, format, s)
                                      : attn_type<__nv_bfloat16>(L, P, format, s);
   if (e != cudaSuccess || !P.ws_bytes) return e;
-  const dim3 grid((unsigned)P.units, (unsigned)std::min<int64_t>((int64_t)L.s.max_rows * L.G, P.nr));
+  const unsigned rows = (unsigned)std::min<int64_t>((int64_t)L.s.max_rows * L.G, P.nr);
   const CacheAttnArgs& A = L;
-  if (type == kTypeF32) cache_attn_join<float><<<grid, 256, 0, s>>>(A, P.tiles, P.nr, P.tc);
-  else if (type == kTypeF16) cache_attn_join<__half><<<grid, 256, 0, s>>>(A, P.tiles, P.nr, P.tc);
-  else cache_attn_join<__nv_bfloat16><<<grid, 256, 0, s>>>(A, P.tiles, P.nr, P.tc);
+  auto join = P.tc ? (type == kTypeF32 ? cache_attn_join_rows<float> : type == kTypeF16 ? cache_attn_join_rows<__half> : cache_attn_join_rows<__nv_bfloat16>)
+                   : (type == kTypeF32 ? cache_attn_join<float> : type == kTypeF16 ? cache_attn_join<__half> : cache_attn_join<__nv_bfloat16>);
+  join<<<dim3((unsigned)P.units, P.tc ? (rows + 7) / 8 : rows), 256, 0, s>>>(A, P.tiles, P.nr);
   return cudaGetLastError();
 }
 const char* cache_attn_name(const CacheAttnPlan& P, int type) {

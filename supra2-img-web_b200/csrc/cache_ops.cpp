@@ -462,7 +462,7 @@ int flush_cache(supra_attn_ctx* c) {
         CacheAttnLaunch L;
         static_cast<CacheAttnArgs&>(L) = call.attn;
         L.status = c->d_status;
-        const CacheAttnPlan plan = plan_cache_attn(L);
+        const CacheAttnPlan plan = plan_cache_attn(L, call.type);
         name = cache_attn_name(plan, call.type);
         const int64_t tokens = ((int64_t)L.c.blocks * L.c.H) << L.c.log2t;
         const int cols = cache_attn_box_cols(L.c.D), rows = cache_attn_box_rows(L.c.log2t, plan.tc);

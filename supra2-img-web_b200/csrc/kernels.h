@@ -398,7 +398,7 @@ struct CacheAttnPlan {
   int splits;
   size_t ws_bytes;   // workspace: parts of O (units * splits * nr * D floats), then (m, l) of each row
 };
-CacheAttnPlan plan_cache_attn(const CacheAttnArgs& L);
+CacheAttnPlan plan_cache_attn(const CacheAttnArgs& L, int type);
 cudaError_t launch_cache_attn(const CacheAttnLaunch& L, const CacheAttnPlan& P, int type, int format, cudaStream_t s);
 const char* cache_attn_name(const CacheAttnPlan& P, int type);
 // cache_attn_tc.cu, and the rows of its row tiles
