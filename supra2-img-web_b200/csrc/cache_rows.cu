@@ -215,11 +215,13 @@ int touched(const CacheSeqs& s, int log2t) { return (int)((s.max_rows + 2ll * (1
 template <typename T, int FMT, bool VEC>
 cudaError_t write_as(const CacheRowsLaunch& L, cudaStream_t s) {
   const int nblk = touched(L.s, L.c.log2t);
-  // As many threads as there are pieces, up to 128 (256 where a thread would hold more than 8 pieces): whole
-  // rows of pieces, the last warp filled up. What a warp does besides its pieces is worth four of them.
+  // 128 threads: 64 where each would hold one piece (what a warp does besides its pieces is worth four of them),
+  // 256 where each would hold more than 8; whole rows of pieces, the last warp filled up. 20000 rows, us with 64 /
+  // 128 / 256 threads: blocks of 16 x 64 bf16 (128 pieces) 27 / 35 / 35, 128 x 64 bf16 (1024) 23 / 21 / 23, 64 x 128
+  // bf16 (1024) 41 / 33 / 39, 64 x 128 fp32 (2048) - / 53 / 47.
   constexpr int V = 16 / (int)sizeof(T);
   const int per_row = L.c.D / V, tokens = 1 << L.c.log2t;
-  int rows = std::min(tokens, 128 / per_row);
+  int rows = std::min(tokens, (tokens * per_row <= 128 ? 64 : 128) / per_row);
   if ((tokens + rows - 1) / rows > 8) rows = std::min(tokens, 256 / per_row);
   const int nv = (tokens + rows - 1) / rows;
   const int threads = (rows * per_row + 31) / 32 * 32;
