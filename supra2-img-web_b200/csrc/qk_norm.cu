@@ -28,7 +28,7 @@ __device__ __forceinline__ const float* turns_of(const QkNormLaunch& L, int64_t 
 // rotation, 1 pairs half a rotation apart, 2 neighbours.
 template <typename T, int LPH, int ROT>
 __global__ void __launch_bounds__(128) qk_norm_vec(const __grid_constant__ QkNormLaunch L, int wpr) {
-  constexpr int V = 16 / (int)sizeof(T);
+  constexpr int V = 16 / (int)sizeof(T), V2 = V / 2;
   constexpr int UNROLL = 4;
   const int lane = threadIdx.x & 31, g = lane / LPH, l = lane % LPH;
   const uint32_t w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -41,27 +41,40 @@ __global__ void __launch_bounds__(128) qk_norm_vec(const __grid_constant__ QkNor
   const bool on = e0 < L.D;             // lanes past the head only take part in the shuffles
   const int half = L.rot >> 1;
   const bool turn = ROT != 0 && on && e0 < L.rot;
-  // Pairs half a rotation apart: the partner piece is in the lane `peer`, and this lane's results are
-  // n cos -+ partner sin.
+  // Pairs half a rotation apart: the partner piece is in the lane `peer`.
   const bool second = ROT == 1 && e0 >= half;
-  const int peer = ROT == 1 && turn ? g * LPH + (second ? e0 - half : e0 + half) / V : lane;
-  constexpr int NC = ROT == 2 ? V / 2 : V;  // cosines of a lane
-  float co[NC], si[NC], wq[V], wk[V];
+  const int pe = ROT == 1 && turn ? (second ? e0 - half : e0 + half) : e0;  // the partner piece's first channel
+  const int peer = g * LPH + pe / V;
+  // y_i = r (x_i a_i + partner_i s_i): the weights folded into the row's cosines and sines, for the queries or
+  // the keys, whichever the lane's head is
+  float2 a[V2], s[V2];
+  auto fold = [&](const float* wt) {
+    float co[V], si[V], wi[V], wp[V];
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    co[i] = 1.f, si[i] = 0.f;
+    for (int i = 0; i < V; ++i) co[i] = wi[i] = wp[i] = 1.f, si[i] = 0.f;
+    if (on && wt) load_row<float, V, true>(wt + e0, wi);
     if (turn) {
-      const int p = ROT == 2 ? (e0 >> 1) + i : (second ? e0 - half : e0) + i;
-      co[i] = turns[p];
-      si[i] = turns[half + p];
-      if (ROT == 1 && !second) si[i] = -si[i];
-    }
-  }
+      if constexpr (ROT == 1) {
+        if (wt) load_row<float, V, true>(wt + pe, wp);
+        load_row<float, V, true>(turns + (second ? pe : e0), co);
+        load_row<float, V, true>(turns + half + (second ? pe : e0), si);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    wq[i] = on && L.q.w ? L.q.w[e0 + i] : 1.f;
-    wk[i] = on && L.k.w ? L.k.w[e0 + i] : 1.f;
-  }
+        for (int i = 0; i < V; ++i) si[i] = second ? si[i] : -si[i];
+      } else if constexpr (ROT == 2) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          co[i] = turns[(e0 + i) >> 1];
+          si[i] = (i & 1) ? turns[half + ((e0 + i) >> 1)] : -turns[half + ((e0 + i) >> 1)];
+          wp[i] = wi[i ^ 1];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V2; ++i) {
+      a[i] = make_float2(co[2 * i] * wi[2 * i], co[2 * i + 1] * wi[2 * i + 1]);
+      s[i] = make_float2(si[2 * i] * wp[2 * i], si[2 * i + 1] * wp[2 * i + 1]);
+    }
+  };
   const int Hq = L.q.H, heads = Hq + L.k.H;
   const int step = wpr * (32 / LPH);
   const float inv_d = 1.f / (float)L.D;
@@ -70,51 +83,63 @@ __global__ void __launch_bounds__(128) qk_norm_vec(const __grid_constant__ QkNor
   const T* xk = static_cast<const T*>(L.k.x) + (int64_t)row * L.k.ldx + e0 - Hq * L.D;
   T* yq = static_cast<T*>(L.q.y) + (int64_t)row * L.q.ldy + e0;
   T* yk = static_cast<T*>(L.k.y) + (int64_t)row * L.k.ldy + e0 - Hq * L.D;
+  int have = -1;  // whose weights are folded in: 0 the queries', 1 the keys'
   // (whole warps stay in the loop: the shuffles need every lane)
   for (int base = part * (32 / LPH); base < heads; base += step * UNROLL) {
-    float x[UNROLL][V];
+    uint4 raw[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const int h = base + u * step + g;
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[u][i] = 0.f;
-      if (on && h < heads) load_row<T, V, true>((h < Hq ? xq : xk) + h * L.D, x[u]);
+      raw[u] = make_uint4(0, 0, 0, 0);
+      if (on && h < heads) raw[u] = *reinterpret_cast<const uint4*>((h < Hq ? xq : xk) + h * L.D);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       if (base + u * step >= heads) break;  // uniform over the warp
       const int h = base + u * step + g;
-      const bool key = h >= Hq;
+      const int key = h >= Hq;
+      if (key != have) {
+        if (have < 0 || L.q.w != L.k.w) fold(key ? L.k.w : L.q.w);
+        have = key;
+      }
+      auto pairs = [](const uint4& r, float2 (&x)[V2]) {
+        const uint32_t u4[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < V2; ++i) {
+          if constexpr (V == 4) x[i] = make_float2(__uint_as_float(u4[2 * i]), __uint_as_float(u4[2 * i + 1]));
+          else x[i] = unpack2<T>(u4[i]);
+        }
+      };
+      float2 x[V2], o[V2];
+      pairs(raw[u], x);
+      float r = 1.f;
       if (L.norm) {
-        float ss = 0.f;
+        float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < V; ++i) ss = fmaf(x[u][i], x[u][i], ss);
+        for (int i = 0; i < V2; ++i) ss = __ffma2_rn(x[i], x[i], ss);
+        float sum = ss.x + ss.y;
 #pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float r = rsqrtf(fmaf(ss, inv_d, L.eps));
+        for (int d = LPH / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        r = rsqrtf(fmaf(sum, inv_d, L.eps));
+      }
+      // partners as they were read (a channel that does not turn has none: 0, lest it meet an infinity)
+      if constexpr (ROT == 1) {
+        uint4 p;
+        p.x = __shfl_sync(0xffffffffu, raw[u].x, peer), p.y = __shfl_sync(0xffffffffu, raw[u].y, peer);
+        p.z = __shfl_sync(0xffffffffu, raw[u].z, peer), p.w = __shfl_sync(0xffffffffu, raw[u].w, peer);
+        if (!turn) p = make_uint4(0, 0, 0, 0);
+        pairs(p, o);
+      } else if constexpr (ROT == 2) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[u][i] = x[u][i] * r * (key ? wk[i] : wq[i]);
+        for (int i = 0; i < V2; ++i) o[i] = turn ? make_float2(x[i].y, x[i].x) : make_float2(0.f, 0.f);
       }
       float y[V];
-      if constexpr (ROT == 1) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float other = __shfl_sync(0xffffffffu, x[u][i], peer);
-          y[i] = turn ? fmaf(x[u][i], co[i], other * si[i]) : x[u][i];
-        }
-      } else if constexpr (ROT == 2) {  // (lanes that do not turn have cosine 1 and sine 0)
-#pragma unroll
-        for (int i = 0; i < V; i += 2) {
-          y[i] = fmaf(x[u][i], co[i / 2], -(x[u][i + 1] * si[i / 2]));
-          y[i + 1] = fmaf(x[u][i + 1], co[i / 2], x[u][i] * si[i / 2]);
-        }
-        if (!turn) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) y[i] = x[u][i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = x[u][i];
+      for (int i = 0; i < V2; ++i) {
+        float2 n = __fmul2_rn(x[i], a[i]);
+        if constexpr (ROT != 0) n = __ffma2_rn(o[i], s[i], n);
+        n = __fmul2_rn(n, make_float2(r, r));
+        y[2 * i] = n.x, y[2 * i + 1] = n.y;
       }
       if (on && h < heads) store_row<T, V, true>((key ? yk : yq) + h * L.D, y);
     }
