@@ -6,9 +6,10 @@
 // row's cosines and sines in registers (1 / sqrt is rsqrtf, 2 ulp; a correctly rounded root and division a
 // head made the kernel issue-bound). Pieces stay as they were read until their turn comes, and products
 // are formed two at a time: fewer instructions, and registers for more warps (the bf16 case below took 108 us
-// with channels unpacked at once and weights apart). Every lane stores only pieces that it loaded itself, so in-place calls need no ordering. The scalar form
-// (sizes and alignments that do not split into 16-byte pieces) gives a head to a warp.
-// Measured: 16384 rows of 9 + 9 heads of 64, fp32: 31 us, 4.9 TB/s (scalar form 121); 16384 rows of 32 + 8 heads
+// with channels unpacked at once and weights apart). Every lane stores only pieces that it loaded itself,
+// so in-place calls need no ordering. The scalar form (sizes and alignments that do not split into 16-byte
+// pieces) gives a head to a warp.
+// Measured: 16384 rows of 9 + 9 heads of 64, fp32: 30 us, 5.0 TB/s (scalar form 121); 16384 rows of 32 + 8 heads
 // of 128, bf16: 68 us, 5.0 TB/s (scalar form 338); 61 rows: 8 us, the launch.
 #include "cache.cuh"
 
