@@ -233,8 +233,7 @@ int check_qk_norm(supra_attn_ctx* c, const supra_attn_qk_norm_desc* d, Checked* 
   QkOperand* to[2] = {&L.q, &L.k};
   const char* xn[2] = {"q", "k"};
   const char* yn[2] = {"the q output", "the k output"};
-  bool vec = (d->D * es) % 16 == 0 && (d->flags & SUPRA_ATTN_QK_INTERLEAVED ? d->rot : d->rot / 2) % (16 / es) == 0 &&
-             (d->rot == 0 || !misaligned(d->turns, 16));
+  bool vec = (d->D * es) % 16 == 0;
   for (int i = 0; i < 2; ++i) {
     const supra_attn_qk_operand& o = *op[i];
     if (o.H == 0) continue;

@@ -324,8 +324,7 @@ struct QkNormLaunch {
   int32_t norm, interleaved;
   int32_t* status;
 };
-// vec: every head row starts on a 16-byte boundary and D, rot / 2 (or rot, interleaved) split into
-// 16-byte pieces
+// vec: every head row and the weights start on a 16-byte boundary and D splits into 16-byte pieces
 cudaError_t launch_qk_norm(const QkNormLaunch& L, int type, bool vec, cudaStream_t s);
 
 // The cache's pool and the sequences of a call as the kernels see them.

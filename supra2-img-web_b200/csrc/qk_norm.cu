@@ -8,7 +8,9 @@
 // are formed two at a time: fewer instructions, and registers for more warps (the bf16 case below took 108 us
 // with channels unpacked at once and weights apart). Every lane stores only pieces that it loaded itself,
 // so in-place calls need no ordering. The scalar form (sizes and alignments that do not split into 16-byte
-// pieces) gives a head to a warp.
+// pieces) gives a head to a warp. Rotations that end inside a piece or pair channels of unlike places in
+// theirs stay in the vector form, partners through shared memory (16384 rows of 9 + 9 heads of 64, 50 channels
+// turned, bf16: 41 us, neighbours 31; scalar form 119 and 127).
 // Measured: 16384 rows of 9 + 9 heads of 64, fp32: 30 us, 5.0 TB/s (scalar form 121); 16384 rows of 32 + 8 heads
 // of 128, bf16: 68 us, 5.0 TB/s (scalar form 338); 61 rows: 8 us, the launch.
 #include "cache.cuh"
@@ -30,7 +32,8 @@ __device__ __forceinline__ const float* turns_of(const QkNormLaunch& L, int64_t 
 }
 
 // LPH lanes per head (a power of two), V elements per lane; `wpr` warps share a row's heads. ROT: 0 no
-// rotation, 1 pairs half a rotation apart, 2 neighbours.
+// rotation, 1 pairs half a rotation apart, 2 neighbours, 3 pairs half a rotation apart where that is not whole
+// pieces (or the table is not aligned): partners by their channels, through shared memory.
 template <typename T, int LPH, int ROT>
 __global__ void __launch_bounds__(128) qk_norm_vec(const __grid_constant__ QkNormLaunch L, int wpr) {
   constexpr int V = 16 / (int)sizeof(T), V2 = V / 2;
@@ -45,7 +48,9 @@ __global__ void __launch_bounds__(128) qk_norm_vec(const __grid_constant__ QkNor
   const int e0 = l * V;                 // the lane's first channel
   const bool on = e0 < L.D;             // lanes past the head only take part in the shuffles
   const int half = L.rot >> 1;
-  const bool turn = ROT != 0 && on && e0 < L.rot;
+  const bool turn = ROT != 0 && on && e0 < L.rot;  // (with 2 and 3 perhaps only the first channels)
+  __shared__ uint4 own[ROT == 3 ? 4 : 1][32];
+  auto partner = [&](int e) { return e < half ? e + half : e - half; };  // of channel e < rot
   // Pairs half a rotation apart: the partner piece is in the lane `peer`.
   const bool second = ROT == 1 && e0 >= half;
   const int pe = ROT == 1 && turn ? (second ? e0 - half : e0 + half) : e0;  // the partner piece's first channel
@@ -68,9 +73,20 @@ __global__ void __launch_bounds__(128) qk_norm_vec(const __grid_constant__ QkNor
       } else if constexpr (ROT == 2) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
+          if (e0 + i >= L.rot) break;
           co[i] = turns[(e0 + i) >> 1];
           si[i] = (i & 1) ? turns[half + ((e0 + i) >> 1)] : -turns[half + ((e0 + i) >> 1)];
           wp[i] = wi[i ^ 1];
+        }
+      } else if constexpr (ROT == 3) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int e = e0 + i;
+          if (e >= L.rot) break;
+          const bool first = e < half;
+          co[i] = turns[first ? e : e - half];
+          si[i] = first ? -turns[half + e] : turns[e];
+          if (wt) wp[i] = wt[partner(e)];
         }
       }
     }
@@ -136,7 +152,19 @@ __global__ void __launch_bounds__(128) qk_norm_vec(const __grid_constant__ QkNor
         pairs(p, o);
       } else if constexpr (ROT == 2) {
 #pragma unroll
-        for (int i = 0; i < V2; ++i) o[i] = turn ? make_float2(x[i].y, x[i].x) : make_float2(0.f, 0.f);
+        for (int i = 0; i < V2; ++i) o[i] = on && e0 + 2 * i < L.rot ? make_float2(x[i].y, x[i].x) : make_float2(0.f, 0.f);
+      } else if constexpr (ROT == 3) {
+        uint4* mine = own[threadIdx.x >> 5];
+        mine[lane] = raw[u];
+        __syncwarp();
+        const T* head = reinterpret_cast<const T*>(mine + g * LPH);
+#pragma unroll
+        for (int i = 0; i < V2; ++i) {
+          const int e = e0 + 2 * i;
+          o[i].x = on && e < L.rot ? to_f32<T>(head[partner(e)]) : 0.f;
+          o[i].y = on && e + 1 < L.rot ? to_f32<T>(head[partner(e + 1)]) : 0.f;
+        }
+        __syncwarp();  // (before the next head's pieces)
       }
       float y[V];
 #pragma unroll
@@ -219,11 +247,13 @@ cudaError_t norm_as(const QkNormLaunch& L, bool vec, cudaStream_t s) {
     wpr = wpr < groups ? wpr : groups;
     const int64_t grid = (L.M * wpr + 3) / 4;
     if (grid > INT32_MAX) return cudaErrorInvalidValue;
+    const bool whole = (L.rot / 2) % (16 / (int)sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(L.turns) % 16 == 0;
 #define SUPRA_QK(N)                                                                               \
   case N:                                                                                         \
     if (L.rot == 0) qk_norm_vec<T, N, 0><<<(unsigned)grid, 128, 0, s>>>(L, (int)wpr);             \
-    else if (!L.interleaved) qk_norm_vec<T, N, 1><<<(unsigned)grid, 128, 0, s>>>(L, (int)wpr);    \
-    else qk_norm_vec<T, N, 2><<<(unsigned)grid, 128, 0, s>>>(L, (int)wpr);                        \
+    else if (L.interleaved) qk_norm_vec<T, N, 2><<<(unsigned)grid, 128, 0, s>>>(L, (int)wpr);     \
+    else if (whole) qk_norm_vec<T, N, 1><<<(unsigned)grid, 128, 0, s>>>(L, (int)wpr);             \
+    else qk_norm_vec<T, N, 3><<<(unsigned)grid, 128, 0, s>>>(L, (int)wpr);                        \
     break;
     switch (lph) {
       SUPRA_QK(1)

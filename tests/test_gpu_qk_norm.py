@@ -146,3 +146,62 @@ def test_rotation_turns(gpu):
         t[7, 8:16], np.cos(3 * 10000.0 ** (-np.arange(0, 16, 2) / 16)))
     with pytest.raises(ValueError):
         supra_attn.rotation_turns(gpu, grid, 30)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("D,rot", [(64, 50), (128, 30), (80, 36), (128, 126), (16, 4), (64, 2), (96, 94)])
+def test_rotations_that_are_not_whole_pieces(gpu, D, rot, inplace, interleaved, dtype):
+    check(gpu, dtype, 37, 5, 2, D, rot, interleaved, inplace=inplace, seed=7)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_table_that_is_not_aligned(gpu, dtype):
+    rng = np.random.default_rng(8)
+    M, H, D = 21, 3, 64
+    flat = torch.from_numpy(rng.uniform(-1, 1, 1 + 30 * D).astype(np.float32)).cuda()
+    turns = flat[1:].view(30, D)
+    x = torch.from_numpy(rng.standard_normal((M, H * D)).astype(np.float32)).to(TYPES[dtype]).cuda()
+    y = torch.empty_like(x)
+    supra_attn.qk_norm(gpu, q=x, M=M, Hq=H, D=D, qOut=y, turns=turns, rot=D)
+    gpu.sync()
+    ref, mag = oc.qk_norm(x.cpu().double().numpy().reshape(M, H, D), None, 1e-6, True, turns.cpu().numpy(), D, np.arange(M), False)
+    assert (np.abs(y.cpu().double().numpy().reshape(M, H, D) - ref) <= bound(dtype, ref, mag)).all()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("rot", [32, 10])
+def test_channels_that_do_not_turn_are_left_alone(gpu, rot, interleaved):
+    """Without a norm they come out as they went in, infinities and NaN among them."""
+    M, H, D = 9, 3, 64
+    x = torch.randn(M, H, D, device="cuda")
+    x[:, :, rot] = float("inf")
+    x[:, :, D - 1] = float("nan")
+    x[:, :, rot + 1:rot + 3] = 3e38
+    y = torch.zeros_like(x)
+    turns = supra_attn.rotation_turns(gpu, np.arange(M), rot)
+    supra_attn.qk_norm(gpu, q=x, M=M, Hq=H, D=D, qOut=y, norm=False, turns=turns, rot=rot, interleaved=interleaved)
+    gpu.sync()
+    torch.cuda.synchronize()
+    assert torch.equal(y[:, :, rot:].nan_to_num(nan=5.0), x[:, :, rot:].nan_to_num(nan=5.0))
+    assert torch.isfinite(y[:, :, :rot]).all()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_weights_of_one_operand_only(gpu, dtype):
+    rng = np.random.default_rng(9)
+    M, Hq, Hk, D = 50, 3, 3, 64  # (a warp's heads pass from the queries to the keys in the middle of a group)
+    x = torch.from_numpy(rng.standard_normal((M, (Hq + Hk) * D)).astype(np.float32)).to(TYPES[dtype]).cuda()
+    w = torch.from_numpy(rng.standard_normal(D).astype(np.float32)).cuda()
+    turns = torch.from_numpy(rng.uniform(-1, 1, (M, D)).astype(np.float32)).cuda()
+    for wq, wk in ((w, None), (None, w), (w, w)):
+        q, k = torch.empty(M, Hq * D, dtype=x.dtype, device="cuda"), torch.empty(M, Hk * D, dtype=x.dtype, device="cuda")
+        supra_attn.qk_norm(gpu, q=x, k=x, M=M, Hq=Hq, Hk=Hk, D=D, ldq=(Hq + Hk) * D, ldk=(Hq + Hk) * D, kOff=Hq * D, qOut=q, kOut=k, wq=wq, wk=wk,
+                           turns=turns, rot=D)
+        gpu.sync()
+        xn = x.cpu().double().numpy().reshape(M, Hq + Hk, D)
+        for lo, h, ww, out in ((0, Hq, wq, q), (Hq, Hk, wk, k)):
+            ref, mag = oc.qk_norm(xn[:, lo:lo + h], ww.cpu().double().numpy() if ww is not None else None, 1e-6, True, turns.cpu().numpy(), D,
+                                  np.arange(M), False)
+            assert (np.abs(out.cpu().double().numpy().reshape(M, h, D) - ref) <= bound(dtype, ref, mag)).all()
