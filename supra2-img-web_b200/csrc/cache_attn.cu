@@ -719,43 +719,55 @@ CacheAttnPlan plan_cache_attn(const CacheAttnArgs& L, int type) {
   //   128 sequences of 128, 9 heads of 64, bf16  34 / 39      57 / 39                   100 / 39
   //   the same, fp32                             39 / 47      70 / 49      98 / 49      127 / 49
   //   1 of 512, 4 heads of 64, fp32                           14 / 21      14 / 21      14 / 21
+  //   2 of up to 899, 9 heads of 32, fp16                                               (80: 16 / 21)
   //   64 of 2048, 8 heads of 128, bf16           131 / 209    162 / 209    229 / 211    279 / 211
   //   4 of 8192, 8 heads of 128, bf16                         49 / 68      86 / 68      88 / 70
   //   64 of 2048, 8 heads of 128, fp32           132 / 460    234 / 467                 320 / 467 (96: 472 / 469)
-  P.tc = rows > (L.c.D > 64 ? (type == kTypeF32 ? 64 : 48) : units16 > 2 * 148 ? 16 : 64);
+  P.tc = rows > (L.c.D > 64 ? (type == kTypeF32 ? 64 : 48) : units16 > 2 * 148 ? 16 : 128);
   P.nr = P.tc ? cache_attn_tc_rows(L.c.D) : rows > 8 ? 16 : 8;
   P.tiles = (int)((rows + P.nr - 1) / P.nr);
   P.units = (int64_t)L.s.B * L.c.H * P.tiles;
   P.splits = 1;
-  const int wave = P.tc ? (L.c.D <= 64 ? 148 * 2 : 148) : P.nr == 16 ? 148 * 2 : kMaxSplits;  // CTAs that run at once
+  const int wave = P.tc ? (L.c.D <= 64 ? 148 * 2 : 148) : kMaxSplits;  // CTAs that run at once
   // CTAs for each unit in one wave, each left with some tokens of the longest sequence
   const int64_t wide = std::min<int64_t>(wave / std::max<int64_t>(P.units, 1), L.s.max_len / (P.tc ? 256 : 512));
   if (P.tc) {
     // Split units of many tiles, joined by a second launch (us whole / split):
     //   4 units of 2048 tokens, D 64: 41 / 23      18 of 1024, D 64: 31 / 25       18 of 512: 20 / 21
     //   72 of 1024, D 64: 27 / 29                  64 of 4096, D 128: 102 / 74     16 of 8192, D 128: 180 / 49
+    // Of units that just run at once, two parts each shorten the longest sequence's way: 200 of up to 4433 tokens, D
+    // 48: 92 / 72, 126 of up to 4412, D 96: 105 / 78; 144 of 4096 each, D 64: 90 / 82. (256 units at one CTA an SM, D
+    // 128: 152 / 184.)
     if (wide >= 2 && L.s.max_len >= 1024) P.splits = (int)wide;
+    else if (P.units <= wave && L.s.max_len >= 2048) P.splits = 2;
   } else if (wide >= 20 && L.s.max_len > 16 * 2048) {
     // Without clusters: one wave, each CTA left with 512 tokens. Worth the second launch where 16 CTAs a unit
     // would have more than 2048 tokens each (8 units, 16 CTAs / one wave: 32768 tokens 35 / 35 us, 131072 97 / 74).
     P.splits = (int)wide;
   } else {
-    // CTAs of a cluster that split one unit: as many as run at once while each is left with 128 tokens of the
-    // longest sequence; and up to 8 for two to three waves, for sequences of unlike length to even out, while
-    // each is left with 2048. us by cluster size:
+    // CTAs of a cluster that split one unit: as long as all run at once (large clusters find room later than
+    // small ones) and each is left with 128 tokens of the longest sequence (256 with 16 rows a CTA, two of which
+    // share an SM); and up to 8 for two to three waves, for sequences of unlike length to even out, while each is
+    // left with 2048. us by cluster size:
     //                                    1     2     4     8     16
     //   4 units of 2048 tokens           27    21    16    14    12
-    //   66 of up to 1511                 23    20    16    23    35
+    //   22 of up to 2661                 29    20    16    14
     //   32 of 8192                       78    47    33    27    36
-    //   128 of up to 8192                80    56    53    59    84
+    //   55 of up to 1519                 23    18    14    18
+    //   90 of up to 4945                 43    29    23    25
+    //   210 of up to 3567                37    27    29    39
     //   512 of up to 8192                152   135   135   170   279
     //   2048 of up to 2048               128   162   223   381   780
-    // (Of the row tiles only those of `rows` rows exist, half a tile a sequence more for the ragged ends.)
-    const int64_t tiles = std::min<int64_t>((int64_t)L.s.B * P.tiles, (L.s.rows * L.G + (int64_t)L.s.B * P.nr / 2) / P.nr);
+    // (Of the row tiles only those of `rows` rows exist: one a sequence, or half a one more for ragged ends.)
+    const int64_t tiles = std::min<int64_t>((int64_t)L.s.B * P.tiles,
+                                            std::max<int64_t>(L.s.B, (L.s.rows * L.G + (int64_t)L.s.B * P.nr / 2) / P.nr));
+    const int least = P.nr == 16 ? 256 : 128;
     while (P.splits < 16) {
-      const int64_t ctas = tiles * L.c.H * P.splits * 2, tokens = L.s.max_len / (P.splits * 2);
-      if (!(ctas <= wave && tokens >= 128) && !(ctas <= 148 * 8 && tokens >= 2048 && P.splits < 8)) break;
-      P.splits *= 2;
+      const int next = P.splits * 2;
+      const int64_t ctas = tiles * L.c.H * next, tokens = L.s.max_len / next;
+      const int room = P.nr == 16 || next > 4 ? 2 * 148 : kMaxSplits;
+      if (!(ctas <= room && tokens >= least) && !(ctas <= 148 * 8 && tokens >= 2048 && next <= 8)) break;
+      P.splits = next;
     }
   }
   if (P.splits > (P.tc ? 1 : 16)) P.ws_bytes = (size_t)(P.units * P.splits * P.nr) * (L.c.D * sizeof(float) + sizeof(float2));
