@@ -376,6 +376,48 @@ def test_captured_split_over_many_ctas(gpu):
     ctx.close()
 
 
+@pytest.mark.parametrize("fmt,dtype,rows", [("int8", "fp32", 1), ("e4m3", "bf16", 40)])
+def test_blocks_past_four_gib(gpu, fmt, dtype, rows):
+    """Blocks at the end of a pool of more than 2^32 bytes (and, with strides of their own, rows past 2^31 elements)
+    give what the same blocks give in a small pool."""
+    T, H, D, G, n = 64, 2, 128, 2, 200
+    per = T * H * D
+    big = (1 << 32) // per + 40
+    dt = TYPES[dtype]
+    rng = np.random.default_rng(30)
+    k = torch.from_numpy(rng.standard_normal((n, H * D)).astype(np.float32)).to(dt).cuda()
+    v = torch.from_numpy(rng.standard_normal((n, H * D)).astype(np.float32)).to(dt).cuda()
+    q = torch.from_numpy(rng.standard_normal((rows, H * G * D)).astype(np.float32)).to(dt).cuda()
+    ln = torch.tensor([n], dtype=torch.int32, device="cuda")
+    ld = (1 << 31) // (n - 1) + 16 - ((1 << 31) // (n - 1)) % 16  # the last row starts past 2^31
+    far = torch.zeros((n - 1) * ld + H * D, dtype=dt, device="cuda")
+    got = []
+    for blocks, first in ((8, 2), (big, big - 4)):
+        cache = supra_attn.KVCache(gpu, blocks, H, D, block_tokens=T, format=fmt)
+        table = torch.arange(first, first + 4, dtype=torch.int32, device="cuda").flip(0).contiguous().view(1, 4)
+        new = supra_attn.CacheBatch(gpu, ln, table, max_rows=n)
+        if first == 2:
+            supra_attn.cache_write(gpu, cache, new, k=k, v=v)
+        else:  # from rows far apart
+            far.as_strided((n, H * D), (ld, 1)).copy_(k)
+            torch.cuda.synchronize()
+            supra_attn.cache_write(gpu, cache, new, k=far, v=v, ldk=ld)
+            gpu.sync()
+            far.zero_()
+        out, kr, vr = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+        torch.cuda.synchronize()
+        supra_attn.cache_attention(gpu, cache, supra_attn.CacheBatch(gpu, ln, table, max_rows=rows), q=q, H=H * G, out=out, causal=True)
+        if first == 2:
+            supra_attn.cache_read(gpu, cache, new, k=kr, v=vr)
+        else:
+            supra_attn.cache_read(gpu, cache, new, k=far, v=vr, ldk=ld)
+        gpu.sync()
+        got.append((out, far.as_strided((n, H * D), (ld, 1)).clone() if first != 2 else kr, vr))
+        cache.release()
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and a.abs().max() > 0
+
+
 def test_first_call_of_a_context_may_be_a_captured_one(gpu):
     """Nothing of a context has been set up yet when its first call, one with a workspace, is captured."""
     p = Pool(gpu, np.random.default_rng(23), "int8", 128, 1, 64, [12000])
