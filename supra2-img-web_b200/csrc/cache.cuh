@@ -186,6 +186,12 @@ __device__ __forceinline__ bool mbar_wait_clocked(uint64_t* bar, uint32_t parity
   }
 }
 
+// ---- a launch and the one that joins its parts ---------------------------------------------------
+// The join's CTAs may be placed once every CTA of the parts' launch has said so or ended, and wait until that
+// launch has ended and its writes can be seen.
+__device__ __forceinline__ void join_may_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void parts_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- sequences ---------------------------------------------------------------------------------
 struct SeqView {
   int64_t row0;  // first row of the operands

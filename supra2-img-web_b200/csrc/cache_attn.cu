@@ -25,7 +25,8 @@
 //
 // Measured: 64 sequences of 1000 to 8000 tokens, 8 heads of 128, 4 query heads each, E4M3 and bf16: 118 us, 5.0 TB/s (77 %
 // of the copy rate; what is missing is the first loads of each CTA, three of which share an SM, and the last
-// wave); one sequence of 131072 tokens, INT8 and fp16: 50 us, 5.4 TB/s, and 7 for the join.
+// wave); one sequence of 131072 tokens, INT8 and fp16: 54 us, 5.0 TB/s (49 for the
+// parts, 5.5 TB/s; the join, placed while they are formed, the rest: 57 in all when it was an ordinary launch).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -140,6 +141,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   cg::cluster_group cluster = cg::this_cluster();
+  if (L.ws_o) join_may_start();
   const int csize = L.splits, crank = blockIdx.x % csize;  // (the rank in the cluster, where there is one)
 
   // unit = (sequence, cache head, row tile); the whole cluster has the same one
@@ -566,8 +568,19 @@ __global__ void __launch_bounds__(256) cache_attn_join(const __grid_constant__ C
   const CachePool& c = L.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   JoinRow row;
-  if (!join_row(L, tiles, NR, false, blockIdx.x, blockIdx.y, row)) return;
+  const bool there = join_row(L, tiles, NR, false, blockIdx.x, blockIdx.y, row);  // (reads what no launch of ours writes)
+  parts_done();
+  if (!there) return;
   const int64_t part0 = row.part0;
+  const int per = c.D / 4, groups = 256 / per;
+  const int g = threadIdx.x / per, e = (threadIdx.x - g * per) * 4;
+  auto part_of = [&](int s) { return *reinterpret_cast<const float4*>(L.ws_o + (part0 + (int64_t)s * NR) * c.D + e); };
+  float4 first[8];  // under way while the weights are worked out
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int s = g + k * groups;
+    first[k] = g < groups && s < L.splits ? part_of(s) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   float mx = -INFINITY, m[2], l[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -597,16 +610,16 @@ __global__ void __launch_bounds__(256) cache_attn_join(const __grid_constant__ C
   sum = 0.f;
 #pragma unroll
   for (int w = 0; w < 8; ++w) sum += red[8 + w];
-  const int per = c.D / 4, groups = 256 / per;
-  const int g = threadIdx.x / per, e = (threadIdx.x - g * per) * 4;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   if (g < groups) {
-#pragma unroll 8
-    for (int s = g; s < L.splits; s += groups) {
-      const float4 v = *reinterpret_cast<const float4*>(L.ws_o + (part0 + (int64_t)s * NR) * c.D + e);
-      const float f = wt[s];
+    auto add = [&](const float4& v, float f) {
       x.x = fmaf(v.x, f, x.x), x.y = fmaf(v.y, f, x.y), x.z = fmaf(v.z, f, x.z), x.w = fmaf(v.w, f, x.w);
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (g + k * groups < L.splits) add(first[k], wt[g + k * groups]);
+#pragma unroll 8
+    for (int s = g + 8 * groups; s < L.splits; s += groups) add(part_of(s), wt[s]);
   }
   po[threadIdx.x] = x;
   __syncthreads();
@@ -623,7 +636,9 @@ __global__ void __launch_bounds__(256) cache_attn_join_rows(const __grid_constan
   const CachePool& c = L.c;
   const int lane = threadIdx.x & 31;
   JoinRow row;
-  if (!join_row(L, tiles, NR, true, blockIdx.x, blockIdx.y * 8 + (threadIdx.x >> 5), row)) return;  // (whole warps)
+  const bool there = join_row(L, tiles, NR, true, blockIdx.x, blockIdx.y * 8 + (threadIdx.x >> 5), row);  // (of whole warps)
+  parts_done();
+  if (!there) return;
   auto part = [&](int s) { return s < L.splits ? L.ws_ml[row.part0 + (int64_t)s * NR] : make_float2(-INFINITY, 0.f); };
   float mx = -INFINITY;
   for (int s0 = 0; s0 < L.splits; s0 += 32) mx = fmaxf(mx, part(s0 + lane).x);
@@ -785,8 +800,17 @@ cudaError_t launch_cache_attn(const CacheAttnLaunch& L, const CacheAttnPlan& P, 
   const CacheAttnArgs& A = L;
   auto join = P.tc ? (type == kTypeF32 ? cache_attn_join_rows<float> : type == kTypeF16 ? cache_attn_join_rows<__half> : cache_attn_join_rows<__nv_bfloat16>)
                    : (type == kTypeF32 ? cache_attn_join<float> : type == kTypeF16 ? cache_attn_join<__half> : cache_attn_join<__nv_bfloat16>);
-  join<<<dim3((unsigned)P.units, P.tc ? (rows + 7) / 8 : rows), 256, 0, s>>>(A, P.tiles, P.nr);
-  return cudaGetLastError();
+  // launched while the parts are still being formed: its CTAs wait for the whole of that launch (parts_done)
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)P.units, P.tc ? (rows + 7) / 8 : rows);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join, A, P.tiles, P.nr);
 }
 const char* cache_attn_name(const CacheAttnPlan& P, int type) {
   if (P.tc) return type == kTypeF32 ? "cache_attention_tc_fp32" : "cache_attention_tc";

@@ -214,6 +214,7 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
   const CachePool& c = L.c;
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;  // (uniform)
 
+  if (L.ws_o) join_may_start();
   // unit = (row tile, sequence, cache head), the longest causal row tiles first; the CTAs that split a
   // unit's tokens are neighbours
   const int unit = blockIdx.x / L.splits, split = blockIdx.x % L.splits;
