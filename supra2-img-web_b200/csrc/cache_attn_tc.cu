@@ -26,7 +26,7 @@
 // ones, and its last product behind them, so that neither MMA nor conversion is waited for. What bounds
 // the kernel is the softmax: 16 exponentials per cycle and SM, and about five instructions a score.
 // Measured: 4 causal chunks of 700 to 1024 rows over 2049 to 4096 tokens, 16 heads of 128, 4 cache heads, INT8 and bf16:
-// 144 us, 525 TFLOP/s; 128 prompts of 1 to 128 tokens, 256 rows each, 9 heads of 64, INT8 and fp32 rows: 90 us,
+// 146 us, 517 TFLOP/s; 128 prompts of 1 to 128 tokens, 256 rows each, 9 heads of 64, INT8 and fp32 rows: 90 us,
 // 1.8 TB/s (a CTA has two tiles at most; its q, its output and the latencies between take the time). A fourth
 // converter warp did not change the first.
 // Every wait is bounded; on a timeout the CTA records the failure, waits for its own copies and MMAs, frees its
