@@ -12,7 +12,11 @@
 // converter warps turn the raw bytes, which the TMA unit brings in block by block, into the swizzled
 // operand tiles, once for all rows of the CTA. P carries the V scale as an exponent, which costs nothing
 // per score, and m follows the product of both, so each row's P is as large as fp16 allows whatever the
-// scales of the blocks that it sees; only the sum divides the scale out again, once per 16 tokens.
+// scales of the blocks that it sees; only the sum divides the scale out again, once per 16 tokens. That holds
+// while V scales are within 2^32 of 1: P of a token whose score is within 2^-69 of the row's largest is then above
+// 2^-126, and the sum, in units of 2^m, within the range of 32 bits. Tiles with others (blocks of zeros have
+// 2^-107) are odd ones: their sum is formed from exponentials of its own, in units of 2^(m - d), with d the whole
+// number that keeps m - d near the row's largest score alone; warps with a row whose d is not 0 stay with that form.
 // q carries a power of two per row (cache_attn.cu).
 // 16-bit rows keep O in TMEM, where m moves only when a tile exceeds it by 2^8 (then the softmax threads
 // rescale O there). fp32 rows use two fp16 parts of q and p (each product two MMAs), move m exactly, and
@@ -46,8 +50,12 @@ constexpr int kN = 64;   // tokens of a tile
 template <bool SPLIT>
 constexpr float kPShift = SPLIT ? 15.f : 7.f;
 constexpr float kLag = 8.f;
-constexpr float kScaleFloor = 7.7037197775489434e-34f;  // 2^-110, below any scale that a write makes
-constexpr int kMeta = 8;  // tiles whose scales are kept at once
+constexpr float kScaleMin = 2.3283064365386963e-10f, kScaleMax = 4294967296.f;  // 2^-32, 2^32: V scales of common tiles
+constexpr float kNear = 32.f;   // d is 0 where m is within this of the row's largest score
+constexpr float kSlack = 16.f;  // elsewhere m - d is
+// Tiles whose scales are kept at once: while the converters have tile i, the softmax threads are past tile i - 4 (tile
+// i - 2 has its scores, for which product i - 4 was waited for), and tiles i + 2 .. i + 9 are described together.
+constexpr int kMeta = 13;
 
 template <int DT, bool SPLIT>
 struct Cfg {
@@ -85,12 +93,13 @@ struct Cfg {
 
 struct TileMeta {  // of a tile's four 16-token groups
   float ks[4];
-  float lv[4];   // log2 |v_scale|
+  float lv[4];   // log2 |v_scale|; where |v_scale| is outside [kScaleMin, kScaleMax], without its whole part
   float iv[4];   // 1 / |v_scale|
   int32_t dead;  // groups whose block does not exist (bits), tokens past the end not among them
   int32_t neg;   // groups with a negative V scale (bits), which no write makes
-  int32_t odd;   // groups that are dead, or a scale of theirs is negative, not finite, or the K scale 0
-  int32_t pad;
+  int32_t odd;   // groups that are dead, or a scale of theirs is negative or not finite, the K scale 0 or the V scale
+                 // outside [kScaleMin, kScaleMax]
+  int8_t whole[4];  // what lv is without
 };
 static_assert(sizeof(TileMeta) == 64, "META");
 
@@ -163,6 +172,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -351,45 +366,49 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       }
     };
     int page = -2, page_n = -2;
-    float ks = 0.f, vs = 0.f, ks_n = 0.f, vs_n = 0.f, lv = 0.f, iv = 1.f;
-    // Of the 8 tiles: the pool row of the lane's group, and over all groups (bits) those that a box starts at,
-    // whose block does not exist, with a negative V scale, and odd ones.
+    float ks_n = 0.f, vs_n = 0.f;
+    // Of the 8 tiles: the pool row of the lane's group, and over all groups (bits) those that a box starts at.
     const uint32_t box_bytes = (uint32_t)min(kN, 1 << log2t) * 2 * DT;  // K and V
     int y = 0;
-    uint32_t boxes = 0, dead = 0, neg = 0, odd = 0;
-    auto place = [&] {
+    uint32_t boxes = 0;
+    // Tiles n .. n + 7 after the CTA's first: where their blocks are, and (place runs before the first copies, whose
+    // arrival the converters wait for) which do not exist; then their scales.
+    auto place = [&](int n) {
       const bool live = page >= 0 && page < c.blocks;
       if (!live && page != -2) report_error(L.status, DEV_BAD_BLOCK, 2, page);
       const int at = 16 * (lane & 3);  // of the group in its tile
       const bool first = log2t >= 6 ? at == 0 : (at & ((1 << log2t) - 1)) == 0;  // one box per block of a tile
       y = ((page * c.H + hk) << log2t) + ((16 * (g0 + lane)) & ((1 << log2t) - 1));  // (8 tiles on: the same slot)
       boxes = __ballot_sync(0xffffffffu, live && first);
-      dead = __ballot_sync(0xffffffffu, !live && page != -2);
+      const uint32_t dead = __ballot_sync(0xffffffffu, !live && page != -2);
+      if ((lane & 3) == 0) meta[(n + (lane >> 2)) % kMeta].dead = (int32_t)(dead >> lane & 15u);
     };
-    auto weigh = [&] {
+    auto weigh = [&](int n, float ks, float vs) {
       const bool live = page >= 0 && page < c.blocks;
-      const float av = fmaxf(fabsf(vs), kScaleFloor);
-      lv = vs == vs ? log2f(av) : vs;
-      iv = vs == vs ? 1.f / av : vs;
-      neg = __ballot_sync(0xffffffffu, live && vs < 0.f);
-      odd = dead | neg | __ballot_sync(0xffffffffu, live && !(ks > 0.f && ks <= 3.4028234e38f && fabsf(vs) <= 3.4028234e38f));
-      if (!live) ks = 1.f;  // (past the end: -inf times it stays -inf)
+      const float av = fabsf(vs);
+      const uint32_t bits = __float_as_uint(av), ex = bits >> 23;
+      const bool common = av >= kScaleMin && av <= kScaleMax, parts = live && !common && ex > 0u && ex < 255u;
+      TileMeta& mt = meta[(n + (lane >> 2)) % kMeta];
+      mt.ks[lane & 3] = live ? ks : 1.f;  // (past the end: -inf times it stays -inf)
+      mt.lv[lane & 3] = live ? log2f(parts ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : av) : 0.f;
+      mt.whole[lane & 3] = (int8_t)(parts ? (int)ex - 127 : 0);
+      mt.iv[lane & 3] = live ? 1.f / av : 1.f;
+      const uint32_t neg = __ballot_sync(0xffffffffu, live && vs < 0.f);
+      const uint32_t odd = __ballot_sync(0xffffffffu, live ? vs < 0.f || !common || !(ks > 0.f && ks <= 3.4028234e38f) : page != -2);
+      if ((lane & 3) == 0) mt.neg = (int32_t)(neg >> lane & 15u), mt.odd = (int32_t)(odd >> lane & 15u);
     };
-    // The blocks of the CTA's n-th tile into its raw stage, and its scales into meta[n % kMeta]: lanes w .. w + 3
-    // know its groups.
+    // The blocks of the CTA's n-th tile into its raw stage: lanes w .. w + 3 know its groups.
     auto copy = [&](int n) {
       const int w = 4 * (n & 7), a = lane - w, st = n & 1;
       if (w == 0 && n > 0) {
-        page = page_n, ks = ks_n, vs = vs_n;
+        page = page_n;
         page_n = page_at(g0 + 4 * n + 32 + lane);
-        place();
-        weigh();
+        place(n);
+        weigh(n, ks_n, vs_n);
       }
       const uint32_t b4 = boxes >> w & 15u;
-      if (lane == 0) {
-        meta[n % kMeta].dead = (int32_t)(dead >> w & 15u);  // (before the arrival: the converters read it)
-        mbar_arrive_expect_tx(&B->raw[st], (uint32_t)__popc(b4) * box_bytes);
-      }
+      __syncwarp();  // (place's stores come before the arrival)
+      if (lane == 0) mbar_arrive_expect_tx(&B->raw[st], (uint32_t)__popc(b4) * box_bytes);
       __syncwarp();
       if (a >= 0 && a < 4 && (b4 >> a & 1u)) {
         uint8_t* to = base + Y::RAWS + st * 2 * Y::RAWB + 16 * a * DT;
@@ -398,28 +417,15 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       }
       if (w == 16) scales_at(page_n, ks_n, vs_n);
     };
-    auto describe = [&](int n) {
-      const int w = 4 * (n & 7), a = lane - w;
-      TileMeta& mt = meta[n % kMeta];
-      if (a >= 0 && a < 4) {
-        mt.ks[a] = ks;
-        mt.lv[a] = lv;
-        mt.iv[a] = iv;
-      }
-      if (lane == 0) {
-        mt.neg = (int32_t)(neg >> w & 15u);
-        mt.odd = (int32_t)(odd >> w & 15u);
-      }
-    };
     int loaded = min(2, j1 - j0);
     if (ct < 32) {
       page = page_at(g0 + lane);
       page_n = page_at(g0 + 32 + lane);
-      place();
+      place(0);
       for (int n = 0; n < loaded; ++n) copy(n);
+      float ks, vs;
       scales_at(page, ks, vs);
-      weigh();
-      for (int n = 0; n < loaded; ++n) describe(n);
+      weigh(0, ks, vs);
     }
     constexpr int CPR = DT / 16;                                       // 16-byte pieces per row
     constexpr int PIECES = kN * CPR, NP = (PIECES + Y::CONV - 1) / Y::CONV;  // of a tile, of a thread
@@ -472,10 +478,7 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       ok = ok && convert(n, 0, w[0]);
       if (!(ok = bar_and(1, Y::CONV, ok))) break;  // every converter has left the raw stage
       if (loaded < j1 - j0) {
-        if (ct < 32) {
-          copy(loaded);
-          describe(loaded);
-        }
+        if (ct < 32) copy(loaded);
         ++loaded;
       }
       ok = convert(n, 1, w[1]);
@@ -599,7 +602,19 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
     float2 o[OR];  // fp32 rows: O
 #pragma unroll
     for (int e = 0; e < OR; ++e) o[e] = make_float2(0.f, 0.f);
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;  // l is in units of 2^(m - d) (m taken for 0 while it is -inf)
+    float* unit = reinterpret_cast<float*>(base + Y::RS) + r;  // d, which only odd tiles change
+    *unit = 0.f;
+    bool far = false;  // some row of the warp has another unit than 2^m
+    // Two values of P as words of its parts
+    auto p_words = [](float2 x, uint32_t& hi, uint32_t& lo) {
+      hi = pack2<__half>(x.x, x.y);
+      if constexpr (SPLIT) {
+        const float2 y = unpack2<__half>(hi);
+        const float2 z = __ffma2_rn(y, make_float2(-1.f, -1.f), x);
+        lo = pack2<__half>(z.x, z.y);
+      }
+    };
     auto product_done = [&](int n) {  // of the tile n after the CTA's first
       return __all_sync(0xffffffffu, wait_for(&B->pv_full[rt], (uint32_t)n & 1u, abort, L.status, W_PV, n));
     };
@@ -633,28 +648,28 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       };
       // The common tile, all of it seen by every row of the warp; one that ends for some row, whose scores
       // past the end become -inf; and an odd one, taken score by score.
-      const bool odd = mt.odd || L.scale_log2 == 0.f;
-      const bool edge = !odd && !__all_sync(0xffffffffu, lim >= tok0 + kN - 1);
-      uint64_t vis = ~0ull;  // the columns that the row sees
-      if (odd) {
-        const int hi = min(max(lim - tok0 + 1, 0), kN);
-        vis = hi == kN ? ~0ull : (1ull << hi) - 1ull;
+      const bool odd = mt.odd || L.scale_log2 == 0.f || far;
+      float mx = -INFINITY;  // the row's largest exponent
+      float ref, al, sum = 0.f;
+      bool moved;
+      auto move = [&] {
+        const float mn = SPLIT ? fmaxf(m, mx) : mx > m + kLag || m == -INFINITY ? fmaxf(m, mx) : m;
+        moved = __any_sync(0xffffffffu, mn != m);
+        ref = mn == -INFINITY ? 0.f : mn;
+        al = ex2f(m - ref);
+        m = mn;
+      };
+      if (!odd) {
+        const bool edge = !__all_sync(0xffffffffu, lim >= tok0 + kN - 1);
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          if (mt.dead >> g & 1) vis &= ~(0xffffull << (16 * g));
-      }
-      // the row's largest exponent
-      float mx = -INFINITY;
+        for (int c0 = 0; c0 < kN; c0 += CH) {
+          load_s(c0);
+          if (edge) {
+            const int hi = lim - tok0 - c0;
 #pragma unroll
-      for (int c0 = 0; c0 < kN; c0 += CH) {
-        load_s(c0);
-        if (edge) {
-          const int hi = lim - tok0 - c0;
-#pragma unroll
-          for (int e = 0; e < CH; ++e)
-            if (e > hi) s[e] = -INFINITY;
-        }
-        if (!odd) {
+            for (int e = 0; e < CH; ++e)
+              if (e > hi) s[e] = -INFINITY;
+          }
 #pragma unroll
           for (int g = 0; g < CH / 16; ++g) {
             const float* x = s + 16 * g;
@@ -664,34 +679,20 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
             u = max3(u, x[14], x[15]);
             mx = fmaxf(mx, fmaf(fmaxf(u, w), mt.ks[c0 / 16 + g] * rs, mt.lv[c0 / 16 + g]));
           }
-        } else {
-          const uint64_t v = vis >> c0;
-#pragma unroll
-          for (int e = 0; e < CH; ++e) {
-            const int g = (c0 + e) >> 4;
-            if (v >> e & 1) mx = fmaxf(mx, fmaf(s[e], mt.ks[g] * rs, mt.lv[g]));
-          }
         }
-      }
-      const float mn = SPLIT ? fmaxf(m, mx) : mx > m + kLag || m == -INFINITY ? fmaxf(m, mx) : m;
-      const bool moved = __any_sync(0xffffffffu, mn != m);
-      const float ref = mn == -INFINITY ? 0.f : mn;
-      const float al = ex2f(m - ref);
-      m = mn;
-      // P into the columns of the scores that it comes from, and its sum
-      float sum = 0.f;
+        move();
+        // P into the columns of the scores that it comes from, and its sum
 #pragma unroll
-      for (int c0 = 0; c0 < kN; c0 += CH) {
-        if (CH < kN) {
-          load_s(c0);
-          if (edge) {
-            const int hi = lim - tok0 - c0;
+        for (int c0 = 0; c0 < kN; c0 += CH) {
+          if (CH < kN) {
+            load_s(c0);
+            if (edge) {
+              const int hi = lim - tok0 - c0;
 #pragma unroll
-            for (int e = 0; e < CH; ++e)
-              if (e > hi) s[e] = -INFINITY;
+              for (int e = 0; e < CH; ++e)
+                if (e > hi) s[e] = -INFINITY;
+            }
           }
-        }
-        auto form = [&](auto masked) {
 #pragma unroll
           for (int h = 0; h < CH / 32; ++h) {
             uint32_t ph[16], pl[SPLIT ? 16 : 1];
@@ -704,36 +705,81 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
               for (int e = 0; e < 16; e += 2) {
                 const int i = 32 * h + 16 * g + e;
                 float2 x = __ffma2_rn(make_float2(s[i], s[i + 1]), make_float2(k, k), make_float2(sh, sh));
-                if constexpr (decltype(masked)::value) {
-                  if (!(vis >> (c0 + i) & 1)) x.x = -INFINITY;
-                  if (!(vis >> (c0 + i + 1) & 1)) x.y = -INFINITY;
-                }
                 x.x = ex2f(x.x);
                 x.y = ex2f(x.y);
                 part = __fadd2_rn(part, x);
-                if constexpr (decltype(masked)::value) {
-                  if (mt.neg >> grp & 1) x.x = -x.x, x.y = -x.y;
-                }
-                const int w = 8 * g + (e >> 1);
-                ph[w] = pack2<__half>(x.x, x.y);
-                if constexpr (SPLIT) {
-                  const float2 y = unpack2<__half>(ph[w]);
-                  const float2 d = __ffma2_rn(y, make_float2(-1.f, -1.f), x);
-                  pl[w] = pack2<__half>(d.x, d.y);
-                }
+                p_words(x, ph[8 * g + (e >> 1)], pl[SPLIT ? 8 * g + (e >> 1) : 0]);
               }
-              const float p = part.x + part.y;
-              if constexpr (decltype(masked)::value) sum += p == 0.f ? 0.f : p * mt.iv[grp];  // (an unseen block's may be NaN)
-              else sum = fmaf(p, mt.iv[grp], sum);
+              sum = fmaf(part.x + part.y, mt.iv[grp], sum);
             }
             tmem_st16(ts + c0 + 32 * h, ph);
             if constexpr (SPLIT) tmem_st16(ts + c0 + 32 * h + 16, pl);
           }
-        };
-        if (odd) form(std::true_type{});
-        else form(std::false_type{});
+        }
+        l = fmaf(l, al, sum);
+      } else {
+        uint64_t vis;  // the columns that the row sees
+        {
+          const int hi = min(max(lim - tok0 + 1, 0), kN);
+          vis = hi == kN ? ~0ull : (1ull << hi) - 1ull;
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            if (mt.dead >> g & 1) vis &= ~(0xffffull << (16 * g));
+        }
+        // the largest score so far: near m - d, m itself where d is 0 (within kNear and kLag)
+        float d = *unit;
+        const bool none = m == -INFINITY;
+        const float r = none ? 0.f : m;
+        float high = l != 0.f ? r - d : -INFINITY;
+#pragma unroll 1
+        for (int c0 = 0; c0 < kN; c0 += 32) {
+          float x[32];
+          tc::tmem_ld32(ts + c0, x);
+          tc::tmem_wait_ld();
+          const uint32_t v = (uint32_t)(vis >> c0);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int g = c0 / 16 + e / 16;
+            const float k = mt.ks[g] * rs;
+            if (v >> e & 1) mx = fmaxf(mx, fmaf(x[e], k, mt.lv[g] + (float)mt.whole[g])), high = fmaxf(high, x[e] * k);
+          }
+        }
+        move();
+        const float apart = ref - high;
+        float dn = 0.f;
+        if (high != -INFINITY && !(fabsf(apart) <= kNear)) dn = fabsf(apart - d) <= kSlack ? d : rintf(apart);
+        if (dn != d || none) l = l == 0.f ? 0.f : l * ex2f((r - ref) + (dn - d));
+        else l *= al;
+        *unit = d = dn;
+        const float low = kPShift<SPLIT> - (ref - d);
+#pragma unroll 1
+        for (int c0 = 0; c0 < kN; c0 += 32) {
+          float x[32];
+          tc::tmem_ld32(ts + c0, x);
+          tc::tmem_wait_ld();
+          const uint32_t v = (uint32_t)(vis >> c0);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int g = c0 / 16 + h;
+            const float k = mt.ks[g] * rs, sh = (((float)mt.whole[g] + kPShift<SPLIT>) - ref) + mt.lv[g];
+            const bool neg = mt.neg >> g & 1;
+            uint32_t ph[8], pl[8];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const int i = 16 * h + e;
+              const bool a = v >> i & 1, b = v >> (i + 1) & 1;
+              sum += (a ? ex2f(fmaf(x[i], k, low)) : 0.f) + (b ? ex2f(fmaf(x[i + 1], k, low)) : 0.f);
+              float2 y = make_float2(a ? ex2f(fmaf(x[i], k, sh)) : 0.f, b ? ex2f(fmaf(x[i + 1], k, sh)) : 0.f);
+              if (neg) y.x = -y.x, y.y = -y.y;
+              p_words(y, ph[e >> 1], pl[e >> 1]);
+            }
+            tmem_st8(ts + c0 + 8 * h, ph);
+            if constexpr (SPLIT) tmem_st8(ts + c0 + 16 + 8 * h, pl);
+          }
+        }
+        l += sum;
+        far = __any_sync(0xffffffffu, d != 0.f || (m == -INFINITY && l != 0.f));
       }
-      l = fmaf(l, al, sum);
       // Every product is waited for in its turn, needed or not: a wait by parity tells a phase only from its
       // neighbours. (This one could not start before the last one's end.)
       if (n > 0) ok = product_done(n - 1);
@@ -782,17 +828,38 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         for (int i = 0; i < 32; ++i) x[i] = 0.f;
       }
     };
+    // O is in units of 2^m, l of 2^(m - d): what O has to be multiplied by, as two factors that are in range (where m is
+    // -inf, O is 0 or NaN)
+    float ref = m == -INFINITY ? 0.f : m, up0 = 1.f, up1 = 1.f;
+    if (far && *unit != 0.f) {
+      float by = *unit;
+      ref -= by;
+      if (L.ws_o) {  // with l's own power of two, so that O is as large as the part's output
+        const int ex = l > 0.f && l <= 3.4028234e38f ? ilogbf(l) : 0;
+        l = scalbnf(l, -ex);
+        ref += (float)ex;
+        by -= (float)ex;
+      }
+      if (m != -INFINITY) {
+        const float half = rintf(0.5f * by);
+        up0 = ex2f(half), up1 = ex2f(by - half);
+      }
+    }
     if (L.ws_o) {
       const int64_t at = (int64_t)blockIdx.x * (kM * RT) + r;
 #pragma unroll
       for (int e = 0; e < DT; e += 32) {
         float x[32];
         channels(e, x);
+        if (far) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = x[i] * up0 * up1;
+        }
 #pragma unroll
         for (int i = 0; i < 32; i += 4)
           if (live && e + i < c.D) *reinterpret_cast<float4*>(L.ws_o + at * c.D + e + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
       }
-      if (live) L.ws_ml[at] = make_float2(m, l);
+      if (live) L.ws_ml[at] = make_float2(l == 0.f ? -INFINITY : ref, l);
     } else {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       uint8_t* mine = Qs + tr * (PER * 16);
@@ -800,11 +867,18 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       for (int e = 0; e < DT; e += 32) {
         float x[32];
         channels(e, x);
+        if (far) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = x[i] * inv * up0 * up1;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] *= inv;
+        }
 #pragma unroll
         for (int i = 0; i < 32; i += V8) {
           float y[V8];
 #pragma unroll
-          for (int k = 0; k < V8; ++k) y[k] = l == 0.f ? 0.f : x[i + k] * inv;
+          for (int k = 0; k < V8; ++k) y[k] = l == 0.f ? 0.f : x[i + k];
           const int p = (e + i) / V8;
           store_row<T, V8, true>(reinterpret_cast<T*>(mine + ((p ^ (tr & 7)) << 4)), y);
         }

@@ -1,0 +1,115 @@
+"""The 8-bit cache at the edges of its ranges. Bounds and oracle as in test_gpu_cache.py."""
+
+import numpy as np
+import pytest
+import torch
+
+import supra_attn
+from oracle import cache as oc
+from test_gpu_cache import TYPES, Pool, attention_bound
+
+pytestmark = pytest.mark.gpu
+
+
+def zero_scale(fmt):
+    """What cache_write gives a block of zeros."""
+    return np.float32(2.0 ** -100) * np.float32(1.0 / oc.QMAX[fmt])
+
+
+def check_bound(gpu, fmt, dtype, T, G, D, lengths, rows, causal, *, seed, sharp=1.0, scale=None, mutate=None):
+    """Attention of one cache head against the definition, every output within attention_bound. (The error over all
+    outputs together has no limit of its own here: a row whose large weights meet V = 0 is formed from small weights
+    alone, and each of those is off, against the sum of all, by what the scores may be: for D = 128 and a score of 30,
+    (2 D / 16 + 6) 2^-23 30 = 8e-5. Ordinary scales with codes of 0 in those places give the same errors.)"""
+    rng = np.random.default_rng(seed + 31 * T + D)
+    p = Pool(gpu, rng, fmt, T, 1, D, lengths)
+    if mutate:
+        mutate(p)
+        p.put()
+    start, seqs = p.batch(rows)
+    q = (torch.from_numpy(rng.standard_normal((start[-1], G * D)).astype(np.float32)) * sharp).to(TYPES[dtype])
+    out = torch.full_like(q, 5.0, device="cuda")
+    supra_attn.cache_attention(gpu, p.cache, seqs, q=q.cuda(), H=G, out=out, scale=scale, causal=causal)
+    gpu.sync()
+    got, qn = (t.cpu().double().numpy().reshape(-1, G, D) for t in (out, q))
+    sc = float(np.float32(1 / np.sqrt(D) if scale is None else scale))
+    ref, *terms = oc.attention(fmt, p.kc, p.ks, p.vc, p.vs, qn, lengths, start, p.table, sc, causal)
+    tol = attention_bound(dtype, D, max(lengths), ref, *terms)
+    bad = ~(np.abs(got - ref) <= tol)
+    assert not bad.any(), f"{bad.sum()} of {bad.size} outside the bound, first at {np.argwhere(bad)[0]}: {got[bad][0]} for {ref[bad][0]}"
+
+
+# ---- V scales far apart -------------------------------------------------------------------------------
+# lead tokens with V = 0, then ordinary ones; whole, and split along the cache (2500 tokens, few units)
+ZERO_V = [(64, 130), (128, 256), (192, 300), (320, 2500)]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lead,tokens", ZERO_V)
+def test_attention_of_leading_zero_values(gpu, lead, tokens, D, dtype, fmt):
+    """Tokens with V = 0 count in the sum of the probabilities like all others, wherever they are."""
+    def zeros(scale, blocks):
+        def f(p):
+            for page in [p.table[0][j] for j in blocks]:
+                p.vc[page] = 0
+                p.vs[page] = scale
+        return f
+
+    n = -(-tokens // 64)
+    first, last = range(lead // 64), range(n - lead // 64, n)
+    # (sharp=0: all scores equal)
+    for sharp, scale, blocks in ((0.0, zero_scale(fmt), first), (1.0, zero_scale(fmt), first), (0.0, 0.0, first), (1.0, 0.0, last),
+                                 (0.0, zero_scale(fmt), range(n))):
+        check_bound(gpu, fmt, dtype, 64, 2, D, [tokens], [130], False, seed=40, sharp=sharp, mutate=zeros(scale, blocks))
+    check_bound(gpu, fmt, dtype, 64, 2, D, [tokens], [130], True, seed=41, mutate=zeros(zero_scale(fmt), first))
+    check_bound(gpu, fmt, dtype, 64, 2, D, [tokens], [2], True, seed=42, mutate=zeros(zero_scale(fmt), first))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("far", [2.0 ** 60, 2.0 ** -60])
+def test_attention_of_values_of_very_unlike_size(gpu, far, D, dtype):
+    """Blocks whose V is zero, tiny or huge beside one another: a block's size counts in what it gives, never in its share."""
+    def spread(sizes):
+        def f(p):
+            for i, page in enumerate(p.table[0]):
+                p.vs[page] = np.float32(sizes[i % len(sizes)]) * p.vs[page]
+                if sizes[i % len(sizes)] == 0:
+                    p.vc[page] = 0
+                    p.vs[page] = zero_scale("int8")
+        return f
+
+    for sizes in ((0, far), (far, 0), (far, 2.0 ** -100, 1.0), (0, 0, 1.0, far), (2.0 ** -125, far, 0), (2.0 ** 100, far)):
+        for T in (16, 64):
+            for sharp in (0.0, 1.0):
+                check_bound(gpu, "int8", dtype, T, 1, D, [11 * T - 3], [140], True, seed=43, sharp=sharp, mutate=spread(sizes))
+    # a caller's own scales below any that a write makes, alone
+    check_bound(gpu, "e4m3", dtype, 32, 2, D, [70], [140], False, seed=44, mutate=spread((2.0 ** -118,)))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_attention_of_many_zero_values_in_16_bits(gpu, dtype):
+    """So many tokens with V = 0 in one piece that a sum in units of V would pass the range of 32 bits: 301 heads, so
+    that no unit is split."""
+    H, D, T, lead, rows = 301, 16, 128, 6016, 18
+    rng = np.random.default_rng(45)
+    blocks = lead // T + 1
+    kc = torch.zeros(blocks, H, T, D, dtype=torch.uint8, device="cuda")
+    vc = torch.zeros_like(kc)
+    ks = torch.full((blocks, H), float(zero_scale("e4m3")), device="cuda")
+    vs = ks.clone()
+    vc[-1] = 0x38  # 1.0
+    vs[-1] = torch.from_numpy(np.exp(rng.standard_normal(H)).astype(np.float32)).cuda()
+    cache = supra_attn.KVCache(gpu, blocks, H, D, block_tokens=T, format="e4m3", k=kc, v=vc, k_scale=ks, v_scale=vs)
+    table = torch.arange(blocks, dtype=torch.int32, device="cuda").view(1, -1)
+    seqs = supra_attn.CacheBatch(gpu, torch.tensor([lead + T], dtype=torch.int32, device="cuda"), table, max_rows=rows)
+    q = torch.randn(rows, H * D, device="cuda").to(TYPES[dtype])
+    out = torch.empty_like(q)
+    supra_attn.cache_attention(gpu, cache, seqs, q=q, H=H, out=out)
+    gpu.sync()
+    ref = (vs[-1].double() * (T / (lead + T)))[None, :, None].expand(rows, H, D).cpu().numpy()
+    got = out.double().cpu().numpy().reshape(rows, H, D)
+    zero = np.zeros((2, 1, 1, 1))
+    assert (np.abs(got - ref) <= attention_bound(dtype, D, lead + T, ref, ref, zero, np.zeros((1, 1)), np.zeros((1, 1)))).all()
