@@ -648,7 +648,10 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       };
       // The common tile, all of it seen by every row of the warp; one that ends for some row, whose scores
       // past the end become -inf; and an odd one, taken score by score.
-      const bool odd = mt.odd || L.scale_log2 == 0.f || far;
+      bool odd = mt.odd || L.scale_log2 == 0.f || far;
+      const bool edge = !odd && !__all_sync(0xffffffffu, lim >= tok0 + kN - 1);
+      // (-inf times a factor that has underflowed to 0, as rows of q that are zeros have it, would be NaN)
+      if (edge) odd = __any_sync(0xffffffffu, fminf(fminf(mt.ks[0], mt.ks[1]), fminf(mt.ks[2], mt.ks[3])) * rs == 0.f);
       float mx = -INFINITY;  // the row's largest exponent
       float ref, al, sum = 0.f;
       bool moved;
@@ -660,7 +663,6 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         m = mn;
       };
       if (!odd) {
-        const bool edge = !__all_sync(0xffffffffu, lim >= tok0 + kN - 1);
 #pragma unroll
         for (int c0 = 0; c0 < kN; c0 += CH) {
           load_s(c0);

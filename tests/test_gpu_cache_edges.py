@@ -113,3 +113,21 @@ def test_attention_of_many_zero_values_in_16_bits(gpu, dtype):
     got = out.double().cpu().numpy().reshape(rows, H, D)
     zero = np.zeros((2, 1, 1, 1))
     assert (np.abs(got - ref) <= attention_bound(dtype, D, lead + T, ref, ref, zero, np.zeros((1, 1)), np.zeros((1, 1)))).all()
+
+
+# ---- scores whose factor underflows ---------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("rows", [3, 150])
+def test_attention_of_zero_queries_and_keys(gpu, rows, dtype, fmt):
+    """Rows of q that are zeros over blocks of K that are zeros, where a tile ends for some row: the mean of V."""
+    def zero_k(p):
+        for page in p.table[0] + p.table[1]:
+            p.kc[page] = 0
+            p.ks[page] = zero_scale(fmt)
+
+    for T, D in ((64, 64), (16, 128), (128, 96)):
+        for causal in (False, True):
+            check_bound(gpu, fmt, dtype, T, 2, D, [100, 257], [min(rows, 100), rows], causal, seed=46, sharp=0.0, mutate=zero_k)
+            # a very small scale reaches the same with any K
+            check_bound(gpu, fmt, dtype, T, 2, D, [100, 257], [min(rows, 100), rows], causal, seed=47, sharp=1e-20, scale=1e-30)
