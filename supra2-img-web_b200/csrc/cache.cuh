@@ -224,4 +224,12 @@ __device__ __forceinline__ int32_t block_of(const CacheSeqs& s, const CachePool&
   return -1;
 }
 
+// The attention kernels look blocks up ahead of their use: the table's entry j of sequence b, whatever it is, but never
+// kPastEnd, which they put in the place of entries after the last token (an entry with that value becomes the next
+// one, which is no block either).
+constexpr int32_t kPastEnd = INT32_MIN;
+__device__ __forceinline__ int32_t page_of(const CacheSeqs& s, int b, int j) {
+  return max(s.table[(int64_t)b * s.ld_table + j], kPastEnd + 1);
+}
+
 }  // namespace supra

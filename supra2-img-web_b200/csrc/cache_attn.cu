@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
   // loads are under way while the first is used up.
   const int log2t = c.log2t;
   auto page_at = [&](int grp) {  // grp: 16-token group of the sequence
-    return grp * 16 < seen ? L.s.table[(int64_t)b * L.s.ld_table + ((grp * 16) >> log2t)] : -2;
+    return grp * 16 < seen ? page_of(L.s, b, (grp * 16) >> log2t) : kPastEnd;
   };
   auto scales_at = [&](int p, float& ks, float& vs) {
     ks = vs = 0.f;
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
       const bool dead = page < 0 || page >= c.blocks;
       Group* gr = groups + (i % kStages) * 2 + a;
       gr->ks = ks, gr->vs = vs, gr->dead = dead;
-      if (dead && page != -2) report_error(L.status, DEV_BAD_BLOCK, 1, page);
+      if (dead && page != kPastEnd) report_error(L.status, DEV_BAD_BLOCK, 1, page);
     }
   };
   // the first copies go out before q and the scales are fetched

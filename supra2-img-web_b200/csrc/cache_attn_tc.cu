@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
     // 8 tiles' while it uses them up.
     const int g0 = j0 * (kN / 16);
     auto page_at = [&](int grp) {
-      return grp * 16 < seen && grp < j1 * (kN / 16) ? L.s.table[(int64_t)b * L.s.ld_table + ((grp * 16) >> log2t)] : -2;
+      return grp * 16 < seen && grp < j1 * (kN / 16) ? page_of(L.s, b, (grp * 16) >> log2t) : kPastEnd;
     };
     auto scales_at = [&](int p, float& ks, float& vs) {
       ks = vs = 0.f;
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         vs = c.vs[u];
       }
     };
-    int page = -2, page_n = -2;
+    int page = kPastEnd, page_n = kPastEnd;
     float ks_n = 0.f, vs_n = 0.f;
     // Of the 8 tiles: the pool row of the lane's group, and over all groups (bits) those that a box starts at.
     const uint32_t box_bytes = (uint32_t)min(kN, 1 << log2t) * 2 * DT;  // K and V
@@ -375,12 +375,12 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
     // arrival the converters wait for) which do not exist; then their scales.
     auto place = [&](int n) {
       const bool live = page >= 0 && page < c.blocks;
-      if (!live && page != -2) report_error(L.status, DEV_BAD_BLOCK, 2, page);
+      if (!live && page != kPastEnd) report_error(L.status, DEV_BAD_BLOCK, 2, page);
       const int at = 16 * (lane & 3);  // of the group in its tile
       const bool first = log2t >= 6 ? at == 0 : (at & ((1 << log2t) - 1)) == 0;  // one box per block of a tile
       y = ((page * c.H + hk) << log2t) + ((16 * (g0 + lane)) & ((1 << log2t) - 1));  // (8 tiles on: the same slot)
       boxes = __ballot_sync(0xffffffffu, live && first);
-      const uint32_t dead = __ballot_sync(0xffffffffu, !live && page != -2);
+      const uint32_t dead = __ballot_sync(0xffffffffu, !live && page != kPastEnd);
       if ((lane & 3) == 0) meta[(n + (lane >> 2)) % kMeta].dead = (int32_t)(dead >> lane & 15u);
     };
     auto weigh = [&](int n, float ks, float vs) {
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       mt.whole[lane & 3] = (int8_t)(parts ? (int)ex - 127 : 0);
       mt.iv[lane & 3] = live ? 1.f / av : 1.f;
       const uint32_t neg = __ballot_sync(0xffffffffu, live && vs < 0.f);
-      const uint32_t odd = __ballot_sync(0xffffffffu, live ? vs < 0.f || !common || !(ks > 0.f && ks <= 3.4028234e38f) : page != -2);
+      const uint32_t odd = __ballot_sync(0xffffffffu, live ? vs < 0.f || !common || !(ks > 0.f && ks <= 3.4028234e38f) : page != kPastEnd);
       if ((lane & 3) == 0) mt.neg = (int32_t)(neg >> lane & 15u), mt.odd = (int32_t)(odd >> lane & 15u);
     };
     // The blocks of the CTA's n-th tile into its raw stage: lanes w .. w + 3 know its groups.

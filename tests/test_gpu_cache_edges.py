@@ -6,7 +6,7 @@ import torch
 
 import supra_attn
 from oracle import cache as oc
-from test_gpu_cache import TYPES, Pool, attention_bound
+from test_gpu_cache import TYPES, Pool, attention_bound, bad_call
 
 pytestmark = pytest.mark.gpu
 
@@ -131,3 +131,38 @@ def test_attention_of_zero_queries_and_keys(gpu, rows, dtype, fmt):
             check_bound(gpu, fmt, dtype, T, 2, D, [100, 257], [min(rows, 100), rows], causal, seed=46, sharp=0.0, mutate=zero_k)
             # a very small scale reaches the same with any K
             check_bound(gpu, fmt, dtype, T, 2, D, [100, 257], [min(rows, 100), rows], causal, seed=47, sharp=1e-20, scale=1e-30)
+
+
+# ---- block numbers ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("what", ["write", "read", "attention"])
+@pytest.mark.parametrize("entry", [-2, -7, -(1 << 31), (1 << 31) - 1])
+def test_every_block_outside_the_cache_is_reported(gpu, what, entry):
+    rng = np.random.default_rng(48)
+    p = Pool(gpu, rng, "int8", 16, 2, 32, [16, 16], spare=3)
+    p.d_table[0, 0] = entry
+    _, seqs = p.batch([2, 2])
+    y = bad_call(gpu, p, seqs, what, 4, "outside the cache")
+    if what == "attention":
+        assert (y[:2] == 0).all() and (y[2:] != 5).all()
+    elif what == "read":
+        assert (y[:2] == 5).all() and (y[2:] != 5).any()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("entry", [-1, -2, -(1 << 31), 9])
+@pytest.mark.parametrize("T,D,rows", [(16, 64, 200), (64, 64, 200), (32, 128, 300), (16, 64, 2), (64, 128, 2)])
+def test_tokens_of_a_missing_block_are_left_out(gpu, T, D, rows, entry, fmt):
+    rng = np.random.default_rng(49)
+    n = 5 * T // 2
+    p = Pool(gpu, rng, fmt, T, 1, D, [n], spare=3)
+    p.d_table[0, 1] = entry
+    seqs = supra_attn.CacheBatch(gpu, p.d_len, p.d_table, max_rows=rows)
+    q = torch.from_numpy(rng.standard_normal((rows, D)).astype(np.float32)).cuda()
+    out = torch.empty_like(q)
+    supra_attn.cache_attention(gpu, p.cache, seqs, q=q, H=1, out=out)
+    with pytest.raises(supra_attn.SupraAttnError, match="outside the cache"):
+        gpu.sync()
+    table = [[p.table[0][0], p.table[0][2]]]
+    ref, pv, av, st, sm = oc.attention(fmt, p.kc, p.ks, p.vc, p.vs, q.cpu().double().numpy().reshape(rows, 1, D), [n - T], [0, rows], table,
+                                       float(np.float32(1 / np.sqrt(D))), False)
+    assert (np.abs(out.cpu().double().numpy().reshape(rows, 1, D) - ref) <= attention_bound("fp32", D, n, ref, pv, av, st, sm)).all()
