@@ -19,7 +19,9 @@
 // number that keeps m - d near the row's largest score alone; warps with a row whose d is not 0 stay with that form.
 // q carries a power of two per row (cache_attn.cu).
 // 16-bit rows keep O in TMEM, where m moves only when a tile exceeds it by 2^8 (then the softmax threads
-// rescale O there). fp32 rows use two fp16 parts of q and p (each product two MMAs), move m exactly, and
+// rescale O there). Sums in TMEM are truncated, which pulls them towards zero by up to 2^-23 for each 16 tokens (measured
+// 2e-4 at 32768 tokens, half a rounding of fp16): after every 4096 tokens O joins a sum that is rounded to nearest, in local
+// memory, and starts anew (32768 tokens: 2.3e-5). fp32 rows use two fp16 parts of q and p (each product two MMAs), move m exactly, and
 // add each tile's product to O in fp32 registers, rounded to nearest, so that the error does not grow
 // with the number of tiles.
 //
@@ -50,6 +52,7 @@ constexpr int kN = 64;   // tokens of a tile
 template <bool SPLIT>
 constexpr float kPShift = SPLIT ? 15.f : 7.f;
 constexpr float kLag = 8.f;
+constexpr int kFold = 64;  // 16-bit rows: tiles that TMEM sums up at a time
 constexpr float kScaleMin = 2.3283064365386963e-10f, kScaleMax = 4294967296.f;  // 2^-32, 2^32: V scales of common tiles
 constexpr float kNear = 32.f;   // d is 0 where m is within this of the row's largest score
 constexpr float kSlack = 16.f;  // elsewhere m - d is
@@ -213,8 +216,9 @@ __device__ __forceinline__ void reg_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// T: q and out; DT: head dim rounded up to 64 or 128.
-template <typename T, int FMT, int DT>
+// T: q and out; DT: head dim rounded up to 64 or 128. FOLD: 16-bit rows whose CTAs may walk over more than kFold tiles (the
+// others are spared its code: 128 prompts of up to 128 tokens, 256 bf16 rows each: 74 us with it, 72 without).
+template <typename T, int FMT, int DT, bool FOLD>
 __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, sizeof(T) == 4>::PER_SM)
     cache_attn_tc_kernel(const __grid_constant__ CacheAttnArgs L, const __grid_constant__ CUtensorMap mk,
                          const __grid_constant__ CUtensorMap mv, int tiles) {
@@ -527,7 +531,7 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         for (int k = 0; k < kN / 16; ++k) {
           if (k >= steps) break;
           const uint32_t a = s0 + 32 * (k >> 1) + 8 * (k & 1);  // P of 32 tokens: 16 columns, then its low part
-          mma_ts(d, a, dvs + ((k * 2048) >> 4), id, k > 0 || (!SPLIT && n > 0));
+          mma_ts(d, a, dvs + ((k * 2048) >> 4), id, k > 0 || (!SPLIT && (FOLD ? n % kFold : n) > 0));
           if constexpr (SPLIT) mma_ts(d, a + 16, dvs + ((k * 2048) >> 4), id, 1);
         }
         tc::commit(&B->pv_full[rt]);
@@ -602,6 +606,9 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
     float2 o[OR];  // fp32 rows: O
 #pragma unroll
     for (int e = 0; e < OR; ++e) o[e] = make_float2(0.f, 0.f);
+    // 16-bit rows: O of the folds so far, in units of 2^m_kept (indexed at run time, so that it stays out of registers)
+    float4 kept[FOLD ? DT / 4 : 1];
+    float m_kept = -INFINITY;
     float m = -INFINITY, l = 0.f;  // l is in units of 2^(m - d) (m taken for 0 while it is -inf)
     float* unit = reinterpret_cast<float*>(base + Y::RS) + r;  // d, which only odd tiles change
     *unit = 0.f;
@@ -631,6 +638,27 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
           x = __fadd2_rn(make_float2(a[2 * i], a[2 * i + 1]), x);
         }
       }
+    };
+    // 16-bit rows: O times al, and what is kept where there is some, in units of 2^ref: kept, or at the end back into TMEM
+    auto fold = [&](bool more, float al, float ref, bool last) {
+      const float f = ex2f(m_kept - ref);
+      tc::fence_after_sync();
+#pragma unroll 1
+      for (int e = 0; e < DT; e += 32) {
+        float a[32];
+        tc::tmem_ld32(tl + Y::COL_ACC + e, a);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          float4& at = kept[FOLD ? (e + i) / 4 : 0];
+          const float4 y = more ? at : make_float4(0.f, 0.f, 0.f, 0.f);
+          a[i] = fmaf(y.x, f, a[i] * al), a[i + 1] = fmaf(y.y, f, a[i + 1] * al);
+          a[i + 2] = fmaf(y.z, f, a[i + 2] * al), a[i + 3] = fmaf(y.w, f, a[i + 3] * al);
+          if (!last) at = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
+        }
+        if (last) tc::tmem_st32(tl + Y::COL_ACC + e, a);
+      }
+      tc::tmem_wait_st();
     };
     for (int j = j0; j < j1; ++j) {
       const int n = j - j0;
@@ -785,7 +813,10 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       // Every product is waited for in its turn, needed or not: a wait by parity tells a phase only from its
       // neighbours. (This one could not start before the last one's end.)
       if (n > 0) ok = product_done(n - 1);
-      if (n > 0 && (SPLIT || moved)) {
+      if (FOLD && n > 0 && n % kFold == 0) {
+        if (ok) fold(n > kFold, al, ref, false);
+        m_kept = m;
+      } else if (n > 0 && (SPLIT || moved)) {
         // fp32 rows: the previous product joins O. Either: O follows m.
         if (SPLIT && ok) add_product();
         if (moved && ok) {
@@ -815,6 +846,7 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
       ok = product_done(j1 - j0 - 1);
       tc::fence_after_sync();
       if (SPLIT && ok) add_product();
+      if (FOLD && ok && j1 - j0 > kFold) fold(true, 1.f, m == -INFINITY ? 0.f : m, true);
     }
     // ---- epilogue: the row through shared memory (its own Q rows), stored in whole 16-byte pieces ----
     // 32 channels of the row's O
@@ -913,10 +945,10 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
   }
 }
 
-template <typename T, int FMT, int DT>
+template <typename T, int FMT, int DT, bool FOLD>
 cudaError_t tc_as(const CacheAttnLaunch& L, const CacheAttnPlan& P, cudaStream_t s) {
   using Y = Cfg<DT, sizeof(T) == 4>;
-  auto kernel = cache_attn_tc_kernel<T, FMT, DT>;
+  auto kernel = cache_attn_tc_kernel<T, FMT, DT, FOLD>;
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = once_per_device(done, L.device, [&] {
     if constexpr (sizeof(T) == 4) {
@@ -931,10 +963,18 @@ cudaError_t tc_as(const CacheAttnLaunch& L, const CacheAttnPlan& P, cudaStream_t
   kernel<<<(unsigned)(P.units * P.splits), Y::THREADS, Y::SMEM, s>>>(L, L.mk, L.mv, P.tiles);
   return cudaGetLastError();
 }
+template <typename T, bool FOLD>
+cudaError_t tc_fold(const CacheAttnLaunch& L, const CacheAttnPlan& P, int format, cudaStream_t s) {
+  if (L.c.D <= 64) return format == kCacheInt8 ? tc_as<T, kCacheInt8, 64, FOLD>(L, P, s) : tc_as<T, kCacheE4m3, 64, FOLD>(L, P, s);
+  return format == kCacheInt8 ? tc_as<T, kCacheInt8, 128, FOLD>(L, P, s) : tc_as<T, kCacheE4m3, 128, FOLD>(L, P, s);
+}
 template <typename T>
 cudaError_t tc_type(const CacheAttnLaunch& L, const CacheAttnPlan& P, int format, cudaStream_t s) {
-  if (L.c.D <= 64) return format == kCacheInt8 ? tc_as<T, kCacheInt8, 64>(L, P, s) : tc_as<T, kCacheE4m3, 64>(L, P, s);
-  return format == kCacheInt8 ? tc_as<T, kCacheInt8, 128>(L, P, s) : tc_as<T, kCacheE4m3, 128>(L, P, s);
+  if constexpr (sizeof(T) == 2) {
+    const int64_t tiles = (L.s.max_len + kN - 1) / kN;
+    if ((tiles + P.splits - 1) / P.splits > kFold) return tc_fold<T, true>(L, P, format, s);
+  }
+  return tc_fold<T, false>(L, P, format, s);
 }
 
 }  // namespace

@@ -166,3 +166,65 @@ def test_tokens_of_a_missing_block_are_left_out(gpu, T, D, rows, entry, fmt):
     ref, pv, av, st, sm = oc.attention(fmt, p.kc, p.ks, p.vc, p.vs, q.cpu().double().numpy().reshape(rows, 1, D), [n - T], [0, rows], table,
                                        float(np.float32(1 / np.sqrt(D))), False)
     assert (np.abs(out.cpu().double().numpy().reshape(rows, 1, D) - ref) <= attention_bound("fp32", D, n, ref, pv, av, st, sm)).all()
+
+
+# ---- long caches in 16 bits ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("D,H,rows", [(128, 150, 49), (64, 300, 17)])
+def test_sums_over_a_long_cache_do_not_drift(gpu, D, H, rows, fmt):
+    """So many heads that no unit is split, V of one sign: truncation of a sum kept in one accumulator over all tokens
+    would pull every output towards zero. An accumulator that takes at most 4096 tokens, 16 at a step, each step off
+    by at most 2^-23 of the sum, is off by 2^-15 of it. Roundings go either way: the results' own (at most 2^-11) over
+    D * H unlike values average to 2^-11 / sqrt(3 D H), of which six are allowed; those of the n weights are as
+    many times smaller again."""
+    n, T = 32768, 128
+    blocks = n // T
+    g = torch.Generator(device="cuda").manual_seed(50)
+    code = torch.int8 if fmt == "int8" else torch.float8_e4m3fn
+    rand = lambda lo, hi: torch.randint(lo, hi, (blocks, H, T, D), generator=g, dtype=torch.int8, device="cuda")  # noqa: E731
+    kc, vc = rand(-100, 101).float().to(code), rand(60, 121).float().to(code)
+    ks = torch.full((blocks, H), 2.0 ** -6, device="cuda")
+    vs = torch.full((blocks, H), 0.011, device="cuda")
+    cache = supra_attn.KVCache(gpu, blocks, H, D, block_tokens=T, format=fmt, k=kc, v=vc, k_scale=ks, v_scale=vs)
+    table = torch.arange(blocks, dtype=torch.int32, device="cuda").view(1, -1)
+    seqs = supra_attn.CacheBatch(gpu, torch.tensor([n], dtype=torch.int32, device="cuda"), table, max_rows=rows)
+    q = torch.randn(rows, H * D, generator=g, device="cuda").half()
+    out = torch.empty_like(q)
+    supra_attn.cache_attention(gpu, cache, seqs, q=q, H=H, out=out)
+    gpu.sync()
+    off = torch.empty(H, rows, D, dtype=torch.float64, device="cuda")
+    for h in range(H):
+        k, v = (c[:, h].float().double().reshape(n, D) for c in (kc, vc))
+        p = torch.softmax(q[:, h * D:(h + 1) * D].double() @ k.T * (2.0 ** -6 * float(np.float32(1 / np.sqrt(D)))), -1)
+        ref = p @ v * float(np.float32(0.011))
+        off[h] = (out[:, h * D:(h + 1) * D].double() - ref) / ref
+    assert off.abs().max() <= 2.0 ** -11 + 2.0 ** -12 + 2.0 ** -14  # (result, weights, sums)
+    assert abs(off.mean().item()) <= 2.0 ** -15 + 6 * 2.0 ** -11 / np.sqrt(3 * D * H)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_a_long_cache_whose_scores_rise(gpu, dtype):
+    """Largest scores and V scales that move along a cache longer than one accumulation, whole (many heads) and against
+    the 64-bit definition for some of the heads."""
+    H, D, T, n, rows = 300, 64, 128, 9000, 17
+    rng = np.random.default_rng(51)
+    blocks = -(-n // T)
+    kc = torch.from_numpy(rng.integers(-127, 128, (blocks, H, T, D)).astype(np.int8)).cuda()
+    vc = torch.from_numpy(rng.integers(-127, 128, (blocks, H, T, D)).astype(np.int8)).cuda()
+    rise = np.linspace(0.2, 3.0, blocks)[:, None]
+    ks = (rise * np.exp(0.3 * rng.standard_normal((blocks, H))) / 127).astype(np.float32)
+    vs = (np.exp2(rng.integers(-8, 9, (blocks, H))) / 127).astype(np.float32)
+    cache = supra_attn.KVCache(gpu, blocks, H, D, block_tokens=T, format="int8", k=kc, v=vc, k_scale=torch.from_numpy(ks).cuda(),
+                               v_scale=torch.from_numpy(vs).cuda())
+    table = torch.arange(blocks, dtype=torch.int32, device="cuda").view(1, -1)
+    seqs = supra_attn.CacheBatch(gpu, torch.tensor([n], dtype=torch.int32, device="cuda"), table, max_rows=rows)
+    q = torch.from_numpy(rng.standard_normal((rows, H * D)).astype(np.float32)).cuda().to(TYPES[dtype])
+    out = torch.empty_like(q)
+    supra_attn.cache_attention(gpu, cache, seqs, q=q, H=H, out=out, causal=True)
+    gpu.sync()
+    got, qn = out.cpu().double().numpy().reshape(rows, H, D), q.cpu().double().numpy().reshape(rows, H, D)
+    raw_k, raw_v = kc.cpu().numpy().view(np.uint8), vc.cpu().numpy().view(np.uint8)
+    for h in range(0, H, 37):
+        one = [np.ascontiguousarray(a[:, h:h + 1]) for a in (raw_k, ks, raw_v, vs)]
+        ref, pv, av, st, sm = oc.attention("int8", *one, qn[:, h:h + 1], [n], [0, rows], [list(range(blocks))], float(np.float32(0.125)), True)
+        assert (np.abs(got[:, h:h + 1] - ref) <= attention_bound(dtype, D, n, ref, pv, av, st, sm)).all()
