@@ -124,6 +124,8 @@ SUPRA_ATTN_API int supra_attn_tensor_alloc(supra_attn_ctx* ctx, int64_t n, float
 SUPRA_ATTN_API int supra_attn_tensor_free(supra_attn_ctx* ctx, float* dptr);
 /* fromArray / write: flushes, then copies n floats host->device (stream-ordered). */
 SUPRA_ATTN_API int supra_attn_upload(supra_attn_ctx* ctx, float* dst, const float* src, int64_t n);
+/* The same for n bytes at any address: tensors of other element types. */
+SUPRA_ATTN_API int supra_attn_upload_bytes(supra_attn_ctx* ctx, void* dst, const void* src, int64_t n);
 /* read(): flushes, copies n floats device->host and waits for them. */
 SUPRA_ATTN_API int supra_attn_download(supra_attn_ctx* ctx, float* dst, const float* src, int64_t n);
 /* Page-locked host memory for fast upload/download (freed with supra_attn_host_free). */

@@ -353,12 +353,16 @@ int supra_attn_tensor_free(supra_attn_ctx* c, float* dptr) {
 }
 
 int supra_attn_upload(supra_attn_ctx* c, float* dst, const float* src, int64_t n) {
+  return supra_attn_upload_bytes(c, dst, src, n < 0 || n > INT64_MAX / 4 ? -1 : n * 4);
+}
+
+int supra_attn_upload_bytes(supra_attn_ctx* c, void* dst, const void* src, int64_t n) {
   if (!c || n < 0 || (n > 0 && (!dst || !src))) return c ? set_err(c, SUPRA_ATTN_EINVAL, "upload: bad arguments") : 1;
   DeviceGuard g(c->device);
   int rc = do_flush(c);  // as fromArray: recorded work that reads dst runs first (app/gpu/device.js:150-157)
   if (rc) return rc;
   if (n == 0) return SUPRA_ATTN_OK;
-  cudaError_t e = cudaMemcpyAsync(dst, src, (size_t)n * 4, cudaMemcpyHostToDevice, c->stream);
+  cudaError_t e = cudaMemcpyAsync(dst, src, (size_t)n, cudaMemcpyHostToDevice, c->stream);
   return e == cudaSuccess ? SUPRA_ATTN_OK : cuda_err(c, e, "upload");
 }
 

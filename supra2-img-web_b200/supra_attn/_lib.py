@@ -133,6 +133,7 @@ SIGNATURES = [
     ("supra_attn_tensor_alloc", C.c_int, [C.c_void_p, C.c_int64, C.POINTER(C.c_void_p)]),
     ("supra_attn_tensor_free", C.c_int, [C.c_void_p, C.c_void_p]),
     ("supra_attn_upload", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64]),
+    ("supra_attn_upload_bytes", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64]),
     ("supra_attn_download", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64]),
     ("supra_attn_host_alloc", C.c_int, [C.c_void_p, C.c_int64, C.POINTER(C.c_void_p)]),
     ("supra_attn_host_free", C.c_int, [C.c_void_p, C.c_void_p]),

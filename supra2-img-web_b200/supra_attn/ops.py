@@ -134,10 +134,7 @@ class GPU:
         """from_array for the other element types; values must already be of the type (bf16: its bits)."""
         if dtype not in DTYPES:
             raise ValueError(f"dtype must be one of {sorted(DTYPES)}")
-        a = np.asarray(arr)
-        if a.size and not np.array_equal(a.astype(DTYPES[dtype]), a, equal_nan=True):
-            raise ValueError(f"from_array: values that {dtype} does not hold")
-        a = np.ascontiguousarray(a.astype(DTYPES[dtype])).reshape(-1)
+        a = _values(arr, dtype, "from_array")
         t = self.empty(list(shape) if shape is not None else [a.size], dtype)
         if t.size != a.size:
             t.release()
@@ -149,10 +146,15 @@ class GPU:
         return t
 
     def write(self, t: Tensor, arr, offset: int = 0):
-        a = np.ascontiguousarray(np.asarray(arr, dtype=np.float32)).reshape(-1)
+        """Writes the values from element `offset` on. Tensors of other types than fp32 take values that the type holds
+        (bf16: its bits)."""
+        if not t.buf:
+            raise ValueError("tensor was released")
+        a = (np.ascontiguousarray(np.asarray(arr, dtype=np.float32)).reshape(-1) if t.dtype == "fp32" else
+             _values(arr, t.dtype, "write"))
         if offset < 0 or offset + a.size > t.capacity:
             raise ValueError("write: out of bounds")
-        check(lib.supra_attn_upload(self.ctx, C.c_void_p(t.buf + 4 * offset), a.ctypes.data_as(C.c_void_p), a.size),
+        check(lib.supra_attn_upload_bytes(self.ctx, C.c_void_p(t.buf + a.itemsize * offset), a.ctypes.data_as(C.c_void_p), a.nbytes),
               self.ctx)
 
     def read(self, t, count: int | None = None) -> np.ndarray:
@@ -227,6 +229,14 @@ class GPU:
 
     def profile_reset(self):
         check(lib.supra_attn_profile_reset(self.ctx), self.ctx)
+
+
+def _values(arr, dtype: str, what: str) -> np.ndarray:
+    """The values as a flat array of the type, which has to hold them."""
+    a = np.asarray(arr)
+    if a.size and not np.array_equal(a.astype(DTYPES[dtype]), a, equal_nan=True):
+        raise ValueError(f"{what}: values that {dtype} does not hold")
+    return np.ascontiguousarray(a.astype(DTYPES[dtype])).reshape(-1)
 
 
 def _as_buf(x):
