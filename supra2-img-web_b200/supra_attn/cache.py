@@ -14,9 +14,10 @@
 Operands are Tensors of the GPU (any dtype of ops.DTYPES) or contiguous CUDA torch tensors on the GPU's
 device; strides and offsets count elements and address rows inside a buffer, as everywhere in this
 package. Calls are recorded and run at the next flush/sync/read; the GPU keeps their operands alive
-until then. lengths, table, row_start and positions are read on the device when the call runs, so they may
-be changed in place between calls and between replays of a captured flush. What is wrong in them is
-found on the device and raised by the next sync() or read().
+until then. A KVCache or CacheBatch uses its operands as they are at each call: a released one is refused.
+lengths, table, row_start and positions are read on the device when the call runs, so they may be changed in
+place (GPU.write, torch) between calls and between replays of a captured flush. What is wrong in them is found on
+the device and raised by the next sync() or read().
 """
 
 from __future__ import annotations
@@ -52,11 +53,13 @@ def _operand(gpu: GPU, x, name: str, dtypes):
         if kind in dtypes:
             return x.buf, x.capacity, kind
     else:
-        if not hasattr(x, "data_ptr"):
-            raise TypeError(f"{name}: unsupported operand type {type(x).__name__}")
+        try:
+            where = x.get_device()  # (-1: not on a GPU)
+        except AttributeError:
+            raise TypeError(f"{name}: unsupported operand type {type(x).__name__}") from None
         if not _kinds:
             _fill_kinds()
-        if x.get_device() != gpu.device:  # (-1: not on a GPU)
+        if where != gpu.device:
             raise ValueError(f"{name}: torch tensors must live on cuda:{gpu.device}")
         if not x.is_contiguous():
             raise ValueError(f"{name}: torch tensors must be contiguous")
@@ -64,6 +67,10 @@ def _operand(gpu: GPU, x, name: str, dtypes):
         if kind in dtypes:
             return x.data_ptr(), x.numel(), kind
     raise ValueError(f"{name}: must be {' or '.join(dtypes)}, not {x.dtype}")
+
+
+def _address(x):
+    return x.buf if x.__class__ is Tensor else x.data_ptr()
 
 
 def _counts(**n):
@@ -110,12 +117,19 @@ class KVCache:
             k, v, k_scale, v_scale = self._owned
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         d = Cache()
-        d.k, d.k_size, _ = _operand(gpu, k, "k", _CODES)
-        d.v, d.v_size, _ = _operand(gpu, v, "v", _CODES)
-        d.k_scale, d.k_scale_size, _ = _operand(gpu, k_scale, "k_scale", _F32)
-        d.v_scale, d.v_scale_size, _ = _operand(gpu, v_scale, "v_scale", _F32)
         d.blocks, d.block_tokens, d.H, d.D, d.format = self.blocks, self.block_tokens, self.H, self.D, FORMATS[format]
         self._desc = d
+        self._find()
+
+    def _find(self):
+        """The operands' addresses, as they are now."""
+        d, gpu = self._desc, self.gpu
+        a, d.k_size, _ = _operand(gpu, self.k, "k", _CODES)
+        b, d.v_size, _ = _operand(gpu, self.v, "v", _CODES)
+        x, d.k_scale_size, _ = _operand(gpu, self.k_scale, "k_scale", _F32)
+        y, d.v_scale_size, _ = _operand(gpu, self.v_scale, "v_scale", _F32)
+        d.k, d.v, d.k_scale, d.v_scale = a, b, x, y
+        self._at = (a, b, x, y)
 
     def release(self):
         for t in self._owned:
@@ -128,6 +142,8 @@ class KVCache:
             raise ValueError("cache was released")
         if gpu.device != self.gpu.device:
             raise ValueError("cache of another device")
+        if (_address(self.k), _address(self.v), _address(self.k_scale), _address(self.v_scale)) != self._at:
+            self._find()
         return self._desc
 
 
@@ -146,14 +162,10 @@ class CacheBatch:
     def __init__(self, gpu: GPU, lengths, table, *, max_rows: int = 1, row_start=None, rows: int | None = None,
                  max_len: int | None = None):
         s = CacheSeqs()
-        s.lengths, s.lengths_size, _ = _operand(gpu, lengths, "lengths", _INTS)
-        s.table, s.table_size, _ = _operand(gpu, table, "table", _INTS)
-        shape = tuple(table.shape)
-        if len(shape) != 2 or tuple(lengths.shape) != shape[:1]:
-            raise ValueError("lengths must be [B] and table [B, blocks]")
-        s.B, s.ld_table = shape
+        self.gpu, self._seqs = gpu, s
+        self._lengths, self._table, self._row_start = lengths, table, row_start
+        self._find()
         if row_start is not None:
-            s.row_start, s.row_start_size, _ = _operand(gpu, row_start, "row_start", _INTS)
             if rows is None:
                 raise ValueError("row_start needs rows, an upper bound of its last entry")
             s.rows = int(rows)
@@ -169,13 +181,31 @@ class CacheBatch:
         s.max_len = -1 if max_len is None else int(max_len)
         if max_len is not None and int(max_len) < 0:
             raise ValueError("max_len must not be negative")
-        self.gpu, self._seqs, self._keep = gpu, s, (lengths, table, row_start)
         self.rows = s.rows
+
+    def _find(self):
+        """The operands' addresses, as they are now."""
+        s, gpu = self._seqs, self.gpu
+        a, s.lengths_size, _ = _operand(gpu, self._lengths, "lengths", _INTS)
+        b, s.table_size, _ = _operand(gpu, self._table, "table", _INTS)
+        shape = tuple(self._table.shape)
+        if len(shape) != 2 or tuple(self._lengths.shape) != shape[:1]:
+            raise ValueError("lengths must be [B] and table [B, blocks]")
+        x = None
+        if self._row_start is not None:
+            x, s.row_start_size, _ = _operand(gpu, self._row_start, "row_start", _INTS)
+            s.row_start = x
+        s.B, s.ld_table = shape
+        s.lengths, s.table = a, b
+        self._at = (a, b, x)  # (last: after a failure the next call looks again)
 
     def _fill(self, gpu: GPU, cache: KVCache, to):
         """Copies the cache and the sequences into a descriptor."""
         if gpu.device != self.gpu.device:
             raise ValueError("batch of another device")
+        start = self._row_start
+        if (_address(self._lengths), _address(self._table), None if start is None else _address(start)) != self._at:
+            self._find()
         to.cache = cache._struct(gpu)
         to.seqs = self._seqs
         if self._seqs.max_len < 0:
@@ -193,7 +223,10 @@ def _rows_desc(gpu: GPU, cache: KVCache, seqs: CacheBatch, k, v, ldk, ldv, kOff,
     width = cache.H * cache.D
     d.ldk = width if ldk is None else int(ldk)
     d.ldv = width if ldv is None else int(ldv)
-    d.k_off, d.v_off = int(kOff), int(vOff)
+    if kOff:
+        d.k_off = int(kOff)
+    if vOff:
+        d.v_off = int(vOff)
     return d
 
 
@@ -245,12 +278,16 @@ def cache_attention(gpu: GPU, cache: KVCache, seqs: CacheBatch, *, q, H: int, ou
         width = d.H * cache.D
         d.ldq = width if ldq is None else int(ldq)
         d.ldo = width if ldo is None else int(ldo)
-        d.q_off, d.o_off = int(qOff), int(oOff)
-        d.flags = _lib.CA_CAUSAL if causal else 0
+        if qOff:
+            d.q_off = int(qOff)
+        if oOff:
+            d.o_off = int(oOff)
+        flags = _lib.CA_CAUSAL if causal else 0
         if scale is None:
-            d.flags |= _lib.CA_DEFAULT_SCALE
+            flags |= _lib.CA_DEFAULT_SCALE
         else:
             d.scale = float(scale)
+        d.flags = flags
         check(lib.supra_attn_enqueue_cache_attention(gpu.ctx, C.byref(d)), gpu.ctx)
     except Exception:
         if own:
