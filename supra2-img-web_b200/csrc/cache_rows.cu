@@ -127,7 +127,9 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant_
   else s = fmaxf(s, old);
   const float inv = 1.f / s;
   const bool again = lo > 0 && s > old;  // false when s is NaN
-  const float ratio = again ? old / s : 1.f;
+  // (a caller's own scale may be negative and larger in size than the new one: codes up to `reach` have a product that
+  // INT8 holds, the others get its largest; E4M3's conversion saturates by itself)
+  const float ratio = again ? fmaxf(old / s, -3.4028234e38f) : 1.f, reach = 127.f / fabsf(ratio);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int slot = slot0 + i * rows;
@@ -143,6 +145,10 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const __grid_constant_
       load_codes(at, u);
 #pragma unroll
       for (int k = 0; k < V / 4; ++k) decode4<FMT>(u[k], x + 4 * k);
+      if constexpr (FMT == kCacheInt8) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[k] = fminf(fmaxf(x[k], -reach), reach);
+      }
       encode_row<FMT, V>(x, ratio, u);
       store_codes(at, u);
     }

@@ -228,3 +228,25 @@ def test_a_long_cache_whose_scores_rise(gpu, dtype):
         one = [np.ascontiguousarray(a[:, h:h + 1]) for a in (raw_k, ks, raw_v, vs)]
         ref, pv, av, st, sm = oc.attention("int8", *one, qn[:, h:h + 1], [n], [0, rows], [list(range(blocks))], float(np.float32(0.125)), True)
         assert (np.abs(got[:, h:h + 1] - ref) <= attention_bound(dtype, D, n, ref, pv, av, st, sm)).all()
+
+
+# ---- held codes --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_write_beside_codes_under_a_negative_scale(gpu, fmt):
+    """A scale that no write makes is taken as the definition says: the larger one is kept, and held codes that the new
+    scale cannot express become the nearest that exist."""
+    T, H, D = 32, 6, 32
+    rng = np.random.default_rng(52)
+    p = Pool(gpu, rng, fmt, T, H, D, [20, 25])
+    for i, page in enumerate(pg for pages in p.table for pg in pages):
+        p.ks[page] = [-1.0, -0.5, -1e-3, 0.0, -3e4, 2.0]
+        p.vs[page] = [-2.0, -0.03, 1.0, -0.0, -1e30, 1e-30]
+    p.put()
+    start, seqs = p.batch([5, 9])
+    x = rng.standard_normal((14, H, D)).astype(np.float32)
+    xd = torch.from_numpy(x.reshape(14, -1)).cuda()
+    supra_attn.cache_write(gpu, p.cache, seqs, k=xd, v=xd)
+    gpu.sync()
+    for c, s in ((p.kc, p.ks), (p.vc, p.vs)):
+        oc.write(fmt, c, s, x.astype(np.float64), [20, 25], start, p.table)
+    p.check_same()
