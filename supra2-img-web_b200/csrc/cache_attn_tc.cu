@@ -955,7 +955,9 @@ cudaError_t tc_as(const CacheAttnLaunch& L, const CacheAttnPlan& P, cudaStream_t
       cudaFuncAttributes fa;
       const cudaError_t r = cudaFuncGetAttributes(&fa, kernel);
       if (r != cudaSuccess) return r;
-      if (fa.numRegs != Y::REGS) return cudaErrorInvalidConfiguration;  // the exchange of registers would not add up
+      // the exchange of registers has to add up, whatever the compiler has given the kernel (Y::REGS, as a rule)
+      if (fa.numRegs < Y::REGS_REST || fa.numRegs > Y::REGS_SOFT || Y::SOFT * Y::REGS_SOFT + 128 * Y::REGS_REST > Y::THREADS * fa.numRegs)
+        return cudaErrorInvalidKernelImage;
     }
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Y::SMEM);
   });

@@ -482,6 +482,10 @@ int flush_cache(supra_attn_ctx* c) {
           ProfScope ps(c, name, call.flops, call.bytes);
           e = launch_cache_attn(L, plan, call.type, call.format, c->stream);
         }
+        if (e == cudaErrorInvalidKernelImage) {
+          if (ws) cudaFreeAsync(ws, c->stream);
+          return set_err(c, SUPRA_ATTN_ECUDA, "%s: built with too few registers (or too many) for the exchange between its warps", name);
+        }
         if (ws) {
           const cudaError_t f = cudaFreeAsync(ws, c->stream);
           if (e == cudaSuccess) e = f;
