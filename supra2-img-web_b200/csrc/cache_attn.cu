@@ -40,6 +40,9 @@ namespace {
 constexpr int kTile = 32;  // tokens of a warp's tile
 constexpr int kStages = 2;
 constexpr float kPShift = 12.f;  // p is formed as 2^12 p: its fp16 part keeps 2^-24 of p = 1 at 2^-12
+// l and O carry that factor up to the join, so that V scales near 2^-126 lose nothing; a warp that meets one above
+// 2^90 takes it off at once, lest O pass the range of 32 bits.
+constexpr float kPUnit = 1.f / 4096.f, kScaleLarge = 1.2379400392853803e27f;
 
 __device__ __forceinline__ float ex2f(float x) {
   float y;
@@ -285,6 +288,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
 
   float o[CH][NT][4];
   float m[NT][2], l[NT][2];
+  float carry = 1.f;  // 1: l and O are 2^12 times what they stand for; kPUnit: they are not
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -373,7 +377,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
             s[a][n][e + 2 * y] = ex2f(s[a][n][e + 2 * y] - ref);
             sum += s[a][n][e + 2 * y];
           }
-        l[n][e] = l[n][e] * al[n][e] + sum;
+        l[n][e] = fmaf(l[n][e], al[n][e], sum * carry);
       }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -400,6 +404,17 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
         }
     // O^T += vscale * (V^T P^T), each block's part from a fresh accumulator
     const float vs0 = gr[0].vs, vs1 = gr[1].vs;
+    if (carry == 1.f && fmaxf(fabsf(vs0), fabsf(vs1)) > kScaleLarge) {
+      carry = kPUnit;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        l[n][0] *= carry, l[n][1] *= carry;
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[k][n][e] *= carry;
+      }
+    }
     // A block whose scale is not finite reaches only the rows that see it: the others' p and partial sum
     // are 0, and so is their factor.
     const bool odd = !(fabsf(vs0) <= 3.4028234e38f) || !(fabsf(vs1) <= 3.4028234e38f);
@@ -409,7 +424,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) vf[a][n][e] = odd && tok0 + 16 * a > lim[n][e] ? 0.f : a ? vs1 : vs0;
+        for (int e = 0; e < 2; ++e) vf[a][n][e] = odd && tok0 + 16 * a > lim[n][e] ? 0.f : (a ? vs1 : vs0) * carry;
     // Bytes after the last token may be anything, NaN codes among them, and 0 * NaN is not 0: the lane's
     // tokens 2t, 2t + 1 of each eight are the halves of its words.
     uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
@@ -463,6 +478,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
       l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
       l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
       l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
+      l[n][e] *= kPUnit / carry;
     }
   __syncthreads();  // every warp has left its ring
 
@@ -479,7 +495,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 && NT == 1 ? 3 : 1) cache_attn_
     for (int k = 0; k < CH; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        wo[(warp * NR + 8 * n + 2 * t + (e & 1)) * DT + 16 * k + 2 * g + (e >> 1)] = o[k][n][e];
+        wo[(warp * NR + 8 * n + 2 * t + (e & 1)) * DT + 16 * k + 2 * g + (e >> 1)] = o[k][n][e] * (kPUnit / carry);
     if (g == 0) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) wml[warp * NR + 8 * n + 2 * t + e] = make_float2(m[n][e], l[n][e]);

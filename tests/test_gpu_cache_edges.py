@@ -250,3 +250,17 @@ def test_write_beside_codes_under_a_negative_scale(gpu, fmt):
     for c, s in ((p.kc, p.ks), (p.vc, p.vs)):
         oc.write(fmt, c, s, x.astype(np.float64), [20, 25], start, p.table)
     p.check_same()
+
+
+# ---- values near the end of the 32-bit range ---------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("tokens,rows,top", [(90, 2, 119), (90, 140, 119), (3000, 2, 115), (3000, 140, 115), (40000, 1, 110)])
+def test_attention_of_values_near_the_end_of_the_range(gpu, tokens, rows, top, D, dtype):
+    """V of up to 2^(top + 1): its sum over the tokens, with weights up to 1, stays below 2^128. And as small ones."""
+    for size in (2.0 ** top, 2.0 ** -top):
+        def scale(p):
+            for page in p.table[0]:
+                p.vs[page] = np.float32(size) / 128 * (1 + p.vs[page] % 1)
+
+        check_bound(gpu, "int8", dtype, 64, 2, D, [tokens], [rows], False, seed=60, mutate=scale)
