@@ -777,7 +777,10 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
         move();
         const float apart = ref - high;
         float dn = 0.f;
-        if (high != -INFINITY && !(fabsf(apart) <= kNear)) dn = fabsf(apart - d) <= kSlack ? d : rintf(apart);
+        if (high != -INFINITY && !(fabsf(apart) <= kNear)) {
+          if (fabsf(apart) <= 3.4028234e38f) dn = fabsf(apart - d) <= kSlack ? d : rintf(apart);
+          else l = __uint_as_float(0x7fffffffu);  // a score that is not finite
+        }
         if (dn != d || none) l = l == 0.f ? 0.f : l * ex2f((r - ref) + (dn - d));
         else l *= al;
         *unit = d = dn;
@@ -808,7 +811,7 @@ __global__ void __launch_bounds__(Cfg<DT, sizeof(T) == 4>::THREADS, Cfg<DT, size
           }
         }
         l += sum;
-        far = __any_sync(0xffffffffu, d != 0.f || (m == -INFINITY && l != 0.f));
+        far = __any_sync(0xffffffffu, d != 0.f || (m == -INFINITY && l > 0.f));  // (not for rows of NaN)
       }
       // Every product is waited for in its turn, needed or not: a wait by parity tells a phase only from its
       // neighbours. (This one could not start before the last one's end.)

@@ -264,3 +264,30 @@ def test_attention_of_values_near_the_end_of_the_range(gpu, tokens, rows, top, D
                 p.vs[page] = np.float32(size) / 128 * (1 + p.vs[page] % 1)
 
         check_bound(gpu, "int8", dtype, 64, 2, D, [tokens], [rows], False, seed=60, mutate=scale)
+
+
+# ---- rows that are not finite ------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("D", [48, 64, 128])
+@pytest.mark.parametrize("rows", [8, 140])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_rows_of_q_that_are_not_finite_stay_alone(gpu, zeros, rows, D, dtype):
+    """The others keep their bits, whatever the cache holds."""
+    p = Pool(gpu, np.random.default_rng(61), "e4m3", 32, 1, D, [300])
+    if zeros:
+        for page in p.table[0][:3]:
+            p.vc[page] = 0
+            p.vs[page] = zero_scale("e4m3")
+        p.put()
+    _, seqs = p.batch([rows])
+    q = torch.randn(rows, D, generator=torch.Generator(device="cuda").manual_seed(D + rows), device="cuda").to(TYPES[dtype])
+    spoilt = q.clone()
+    spoilt[5] = float("nan")
+    spoilt[7, 3] = float("inf")
+    out = [torch.zeros_like(q) for _ in range(2)]
+    for x, o in zip((q, spoilt), out):
+        supra_attn.cache_attention(gpu, p.cache, seqs, q=x, H=1, out=o, causal=True)
+    gpu.sync()
+    keep = [i for i in range(rows) if i not in (5, 7)]
+    assert torch.equal(out[0][keep], out[1][keep]) and torch.isfinite(out[0]).all()
+    assert torch.isnan(out[1][5]).all() and not torch.isfinite(out[1][7]).any()
