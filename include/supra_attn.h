@@ -273,7 +273,8 @@ typedef struct supra_attn_qk_operand {
  * lays the table out once for its positions (n_turns rows), which may stand for one axis or for
  * a patch grid. position = positions[row], or the row index when positions is NULL. A position
  * outside [0, n_turns) leaves its row unwritten and is reported at sync (SUPRA_ATTN_EDEVICE).
- * Sums and products are held in 32 bits; the result is rounded once, to `type`.
+ * Sums and products are held in 32 bits (heads whose squares leave that range come out as such arithmetic has
+ * them); the result is rounded once, to `type`.
  * 1 <= D <= 256, even; 0 <= rot <= D, even (0: no rotation, turns and positions NULL). k.H = 0:
  * no keys. Recorded like an attention problem (same queue and hazard tracking). */
 typedef struct supra_attn_qk_norm_desc {
@@ -297,7 +298,8 @@ SUPRA_ATTN_API int supra_attn_check_qk_norm_desc(const supra_attn_qk_norm_desc* 
  * for V: value = code * scale[block*H + head]. Codes of one block and head are contiguous:
  *   codes[((block*H + head)*block_tokens + slot)*D + channel]
  * SUPRA_ATTN_CACHE_INT8: signed bytes in [-127, 127]; SUPRA_ATTN_CACHE_E4M3: 8-bit floats with 4
- * exponent and 3 mantissa bits. D is a multiple of 16 up to 128, block_tokens 16, 32, 64 or 128;
+ * exponent and 3 mantissa bits (the two bytes that stand for NaN are no codes, and no write makes them: what one
+ * gives at a token in use may also reach rows of its sequence that do not see the token). D is a multiple of 16 up to 128, block_tokens 16, 32, 64 or 128;
  * k and v are 16-byte aligned. All four arrays are the caller's. */
 enum { SUPRA_ATTN_CACHE_INT8 = 0, SUPRA_ATTN_CACHE_E4M3 = 1 };
 typedef struct supra_attn_cache {
@@ -369,9 +371,12 @@ SUPRA_ATTN_API int supra_attn_check_cache_read_desc(const supra_attn_cache_rows_
  * tokens (causal: up to the row's own token). H query heads, a multiple of cache.H: heads
  * g*H/cache.H .. (g+1)*H/cache.H-1 read the cache's head g. Row r, head h of the queries at
  * q[q_off + r*ldq + h*D], of the result at out[o_off + r*ldo + h*D]. A row that sees no token
- * (an empty sequence, or a causal row before the first token) is 0. The codes enter the products
- * exactly; scores, softmax statistics and the sums over tokens are held in 32 bits, and
- * SUPRA_ATTN_T_F32 requests keep FP32 accuracy (queries and probabilities as two 16-bit parts). */
+ * (an empty sequence, or a causal row before the first token) is 0. blocks*H*block_tokens is below 2^31.
+ * The codes enter the products exactly; scores, softmax statistics and the sums over tokens are held in 32
+ * bits. For the products on the tensor cores SUPRA_ATTN_T_F16 and _BF16 requests round each probability to 11
+ * bits (their queries keep all of theirs, but for BF16 channels below 2^-27 of a head's largest);
+ * SUPRA_ATTN_T_F32 requests hold queries and probabilities as two such parts, 22 bits: errors of about 4e-7 where
+ * sums in FP32 throughout have 1e-7 to 3e-7. */
 typedef struct supra_attn_cache_attn_desc {
   supra_attn_cache cache;
   supra_attn_cache_batch seqs;

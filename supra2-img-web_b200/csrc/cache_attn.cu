@@ -23,7 +23,7 @@
 // CTAs are launched without clusters, as many as fill the SMs, write their parts to a workspace that
 // lives from the launch to the join, and a second kernel joins them in order.
 //
-// Measured: 64 sequences of 1000 to 8000 tokens, 8 heads of 128, 4 query heads each, E4M3 and bf16: 118 us, 5.0 TB/s (76 %
+// Measured: 64 sequences of 1000 to 8000 tokens, 8 heads of 128, 4 query heads each, E4M3 and bf16: 120 us, 4.9 TB/s (75 %
 // of the copy rate; what is missing is the first loads of each CTA, three of which share an SM, and the last
 // wave); one sequence of 131072 tokens, INT8 and fp16: 54 us, 5.0 TB/s (49 for the
 // parts, 5.5 TB/s; the join, placed while they are formed, the rest: 57 in all when it was an ordinary launch).

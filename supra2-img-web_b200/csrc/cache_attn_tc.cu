@@ -21,7 +21,7 @@
 // 16-bit rows keep O in TMEM, where m moves only when a tile exceeds it by 2^8 (then the softmax threads
 // rescale O there). Sums in TMEM are truncated, which pulls them towards zero by up to 2^-23 for each 16 tokens (measured
 // 2e-4 at 32768 tokens, half a rounding of fp16): after every 4096 tokens O joins a sum that is rounded to nearest, in local
-// memory, and starts anew (32768 tokens: 2.3e-5). fp32 rows use two fp16 parts of q and p (each product two MMAs), move m exactly, and
+// memory, and starts anew (32768 tokens: 2e-5). fp32 rows use two fp16 parts of q and p (each product two MMAs), move m exactly, and
 // add each tile's product to O in fp32 registers, rounded to nearest, so that the error does not grow
 // with the number of tiles.
 //
@@ -30,11 +30,14 @@
 // move registers from the converters to the softmax threads. K, V and their raw bytes have two stages
 // each, and so has S: a row tile's next scores are formed while its softmax threads work on the present
 // ones, and its last product behind them, so that neither MMA nor conversion is waited for. What bounds
-// the kernel is the softmax: 16 exponentials per cycle and SM, and about five instructions a score.
+// a CTA is the softmax: 16 exponentials per cycle and SM, and about five instructions a score (the busiest SM issues
+// in 65 % of its slots). What bounds a launch of few unlike CTAs is their distribution:
 // Measured: 4 causal chunks of 700 to 1024 rows over 2049 to 4096 tokens, 16 heads of 128, 4 cache heads, INT8 and bf16:
-// 146 us, 517 TFLOP/s; 128 prompts of 1 to 128 tokens, 256 rows each, 9 heads of 64, INT8 and fp32 rows: 90 us,
+// 138 us, 549 TFLOP/s: 220 CTAs of up to 64 tiles, one an SM, leave the 148 SMs idle for a third of the time (94 tiles on
+// the last, 64 in the mean). 128 prompts of 1 to 128 tokens, 256 rows each, 9 heads of 64, INT8 and fp32 rows: 88 us,
 // 1.8 TB/s (a CTA has two tiles at most; its q, its output and the latencies between take the time). A fourth
-// converter warp did not change the first.
+// converter warp did not change the first. FP32 rows of more than 64 channels spill registers (about 670 bytes a thread:
+// O takes 128 of 208): 8 sequences of 300 to 512 causal rows over 1024 to 2048 tokens, 8 heads of 128: 139 us.
 // Every wait is bounded; on a timeout the CTA records the failure, waits for its own copies and MMAs, frees its
 // TMEM and leaves.
 #include <algorithm>
