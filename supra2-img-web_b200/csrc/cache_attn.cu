@@ -747,13 +747,13 @@ CacheAttnPlan plan_cache_attn(const CacheAttnArgs& L, int type) {
   // The tensor-core kernel pads a unit to 128 or 256 rows, this file's reads and converts the cache again for
   // every 16 rows, which costs nothing as long as its CTAs all run at once. Rows kernel / tensor cores, us:
   //                                              16 rows      32           48           64
-  //   128 sequences of 128, 9 heads of 64, bf16  34 / 39      57 / 39                   100 / 39
-  //   the same, fp32                             39 / 47      70 / 49      98 / 49      127 / 49
-  //   1 of 512, 4 heads of 64, fp32                           14 / 21      14 / 21      14 / 21
-  //   2 of up to 899, 9 heads of 32, fp16                                               (80: 16 / 21)
-  //   64 of 2048, 8 heads of 128, bf16           131 / 209    162 / 209    229 / 211    279 / 211
-  //   4 of 8192, 8 heads of 128, bf16                         49 / 68      86 / 68      88 / 70
-  //   64 of 2048, 8 heads of 128, fp32           132 / 460    234 / 467                 320 / 467 (96: 472 / 469)
+  //   128 sequences of 128, 9 heads of 64, bf16  35 / 39      57 / 39                   100 / 39
+  //   the same, fp32                             39 / 47      70 / 49      100 / 49     131 / 49
+  //   1 of 512, 4 heads of 64, fp32                           16 / 20      17 / 20      17 / 21
+  //   2 of up to 899, 9 heads of 32, fp16                                               (80: 18 / 25)
+  //   64 of 2048, 8 heads of 128, bf16           90 / 195     156 / 197    229 / 197    281 / 197
+  //   4 of 8192, 8 heads of 128, bf16                         49 / 58      87 / 60      88 / 60
+  //   64 of 2048, 8 heads of 128, fp32           102 / 451    193 / 455                 334 / 459 (96: 512 / 459)
   P.tc = rows > (L.c.D > 64 ? (type == kTypeF32 ? 64 : 48) : units16 > 2 * 148 ? 16 : 128);
   P.nr = P.tc ? cache_attn_tc_rows(L.c.D) : rows > 8 ? 16 : 8;
   P.tiles = (int)((rows + P.nr - 1) / P.nr);
@@ -764,8 +764,8 @@ CacheAttnPlan plan_cache_attn(const CacheAttnArgs& L, int type) {
   const int64_t wide = std::min<int64_t>(wave / std::max<int64_t>(P.units, 1), L.s.max_len / (P.tc ? 256 : 512));
   if (P.tc) {
     // Split units of many tiles, joined by a second launch (us whole / split):
-    //   4 units of 2048 tokens, D 64: 41 / 23      18 of 1024, D 64: 31 / 25       18 of 512: 20 / 21
-    //   72 of 1024, D 64: 27 / 29                  64 of 4096, D 128: 102 / 74     16 of 8192, D 128: 180 / 49
+    //   4 units of 2048 tokens, D 64: 39 / 19      18 of 1024, D 64: 29 / 21       18 of 512: 21 / 20
+    //   72 of 1024, D 64: 25 / 25                  64 of 4096, D 128: 94 / 68      16 of 8192, D 128: 175 / 45
     // Of units that just run at once, two parts each shorten the longest sequence's way: 200 of up to 4433 tokens, D
     // 48: 92 / 72, 126 of up to 4412, D 96: 105 / 78; 144 of 4096 each, D 64: 90 / 82. (256 units at one CTA an SM, D
     // 128: 152 / 184.)
